@@ -52,6 +52,10 @@ SIGNATURES = {
     "rda_rms_norm_head": (_i, [_p, _p, _p, _i, _i, _i, _i, _l, _l, _l, _f, _p]),
     "rda_rms_norm_row": (_i, [_p, _p, _p, _i, _i, _i, _i, _l, _l, _l, _f, _p]),
     "rda_rms_norm_rope": (_i, [_p, _p, _p, _i, _i, _i, _i, _l, _l, _l, _f, _p, _l, _p]),
+    "rda_rotate_positions": (_i, [_p, _p, _p, _i, _p, _f, _i, _i, _p, _p]),
+    "rda_paged_append": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _p, _p]),
+    "rda_paged_attn_workspace": (_sz, [_l, _l, _l, _l, _l, _i]),
+    "rda_paged_attn": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _f, _f, _i, _i, _i, _p, _p]),
 }
 
 _lib = None

@@ -195,6 +195,40 @@ int rda_rms_norm_row(const void* x, const float* w, void* y, int B, int H, int L
 int rda_rms_norm_rope(const void* x, const float* w, void* y, int B, int H, int L, int D, long sb, long sh, long sl, float eps, const float* freqs,
                       long fb, void* stream);
 
+/* ------------------------------------------------------------------ paged cache -------- */
+/* No counterparts in the reference. `type`: 0 fp16, 1 bf16, 2 fp32. Sizes and element strides are host arrays, read during the call;
+ * every base address and stride is a multiple of 16 bytes (1 otherwise), last dimensions are contiguous. Table entries, starts and
+ * lengths are read on the device, so that captured launches follow their contents; whatever they hold, no kernel reads or writes
+ * outside the tensors. */
+
+/* Rotary positions: x, y (B, L, H, D), positions [B, L] (int32, or int64 with wide = 1), turns [R / 2]: frequencies in turns per
+ * position. Pair i of a head -- values i and i + R / 2, or 2 i and 2 i + 1 with flags & 1 -- turns by 2 pi position turns[i] (flags & 2:
+ * by the negative angle), times factor; values from R on are copied. dims: B, L, H, D, R, strides (b, l, h) of x, of y. D and R
+ * are multiples of 16, R <= D <= 256. y may be x. */
+int rda_rotate_positions(const void* x, void* y, const void* positions, int wide, const double* turns, float factor, int flags, int type,
+                         const long* dims, void* stream);
+
+/* Appends to a paged cache: k, v (T, Hkv, D) of `type` to k_pages, v_pages (P, S, Hkv, D) of `cache_type`, and q (T, H, D) to q_out of
+ * cache_type (H = 0: none). Row t of sequence b (starts[b] <= t < starts[b + 1]) has position n = lengths[b] - starts[b + 1] + t and
+ * goes to row n % S of page table[b, n / S]; k and q turn by n as in rda_rotate_positions (R = 0: not). dims: T, H, Hkv, D, R, B,
+ * N (table entries per sequence), the table's row pitch, P, S, strides (t, h) of q, k, v, q_out, and (page, row, head) of
+ * k_pages, v_pages. Nothing is written for rows of no sequence, nor to the cache where n or its page does not exist. */
+int rda_paged_append(const void* q, const void* k, const void* v, void* q_out, void* k_pages, void* v_pages, const int* table, const int* starts,
+                     const int* lengths, const double* turns, float factor, int interleaved, int type, int cache_type, const long* dims,
+                     void* stream);
+
+/* Attention of rows q (T, H, D) over a paged cache as appended to, D 64 or 128, all of one type: row t of sequence b, at position n as
+ * above, sees keys j < min(lengths[b], N S) with j <= n (window > 0: and n - j < window), or j < prefix[b] (prefix NULL: none). Scores
+ * are scale q.k; with softcap > 0, softcap tanh(scale q.k / softcap); with slopes [H] (or NULL), less slopes[h] |n - j|. Rows that see
+ * nothing are 0; rows of no sequence are left as they were, or set to 0 with fill = 1. At most 8192 sequences. dims: T, H, Hkv, D, B,
+ * N, the table's row pitch, P, S, strides (t, h) of q, of out, and (page, row, head) of k_pages, v_pages. workspace:
+ * rda_paged_attn_workspace bytes of the same sizes, its contents of no account before and after; calls that overlap take one each.
+ * A row's last bits depend on the batch that it is computed in (its sums are cut where the batch's work is). */
+size_t rda_paged_attn_workspace(long T, long B, long H, long Hkv, long D, int type);
+int rda_paged_attn(const void* q, void* out, const void* k_pages, const void* v_pages, const int* table, const int* starts, const int* lengths,
+                   const int* prefix, const float* slopes, void* workspace, float scale, float softcap, int window, int fill, int type,
+                   const long* dims, void* stream);
+
 /* ------------------------------------------------------------------ calibration -------- */
 /* Measurement only, no counterpart in the reference: `blocks` workgroups of four waves each issue `iters` rounds of
  * 8 independent MFMAs (int8 = 1: v_mfma_i32_32x32x32_i8, 65536 ops each; int8 = 0: v_mfma_f32_32x32x16_f16, 32768
