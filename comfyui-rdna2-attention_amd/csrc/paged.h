@@ -3,6 +3,7 @@
 #include "common.h"
 
 typedef __bf16 bf16_t;
+typedef bf16_t b2 __attribute__((ext_vector_type(2)));
 typedef bf16_t b8 __attribute__((ext_vector_type(8)));
 typedef float f8 __attribute__((ext_vector_type(8)));
 

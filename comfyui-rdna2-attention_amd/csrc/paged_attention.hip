@@ -74,6 +74,17 @@ __device__ __forceinline__ WorkTile make_tile(const PagedArgs& p, int b, int j) 
     return t;
 }
 
+// The same in every lane, which the compiler does not see of values that come from memory: in scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+template <class X>
+__device__ __forceinline__ const X* uniform(const X* p) {
+    const unsigned long long u = (unsigned long long)p;
+    return (const X*)((unsigned long long)(u32)uniform((int)(u >> 32)) << 32 | (u32)uniform((int)u));
+}
+__device__ __forceinline__ WorkTile uniform(WorkTile t) {
+    return {uniform(t.first), uniform(t.rows), uniform(t.r0), uniform(t.r1), uniform(t.p0), uniform(t.keys), uniform(t.prefix), uniform(t.lo), uniform(t.hi), uniform(t.units)};
+}
+
 // Inclusive sums over the workgroup's NT values; red holds NT / 64 sums.
 template <int NT>
 __device__ __forceinline__ u32 scan_block(u32 x, u32* red) {
@@ -161,13 +172,13 @@ __device__ Run find_run(const PagedArgs& p, int* smem, u32* shared, int block) {
         }
     }
     __syncthreads();
-    run.kvh = head;
-    run.b = __builtin_amdgcn_readfirstlane(shared[0]);
-    run.j = __builtin_amdgcn_readfirstlane(shared[1]);
-    run.unit = __builtin_amdgcn_readfirstlane(shared[2]);
-    run.tiles = __builtin_amdgcn_readfirstlane(shared[3]);
-    run.count = run.tiles ? (int)min((unsigned long long)quota, total - u0) : 0;  // no tiles: sums past 32 bits (starts that fall)
-    run.quota = quota;
+    run.kvh = uniform((int)head);
+    run.b = uniform((int)shared[0]);
+    run.j = uniform((int)shared[1]);
+    run.unit = uniform((int)shared[2]);
+    run.tiles = uniform((int)shared[3]);
+    run.count = run.tiles ? uniform((int)min((unsigned long long)quota, total - u0)) : 0;  // no tiles: sums past 32 bits (starts that fall)
+    run.quota = (u32)uniform((int)quota);
     __syncthreads();
     return run;
 }
@@ -185,7 +196,7 @@ __device__ __forceinline__ void next_tile(const PagedArgs& p, Run& run) {
             }
         }
         int first;
-        run.tiles = (seq_rows(p, run.b, first) + MT - 1) / MT;
+        run.tiles = uniform((seq_rows(p, run.b, first) + MT - 1) / MT);
     } while (run.tiles == 0);  // ends: the run has units left, so a tile exists
 }
 
@@ -270,7 +281,7 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
     Cut cut = {};
 
     while (run.count > 0) {
-        const WorkTile w = make_tile<MT, UK>(p, run.b, run.j);
+        const WorkTile w = uniform(make_tile<MT, UK>(p, run.b, run.j));
         const int u0 = run.unit, u1 = min(w.units, u0 + run.count), n = u1 - u0;
         const bool whole = u0 == 0 && u1 == w.units;
         const int* table = p.table + run.b * p.pitch;
@@ -291,7 +302,7 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
             pre[m] = row <= w.r1 ? w.prefix : 0;
             slope[m] = MOD && p.slopes ? p.slopes[head] * LOG2E : 0.f;
         }
-        const int n0 = w.p0 + div_by(w.r0, p.G), n1 = w.p0 + div_by(w.r1, p.G);
+        const int n0 = uniform(w.p0 + div_by(w.r0, p.G)), n1 = uniform(w.p0 + div_by(w.r1, p.G));
 
         f4 o[MB][VH][VC];
         float m_[MB], l_[MB];
@@ -611,6 +622,495 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
     if (t == 0) ((Cut*)p.ws)[block] = cut;
 }
 
+// ------------------------------------------------------------------------------------------------ many rows
+
+// Tiles kernel (fp16, bf16): tiles of 128 rows, 32 to each of four waves, which share 32-key tiles of K and V in LDS. Bound by the
+// matrix products and the exponentials beside them, as the fused attention of fixed shapes (attention.hip), whose tile layouts and
+// step order it has: S^T = K Q^T and O^T = V^T P^T in 32x32 blocks, a lane's registers all of its own row (lane % 32; the lane
+// 32 on has the row's other keys); three stages filled by 16-byte global->LDS copies two tiles ahead; step i computes tile i + 1's scores
+// beside tile i's second half of exponentials, then tile i's product with V beside tile i + 1's first half. What differs:
+//
+// * A copy's rows come from pages. A wave's copy has 4 rows (D = 64: 8) of a tile, in one page where the page size is a multiple of 8:
+//   its base is then scalar, else each lane has its own. Table entries are fetched one step before the copies they are for, and have
+//   arrived by the barrier that ends it.
+// * Tiles at the ends of what the wave's rows see are masked, by a branch that the other tiles skip. Scores are replaced by -inf, and m
+//   starts at -1e30, so that a row without keys so far has P = 0.
+// * Keys past the sequence's end are copies of its last row, and those on pages that the cache does not have rows of page 0; masked
+//   tiles whose values are not all finite add them key by key to the rows that see them.
+template <int D>
+struct TilesLds {
+    static constexpr int ROW = 2 * D, TILE = 32 * ROW, V = 3 * TILE;  // K stages, V stages
+    // find_run's tile sums before them and the rows turned around after them (32 x 256 bytes a wave) lie in the same place; then find_run's words.
+    static constexpr int SHARED = 6 * TILE > 33024 ? 6 * TILE : 33024;
+    static_assert(SHARED >= 4 * (MAX_SEQUENCES + 1) && SHARED >= 4 * 32 * 256 && SHARED % 256 == 0);
+    static constexpr int BYTES = SHARED + (256 + 16) * 4;
+};
+typedef __fp16 tr_t __attribute__((__vector_size__(4 * sizeof(__fp16))));
+typedef __attribute__((address_space(3))) tr_t lds_tr_t;
+typedef __attribute__((address_space(3))) u4v lds_u4v_t;
+__device__ __forceinline__ u4v lds_u4(u32 addr) { return *(const lds_u4v_t*)(size_t)addr; }
+__device__ __forceinline__ u2v lds_tr(u32 addr) { return __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr_t*)(size_t)addr)); }
+__device__ __forceinline__ f2 both_halves(float x) {  // x of the lane's row from lanes 0-31, and from lanes 32-63
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return (f2){__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+template <class T>
+__device__ __forceinline__ f16v product32(const u4v& a, const u4v& b, const f16v& c) {
+    if constexpr (std::is_same<T, half_t>::value) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+// Two values rounded to T as one word, and the sum of a word's two values added to l.
+template <class T>
+__device__ __forceinline__ u32 pair_of(float a, float b) {
+    if constexpr (std::is_same<T, half_t>::value) return __builtin_bit_cast(u32, __builtin_convertvector((f2){a, b}, h2));
+    else return __builtin_bit_cast(u32, __builtin_convertvector((f2){a, b}, b2));
+}
+template <class T>
+__device__ __forceinline__ float add_pair(u32 w, float l) {
+    if constexpr (std::is_same<T, half_t>::value) return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), (h2){(_Float16)1.f, (_Float16)1.f}, l, false);
+    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), (b2){(bf16_t)1.f, (bf16_t)1.f}, l, false);
+}
+
+// The lane's number, read again where a rare branch needs it, so that the tile loop holds no registers for it.
+__device__ __forceinline__ int lane_again() {
+    int x;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+    return x;
+}
+
+template <class T, int D, bool MOD, bool RUNS>
+__global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs p) {
+    constexpr int MT = 128, UK = 32, ROW = 2 * D, KS = D / 16, DT = D / 32;  // KS: products of a score block; DT: of a 16-key step with V
+    constexpr int CP = D / 64, CR = 1024 / ROW;  // a wave's copies of K per tile; rows of a copy
+    using L = TilesLds<D>;
+    extern __shared__ __attribute__((aligned(256))) char smem[];
+    const int lane = threadIdx.x & 63, g = lane >> 5, lq = lane & 31;
+    const int wave = uniform((int)(threadIdx.x >> 6));
+    const int block = work_block(p.grid);
+    Run run = find_run<MT, UK, 256>(p, (int*)smem, (u32*)(smem + L::SHARED), block);
+    int* flag = (int*)(smem + L::SHARED) + 256 + 8;
+    Cut cut = {};
+    const u32 smem_u = lds_addr(smem);
+
+    while (run.count > 0) {
+        const WorkTile w = uniform(make_tile<MT, UK>(p, run.b, run.j));
+        const int u0 = run.unit, u1 = min(w.units, u0 + run.count), n = w.hi > w.lo ? u1 - u0 : 0;
+        const bool whole = u0 == 0 && u1 == w.units;
+        const int* table = uniform(p.table + run.b * p.pitch);
+        const T* kbase = uniform((const T*)p.k + run.kvh * p.kph);
+        const T* vbase = uniform((const T*)p.v + run.kvh * p.vph);
+        const int key_first = w.lo + u0 * UK;
+        auto key_of = [&](int i) __attribute__((always_inline)) { return key_first + i * UK; };
+        const int wr0 = w.r0 + 32 * wave;  // the wave's first row
+        const bool active = wr0 <= w.r1;
+        const int n0 = uniform(w.p0 + div_by(min(wr0, w.r1), p.G)), n1 = uniform(w.p0 + div_by(min(wr0 + 31, w.r1), p.G));
+
+        // Copies. Copy c of a tile: rows CR (4 c + wave) .. + CR - 1, the lane's row at + lane / (D / 8); the 16-byte chunks of a row are
+        // permuted in LDS so that reads hit distinct banks: K chunk x of row r at x ^ (r & 15) (D = 64: x ^ (r / 2 & 7)), V chunk at
+        // x ^ 4 (r & 3) (D = 64: x ^ 4 (r / 2 & 1)). Copies 1 differ from copies 0 by rows of a multiple of 16: by the base alone.
+        auto k_chunk = [](int ln, int r) __attribute__((always_inline)) { return (ln % (D / 8)) ^ (D == 128 ? r & 15 : r >> 1 & 7); };
+        auto v_chunk = [](int ln, int r) __attribute__((always_inline)) { return (ln % (D / 8)) ^ (D == 128 ? (r & 3) << 2 : (r >> 1 & 1) << 2); };
+        const int my_row = CR * wave + lane / (D / 8);
+        u32 k_off = (u32)(lane / (D / 8) * (int)p.kpr * 2 + k_chunk(lane, my_row) * 16), v_off = (u32)(lane / (D / 8) * (int)p.vpr * 2 + v_chunk(lane, my_row) * 16);
+        int id[CP];  // table entries of the tile to be copied next: of the lane's rows
+        auto fetch = [&](int i) __attribute__((always_inline)) {
+            const int ln = lane_again();
+#pragma unroll
+            for (int c = 0; c < CP; c++) id[c] = table[div_by(min(key_of(i) + CR * (4 * c + wave) + ln / (D / 8), w.hi - 1), p.S)];
+        };
+        auto issue = [&](int i, int stage) __attribute__((always_inline)) {
+            const int ln = lane_again();
+#pragma unroll
+            for (int c = 0; c < CP; c++) {
+                const int r = CR * (4 * c + wave), lr = r + ln / (D / 8), key = min(key_of(i) + lr, w.hi - 1), kr = key - div_by(key, p.S) * (int)p.S.d;
+                const long at = (u32)id[c] < (u32)p.P ? id[c] : 0;
+                dma16_at(kbase + at * p.kpp + kr * p.kpr + k_chunk(ln, lr) * 8, smem + stage * L::TILE + r * ROW);
+                dma16_at(vbase + at * p.vpp + kr * p.vpr + v_chunk(ln, lr) * 8, smem + L::V + stage * L::TILE + r * ROW);
+            }
+        };
+        // The same for a tile without an end and with none but pages that exist, whose rows of a copy lie in one page (RUNS).
+        auto fetch_plain = [&](int i) __attribute__((always_inline)) {
+            if constexpr (!RUNS) fetch(i);
+            else
+#pragma unroll
+                for (int c = 0; c < CP; c++) id[c] = table[div_by(key_of(i) + CR * (4 * c + wave), p.S)];
+        };
+        auto issue_plain = [&](int i, int stage) __attribute__((always_inline)) {
+            if constexpr (!RUNS) issue(i, stage);
+            else
+#pragma unroll
+                for (int c = 0; c < CP; c++) {
+                    const int r = CR * (4 * c + wave), key = key_of(i) + r, kr = key - div_by(key, p.S) * (int)p.S.d;
+                    const long page = uniform(id[c]);
+                    dma16(uniform(kbase + page * p.kpp + kr * p.kpr), k_off, smem + stage * L::TILE + r * ROW);
+                    dma16(uniform(vbase + page * p.vpp + kr * p.vpr), v_off, smem + L::V + stage * L::TILE + r * ROW);
+                }
+        };
+        bool holes = false;  // whether the cache lacks any page of the run's part
+        if (n > 0) {
+            int first[CP];
+            fetch(0);
+#pragma unroll
+            for (int c = 0; c < CP; c++) first[c] = id[c];
+            fetch(min(1, n - 1));
+            const int e0 = div_by(key_first, p.S), e1 = div_by(min(key_first + n * UK, w.hi) - 1, p.S);
+            bool hole = false;
+            for (int e = e0 + (int)threadIdx.x; e <= e1; e += 256) hole |= (u32)table[e] >= (u32)p.P;
+            if (threadIdx.x == 0) *flag = 0;
+            __syncthreads();
+            if (hole) *flag = 1;
+            int second[CP];
+#pragma unroll
+            for (int c = 0; c < CP; c++) second[c] = id[c], id[c] = first[c];
+            issue(0, 0);
+#pragma unroll
+            for (int c = 0; c < CP; c++) id[c] = second[c];
+            if (n > 1) issue(1, 1);
+            if (n > 2) fetch(2);
+        }
+
+        f16v o[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] = (f16v){};
+        float m = -1e30f, l = 0.f, l_old = 0.f;
+
+        if (!active) {  // no rows: the wave copies its part
+            if (n > 0) {
+                wait_copies();
+                __syncthreads();
+            }
+            for (int i = 0; i < n; i++) {
+                if (i + 2 < n) {
+                    issue(i + 2, (i + 2) % 3);
+                    if (i + 3 < n) fetch(i + 3);
+                }
+                wait_copies();
+                __syncthreads();
+            }
+        } else {
+            // Q as the B operand of S^T = K Q^T.
+            u4v qf[KS];
+            float slope = 0.f;
+            int pos = 0;
+            {
+                const int row = min(wr0 + lq, w.r1), token = div_by(row, p.G), head = run.kvh * (int)p.G.d + row - token * (int)p.G.d;
+                const T* src = (const T*)p.q + (long)(w.first + token) * p.sqt + head * p.sqh;
+#pragma unroll
+                for (int x = 0; x < KS; x++) qf[x] = *(const u4v*)(src + (2 * x + g) * 8);
+#pragma unroll
+                for (int x = 0; x < KS; x++) asm volatile("" : "+v"(qf[x]));  // the loads complete here, not inside the tile loop
+                if constexpr (MOD) {
+                    if (p.slopes) slope = p.slopes[head] * LOG2E;
+                    pos = w.p0 + token;
+                }
+            }
+            // The lane's K reads: row lq, chunk 2 x + g, at k_base ^ 32 x. Its V^T reads: lane i of 16 reads 8 bytes of row 4 g + i / 4 and gets the
+            // transposed values; chunk 4 d on of the row at v_base ^ 64 d.
+            u32 k_base = smem_u + (u32)(lq * ROW + ((g ^ (D == 128 ? lq & 15 : lq >> 1 & 7)) << 4));
+            u32 v_base;
+            {
+                const int sg = lane & 15, vr = 4 * g + (sg >> 2), c = 2 * (lane >> 4 & 1) + (sg >> 1 & 1);
+                v_base = smem_u + (u32)(L::V + vr * ROW + (sg & 1) * 8 + ((c ^ (D == 128 ? (vr & 3) << 2 : (vr >> 1 & 1) << 2)) << 4));
+            }
+            asm volatile("" : "+v"(k_base), "+v"(v_base));
+
+            auto qk = [&](auto stage, float (&out)[16], auto&& hook) __attribute__((always_inline)) {
+                const u32 st = (u32)((int)stage * L::TILE);
+                u32 kb = k_base;
+                asm volatile("" : "+v"(kb));
+                f16v acc = {};
+                u4v ka[KS / 2];
+#pragma unroll
+                for (int x = 0; x < KS / 2; x++) ka[x] = lds_u4((kb ^ (u32)(32 * x)) + st);
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 0; x < KS; x++) {
+                    acc = product32<T>(ka[x % (KS / 2)], qf[x], acc);
+                    if (x < KS / 2) ka[x] = lds_u4((kb ^ (u32)(32 * (KS / 2 + x))) + st);
+                    hook(x);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int r = 0; r < 16; r++) out[r] = acc[r];
+            };
+            // Register r of a lane: key 8 (r / 4) + 4 g + r % 4 of the tile. See: bit r set where the lane's row sees it.
+            auto see_key = [&](int key, int at) __attribute__((always_inline)) {
+                bool ok = key < w.hi && ((key <= at && (p.window <= 0 || at - key < p.window)) || key < w.prefix);
+                if (ok && holes) ok = (u32)table[div_by(key, p.S)] < (u32)p.P;
+                return ok;
+            };
+            auto position_again = [&](int ln) __attribute__((always_inline)) { return w.p0 + div_by(min(wr0 + (ln & 31), w.r1), p.G); };
+            auto bias = [&](float (&x)[16], int key0) __attribute__((always_inline)) {
+                if constexpr (MOD) {
+                    const float d0 = (float)(pos - key0 - 4 * g);
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        float y = x[r] * p.scale;
+                        if (p.cap > 0.f) y = capped<false>(y, p.cap);
+                        x[r] = __builtin_fmaf(-slope, fabsf(d0 - (float)(8 * (r >> 2) + (r & 3))), y);
+                    }
+                }
+            };
+            const float scale = MOD ? 1.f : p.scale;
+            float s[16];
+            u4v pf[2];  // P of the two 16-key steps
+            // Part k (of eight) of the P of scores x: registers 2 k, 2 k + 1.
+            auto exps_into = [&](const float (&x)[16], int k, u4v& d) __attribute__((always_inline)) {
+                const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * k], scale, -m)), b = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * k + 1], scale, -m));
+                const u32 word = pair_of<T>(a, b);
+                l = add_pair<T>(word, l);
+                d[k & 3] = word;
+            };
+            auto exps = [&](int k) __attribute__((always_inline)) { exps_into(s, k, pf[k >> 2]); };
+            auto exps_to = [&](const float (&x)[16], int k, u4v& d) __attribute__((always_inline)) {
+                exps_into(x, k, d);
+                asm volatile("" : "+v"(d), "+v"(l));
+            };
+            auto no_hook = [](int) {};
+            // m moves only where a tile's maximum exceeds it by more than 8.
+            auto move_max = [&]() __attribute__((always_inline)) {
+                float mx = s[0];
+#pragma unroll
+                for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[r]);
+                const f2 h = both_halves(mx);
+                mx = fmaxf(h[0], h[1]) * scale;
+                if (__any(mx > m + 8.f)) {
+                    const float mn = mx > m + 8.f ? mx : m, a = __builtin_amdgcn_exp2f(m - mn);
+                    m = mn;
+                    l *= a;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) o[d] *= a;
+                }
+            };
+            auto read_v = [&](u32 vb, u32 st, int j, int d) __attribute__((always_inline)) {
+                const u32 at = (vb ^ (u32)(64 * d)) + st + 16 * j * ROW;
+                return __builtin_shufflevector(lds_tr(at), lds_tr(at + 8 * ROW), 0, 1, 2, 3);
+            };
+            auto pv = [&](auto stage, auto&& hook) __attribute__((always_inline)) {
+                const u32 st = (u32)((int)stage * L::TILE);
+                u32 vb = v_base;
+                asm volatile("" : "+v"(vb));
+                u4v va[DT];
+#pragma unroll
+                for (int d = 0; d < DT; d++) va[d] = read_v(vb, st, 0, d);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    o[d] = product32<T>(va[d], pf[0], o[d]);
+                    va[d] = read_v(vb, st, 1, d);
+                    hook(d);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    o[d] = product32<T>(va[d], pf[1], o[d]);
+                    hook(DT + d);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+
+            // Tiles all of whose keys all of the wave's rows see: full0 .. full1 - 1; tiles of the run without an end: .. ends - 1.
+            int full0 = 0, full1 = 0;
+            const int ends = min(n, (w.hi - key_first) / UK);
+
+            // One tile from its scores on, wherever it lies: scores, maximum, P, product, one after the other. Leaves nothing pending.
+            auto plain_step = [&](int i) __attribute__((always_inline)) {
+                const int key0 = key_of(i), stage = i % 3;
+                const bool masked = i < full0 || i >= full1;
+                qk(stage, s, no_hook);
+                bias(s, key0);
+                u32 see = 0xffff;
+                if (masked) {
+                    const int ln = lane_again(), at = position_again(ln);
+                    see = 0;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const bool ok = see_key(key0 + 8 * (r >> 2) + 4 * (ln >> 5) + (r & 3), at);
+                        if (!ok) s[r] = -__builtin_inff();
+                        see |= ok ? 1u << r : 0;
+                    }
+                }
+                move_max();
+#pragma unroll
+                for (int k = 0; k < 8; k++) exps(k);
+                if (masked) {
+                    // Values that are not finite, of keys that only some rows see: key by key.
+                    const u32 st = (u32)(stage * L::TILE);
+                    bool odd = false;
+                    constexpr u32 E = std::is_same<T, half_t>::value ? 0x7c00u : 0x7f80u;
+#pragma unroll
+                    for (int x = 0; x < L::TILE / 1024; x++) {
+                        const u4v v = lds_u4(smem_u + L::V + st + x * 1024 + lane * 16);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) odd |= (v[e] & E) == E || (v[e] >> 16 & E) == E;
+                    }
+                    if (__any(odd)) {
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+#pragma unroll
+                            for (int d = 0; d < DT; d++) {
+                                const u4v v = read_v(v_base, st, j, d);
+#pragma unroll 1
+                                for (int kk = 0; kk < 16; kk++) {  // value (kk & 3) + kk / 8 x 4 of the lanes with g = kk / 4 & 1: register 8 j + that
+                                    const int e0 = (kk >> 3) * 4 + (kk & 3);
+                                    u4v one;
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) one[e] = (kk >> 2 & 1) == g && e0 >> 1 == e ? v[e] & (kk & 1 ? 0xffff0000u : 0xffffu) : 0;
+                                    const f16v x = product32<T>(one, pf[j], (f16v){});
+                                    if (__shfl(see >> (8 * j + e0) & 1, (kk >> 2 & 1) * 32 + lq)) o[d] += x;
+                                }
+                            }
+                        return;
+                    }
+                }
+                pv(stage, no_hook);
+            };
+            // Steps of KS (or 2 DT = KS) products: the four parts of half a tile's exponentials beside every (KS / 4)-th.
+            auto beside = [](int x) __attribute__((always_inline)) { return x % (KS / 4) == KS / 4 - 1; };
+            // A step of the full tiles: tile i's scores are in s, its P's first half in pf[0] and l; tile i + 1 is full too. P is first made
+            // with the m at hand; a lane's sum that grew by no more than 64 proves that no P was above it, else the scores are made
+            // again from the tile in LDS, the maximum taken, and P with it.
+            auto settle = [&](auto stage, int i) __attribute__((always_inline)) {
+                if (__builtin_expect(__any(!(l <= l_old + 64.f)), 0)) {
+                    qk(stage, s, no_hook);
+                    bias(s, key_of(i));
+                    l = l_old;
+                    move_max();
+#pragma unroll
+                    for (int k = 0; k < 8; k++) exps(k);
+                }
+            };
+            auto full_step = [&](int i, auto stage) __attribute__((always_inline)) {
+                constexpr int ST = decltype(stage)::value;
+                const std::integral_constant<int, (ST + 1) % 3> next{};
+                issue_plain(i + 2, (ST + 2) % 3);
+                fetch_plain(i + 3);
+                float nxt[16];
+                qk(next, nxt, [&](int x) { if (beside(x)) exps(4 + x / (KS / 4)); });
+                bias(nxt, key_of(i + 1));
+                settle(stage, i);
+                l_old = l;
+                u4v pn;
+                pv(stage, [&](int x) { if (beside(x)) exps_to(nxt, x / (KS / 4), pn); });
+                pf[0] = pn;
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] = nxt[r];
+                wait_copies();
+                __syncthreads();
+            };
+
+            if (n > 0) {
+                wait_copies();
+                __syncthreads();
+                holes = uniform(*flag) != 0;
+                if (!holes) {
+                    const int upto = min(w.hi, p.window > 0 ? n0 + 1 : max(n0 + 1, w.prefix));
+                    full0 = p.window > 0 ? max(n1 - p.window + UK - key_first, 0) / UK : 0;  // the first tile with key0 > n1 - window
+                    full1 = max((upto - key_first) / UK, 0);
+                }
+            }
+            for (int i = 0; i < n;) {
+                // Triples of full steps: tiles i .. i + 3 full, copies up to tile i + 4 and entries up to i + 5 of tiles without an end.
+                const int last = min(full1 - 4, ends - 6);
+                if (i % 3 == 0 && i >= full0 && i <= last) {
+                    qk(std::integral_constant<int, 0>{}, s, no_hook);
+                    bias(s, key_of(i));
+                    move_max();
+                    l_old = l;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) exps(k);
+                    for (; i <= last; i += 3) {
+                        full_step(i, std::integral_constant<int, 0>{});
+                        full_step(i + 1, std::integral_constant<int, 1>{});
+                        full_step(i + 2, std::integral_constant<int, 2>{});
+                    }
+                    l = l_old;  // tile i is begun again
+                }
+                if (i + 2 < n) {
+                    issue(i + 2, (i + 2) % 3);
+                    if (i + 3 < n) fetch(i + 3);
+                }
+                plain_step(i);
+                i++;
+                wait_copies();
+                __syncthreads();
+            }
+        }
+
+        // The rows turn around in LDS (chunk c of row r at c ^ (r & 15) or, of 8, c ^ (r & 7)) so that a store covers whole rows.
+        if (active) {
+            const int ln = lane_again(), lg = ln >> 5, lr = ln & 31;
+            const f2 lh = both_halves(l);
+            const float sum = lh[0] + lh[1];
+            char* turn = smem + wave * (32 * 256);
+            auto settle_lds = []() __attribute__((always_inline)) {
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            };
+            if (whole) {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that saw nothing: O is 0
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; r4++) {
+                        const u2v word = {pair_of<T>(o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv), pair_of<T>(o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv)};
+                        *(u2v*)(turn + lr * ROW + (((4 * d + r4) ^ (lr & (D / 8 - 1))) << 4) + 8 * lg) = word;
+                    }
+                settle_lds();
+#pragma unroll
+                for (int i = 0; i < 32 / CR; i++) {
+                    const int r = CR * i + ln / (D / 8), c = ln % (D / 8), out_row = wr0 + r;
+                    const u4v x = *(const u4v*)(turn + r * ROW + ((c ^ (r & (D / 8 - 1))) << 4));
+                    if (out_row <= w.r1) {
+                        const int token = div_by(out_row, p.G), head = run.kvh * (int)p.G.d + out_row - token * (int)p.G.d;
+                        *(u4v*)((T*)p.o + (long)(w.first + token) * p.sot + head * p.soh + c * 8) = x;
+                    }
+                }
+            } else {
+                float* part = partial<MT, D>(p, block, u0 == 0);
+#pragma unroll
+                for (int half = 0; half < D / 64; half++) {  // 64 values of fp32 at a time
+#pragma unroll
+                    for (int d = 0; d < 2; d++)
+#pragma unroll
+                        for (int r4 = 0; r4 < 4; r4++) {
+                            const f16v& z = o[2 * half + d];
+                            *(f4*)(turn + lr * 256 + (((8 * d + 2 * r4 + lg) ^ (lr & 15)) << 4)) = (f4){z[4 * r4], z[4 * r4 + 1], z[4 * r4 + 2], z[4 * r4 + 3]};
+                        }
+                    settle_lds();
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int r = 4 * i + (ln >> 4), c = ln & 15;
+                        *(f4*)(part + (32 * wave + r) * D + 64 * half + 4 * c) = *(const f4*)(turn + r * 256 + ((c ^ (r & 15)) << 4));
+                    }
+                    settle_lds();
+                }
+                if (lg == 0) {
+                    part[MT * D + 32 * wave + lr] = m;
+                    part[MT * D + MT + 32 * wave + lr] = sum;
+                }
+            }
+        }
+        __syncthreads();
+        if (u0 == 0 && u1 < w.units) {
+            cut.more = (int)((w.units - u1 + run.quota - 1) / run.quota);
+            cut.kvh = run.kvh;
+            cut.first = w.first;
+            cut.rows = w.rows;
+            cut.r0 = w.r0;
+        }
+        run.count -= u1 - u0;
+        run.unit = 0;
+        if (run.count > 0) next_tile<MT>(p, run);
+    }
+    if (threadIdx.x == 0) ((Cut*)p.ws)[block] = cut;
+}
+
 // Adds up the parts of the tiles that the runs cut: workgroup (x, y) takes rows 4 y .. 4 y + 3 of the tile that run x began and did not
 // end, a wave per row; lanes 16 i .. 16 i + 15 take every fourth part from the i-th on, then the four sums meet. Also zeroes the rows
 // of no sequence, where the output was made for the call.
@@ -668,8 +1168,8 @@ static int make_plan(long T, long B, long H, long Hkv, long D, int type, Plan* p
     if (T * (H / Hkv) >= 1L << 31) return RDA_ERR_INVALID;
     // Rows of a sequence and KV head, on average.
     const long rows = T * (H / Hkv) / B;
-    plan->mt = rows <= 16 ? 16 : 32;
-    plan->grid = plan->mt == 16 ? 768 : 512;
+    plan->mt = rows <= 16 ? 16 : rows <= 32 || type == RDA_FP32 ? 32 : 128;
+    plan->grid = plan->mt == 32 || (plan->mt == 128 && D == 128) ? 512 : 768;
     if ((T * (H / Hkv) / plan->mt + 1) * B >= 1L << 31) return RDA_ERR_INVALID;
     plan->workspace = (size_t)plan->grid * sizeof(Cut) + (size_t)plan->grid * 2 * plan->mt * (D + 2) * 4;
     return 0;
@@ -687,7 +1187,21 @@ static int launch_rows(const PagedArgs& a, void* stream) {
     return (int)hipGetLastError();
 }
 template <class T, int D>
+static int launch_tiles(const PagedArgs& a, void* stream) {
+    const size_t lds = TilesLds<D>::BYTES;
+    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.grid), dim3(256), lds, (hipStream_t)stream, a); };
+    const bool mod = a.cap > 0.f || a.slopes;
+    // Rows of a copy from one scalar base: in one page, the lanes' offsets within 32 bits.
+    if (a.S.d % 8 == 0 && a.kpr < 1L << 24 && a.vpr < 1L << 24) mod ? launch(tiles_kernel<T, D, true, true>) : launch(tiles_kernel<T, D, false, true>);
+    else mod ? launch(tiles_kernel<T, D, true, false>) : launch(tiles_kernel<T, D, false, false>);
+    if (const hipError_t e = hipGetLastError()) return (int)e;
+    hipLaunchKernelGGL((merge_kernel<T, D, 128>), dim3(a.grid, 32), dim3(256), 0, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+template <class T, int D>
 static int launch_paged(const PagedArgs& a, const Plan& plan, void* stream) {
+    if constexpr (sizeof(T) == 2)
+        if (plan.mt == 128) return launch_tiles<T, D>(a, stream);
     return plan.mt == 16 ? launch_rows<T, D, 1>(a, stream) : launch_rows<T, D, 2>(a, stream);
 }
 
