@@ -35,7 +35,9 @@ struct PagedArgs {
     char* ws;
     int T, B, H, Hkv, P, N, capacity;  // rows, sequences, heads, KV heads, pages, pages per sequence, N x page size
     Div S, G;                          // page size, query heads per KV head
-    long pitch, sqt, sqh, sot, soh, kpp, kpr, kph, vpp, vpr, vph;
+    Div runs;                          // grid
+    long pitch, sqt, sqh, sot, soh, kph, vph;
+    u32 kpp, kpr, vpp, vpr;  // strides of pages and of rows: products of them with a 32-bit number are one instruction
     float scale;     // scale log2 e, or scale / cap x 2 log2 e (the exponent of tanh)
     float cap;       // cap log2 e, or 0
     int window, grid, fill;
@@ -85,16 +87,22 @@ __device__ __forceinline__ WorkTile uniform(WorkTile t) {
     return {uniform(t.first), uniform(t.rows), uniform(t.r0), uniform(t.r1), uniform(t.p0), uniform(t.keys), uniform(t.prefix), uniform(t.lo), uniform(t.hi), uniform(t.units)};
 }
 
-// Inclusive sums over the workgroup's NT values; red holds NT / 64 sums.
+// Inclusive sums over a wave's lanes, and over the workgroup's NT values (red holds NT / 64 sums).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u32 add_from(u32 x) { return x + (u32)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false); }
+__device__ __forceinline__ u32 scan_wave(u32 x) {
+    x = add_from<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8: within 16 lanes
+    x = add_from<0x112, 0xF>(x);
+    x = add_from<0x114, 0xF>(x);
+    x = add_from<0x118, 0xF>(x);
+    x = add_from<0x142, 0xA>(x);  // lane 15 of rows 0 and 2 to rows 1 and 3
+    return add_from<0x143, 0xC>(x);  // lane 31 to rows 2 and 3
+}
 template <int NT>
 __device__ __forceinline__ u32 scan_block(u32 x, u32* red) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u32 y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
-    if (lane == 63) red[wave] = x;
+    const int wave = threadIdx.x >> 6;
+    x = scan_wave(x);
+    if ((threadIdx.x & 63) == 63) red[wave] = x;
     __syncthreads();
     for (int w = 0; w < wave; w++) x += red[w];
     __syncthreads();
@@ -107,12 +115,51 @@ struct Run {
     int count;
     u32 quota;  // units of every run but the last
 };
+// The run of workgroup `block` of per_head units a KV head: its KV head and how many units, and the unit within the KV head (returned);
+// count 0: none.
+__device__ __forceinline__ u32 cut_run(const PagedArgs& p, u32 per_head, int block, Run& run) {
+    const unsigned long long total = (unsigned long long)per_head * p.Hkv;
+    unsigned long long u0;
+    if (total < (1u << 31) - 65536) {
+        run.quota = (u32)div_by((int)total + p.grid - 1, p.runs);
+        const u32 at = run.quota * (u32)block;  // below total + quota x grid < 2^32
+        if (at >= (u32)total) return 0;
+        run.kvh = (int)(at / per_head);
+        run.count = (int)min(run.quota, (u32)total - at);
+        return at - (u32)run.kvh * per_head;
+    }
+    run.quota = (u32)((total + p.grid - 1) / p.grid);
+    u0 = (unsigned long long)run.quota * block;
+    if (u0 >= total) return 0;
+    run.kvh = (int)(u0 / per_head);
+    run.count = (int)min((unsigned long long)run.quota, total - u0);
+    return (u32)(u0 - (unsigned long long)run.kvh * per_head);
+}
 // smem: B + 1 tile sums; shared: NT + 8 words.
 template <int MT, int UK, int NT>
-__device__ Run find_run(const PagedArgs& p, int* smem, u32* shared, int block) {
+__device__ __forceinline__ Run find_run(const PagedArgs& p, int* smem, u32* shared, int block) {
     const int t = threadIdx.x;
     u32* red = shared + NT;
     Run run = {};
+    // Up to 64 sequences of a tile each at most (a batch of single tokens): every wave by itself, a sequence per lane. (With a lane for
+    // each tile and the general search, a call of one token took 3 us longer.)
+    if (p.B <= 64) {
+        const int lane = t & 63, b = min(lane, p.B - 1);
+        int first;
+        const int rows = lane < p.B ? seq_rows(p, b, first) : 0;
+        if (!__any(rows > MT)) {
+            const u32 units = rows > 0 ? make_tile<MT, UK>(p, b, 0).units : 0, upto = scan_wave(units);
+            const u32 s = cut_run(p, (u32)__builtin_amdgcn_readlane((int)upto, 63), block, run);
+            if (run.count == 0) return run;
+            run.b = uniform((int)__builtin_ctzll(__ballot(upto > s)));
+            run.kvh = uniform(run.kvh);
+            run.count = uniform(run.count);
+            run.quota = (u32)uniform((int)run.quota);
+            run.unit = uniform((int)(s - (u32)__builtin_amdgcn_readlane((int)(upto - units), run.b)));
+            run.tiles = 1;
+            return run;
+        }
+    }
     // Tiles of the sequences before each one.
     const int per = (p.B + NT - 1) / NT, b0 = min(t * per, p.B), b1 = min(b0 + per, p.B);
     u32 tiles = 0;
@@ -149,12 +196,8 @@ __device__ Run find_run(const PagedArgs& p, int* smem, u32* shared, int block) {
     if (t == NT - 1) red[4] = upto;
     if (t == 0) shared[3] = 0;
     __syncthreads();
-    const u32 per_head = red[4];
-    const unsigned long long total = (unsigned long long)per_head * p.Hkv;
-    const u32 quota = (u32)((total + p.grid - 1) / p.grid);
-    const unsigned long long u0 = (unsigned long long)quota * block;
-    if (u0 >= total) return run;
-    const u32 head = (u32)(u0 / per_head), s = (u32)(u0 % per_head);
+    const u32 s = cut_run(p, red[4], block, run);
+    if (run.count == 0) return run;
     if (units && from <= s && s < upto) {  // one thread
         u32 at = from;
         int bb = bt;
@@ -172,13 +215,13 @@ __device__ Run find_run(const PagedArgs& p, int* smem, u32* shared, int block) {
         }
     }
     __syncthreads();
-    run.kvh = uniform((int)head);
+    run.kvh = uniform(run.kvh);
     run.b = uniform((int)shared[0]);
     run.j = uniform((int)shared[1]);
     run.unit = uniform((int)shared[2]);
     run.tiles = uniform((int)shared[3]);
-    run.count = run.tiles ? uniform((int)min((unsigned long long)quota, total - u0)) : 0;  // no tiles: sums past 32 bits (starts that fall)
-    run.quota = (u32)uniform((int)quota);
+    run.count = run.tiles ? uniform(run.count) : 0;  // no tiles: sums past 32 bits (starts that fall)
+    run.quota = (u32)uniform((int)run.quota);
     __syncthreads();
     return run;
 }
@@ -209,6 +252,10 @@ struct Cut {
 template <int MT, int D>
 __device__ __forceinline__ float* partial(const PagedArgs& p, int block, int which) {
     return (float*)(p.ws + (size_t)p.grid * sizeof(Cut)) + ((size_t)block * 2 + which) * MT * (D + 2);
+}
+// The offset of a row of a page.
+__device__ __forceinline__ unsigned long long row_at(u32 page, u32 page_stride, u32 row, u32 row_stride) {
+    return (unsigned long long)page * page_stride + (unsigned long long)row * row_stride;
 }
 // The workgroup's place in the order of the work: an XCD (block ids go round the eight of them) takes consecutive ones.
 __device__ __forceinline__ int work_block(int grid) {
@@ -258,7 +305,7 @@ struct RowsTile {
     static constexpr int UK = 4 * KT;          // keys of a unit
 };
 
-template <class T, int D, int MB, bool MOD>
+template <class T, int D, int MB, bool MOD, bool RUNS>
 __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(PagedArgs p) {
     using R = RowsTile<T>;
     constexpr bool FP32 = R::FP32;
@@ -317,13 +364,12 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
         }
 
         if (w.hi > w.lo) {
-            const bool runs = p.S.d % KG == 0;  // a lane group's keys share a page
             // Table entries of tile i: of the lane's K keys and of its V keys.
             auto key_of = [&](int i) __attribute__((always_inline)) { return w.lo + (u0 + i) * UK + wave * KT; };
-            int kid[NB], vid[KG];
+            int kid[RUNS ? 1 : NB], vid[RUNS ? 1 : KG];
             auto fetch_ids = [&](int i) __attribute__((always_inline)) {
                 const int key0 = key_of(i);
-                if (runs) {
+                if constexpr (RUNS) {
                     const int last = (w.hi - 1) / KG * KG;
                     kid[0] = table[div_by(min(key0 + KG * (r >> 2), last), p.S)];
                     vid[0] = table[div_by(min(key0 + KG * g, last), p.S)];
@@ -331,44 +377,51 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
 #pragma unroll
                     for (int c = 0; c < NB; c++) kid[c] = table[div_by(min(key0 + KG * (r >> 2) + 4 * c + (r & 3), w.hi - 1), p.S)];
 #pragma unroll
-                    for (int i = 0; i < KG; i++) vid[i] = table[div_by(min(key0 + KG * g + i, w.hi - 1), p.S)];
+                    for (int e = 0; e < KG; e++) vid[e] = table[div_by(min(key0 + KG * g + e, w.hi - 1), p.S)];
                 }
             };
-            // Row of a key, and the first row of its page's entry, with pages that the cache does not have read as page 0.
-            auto page_of = [&](int id) __attribute__((always_inline)) { return (u32)id < (u32)p.P ? id : 0; };
+            // The address of a key's row; pages that the cache does not have are read as page 0.
+            auto row_of = [&](const T* base, int id, int key, u32 page_stride, u32 row_stride) __attribute__((always_inline)) {
+                const u32 page = (u32)id < (u32)p.P ? (u32)id : 0, row = (u32)(key - div_by(key, p.S) * (int)p.S.d);
+                return base + row_at(page, page_stride, row, row_stride);
+            };
             kvec kf[NB][KC];
             vvec vf[KG][VH];
             auto load_k = [&](int i) __attribute__((always_inline)) {
-                const int key0 = key_of(i), last = (w.hi - 1) / KG * KG;
+                const int key0 = key_of(i);
+                if constexpr (RUNS) {
+                    const T* src = row_of(kbase, kid[0], min(key0 + KG * (r >> 2), (w.hi - 1) / KG * KG) + (r & 3), p.kpp, p.kpr) + g * EV;
 #pragma unroll
-                for (int c = 0; c < NB; c++) {
-                    const int key = runs ? min(key0 + KG * (r >> 2), last) + 4 * c + (r & 3) : min(key0 + KG * (r >> 2) + 4 * c + (r & 3), w.hi - 1);
-                    const int row = key - div_by(key, p.S) * (int)p.S.d;
-                    const T* src = kbase + page_of(kid[runs ? 0 : c]) * p.kpp + row * p.kpr + g * EV;
+                    for (int c = 0; c < NB; c++)
 #pragma unroll
-                    for (int x = 0; x < KC; x++) kf[c][x] = *(const kvec*)(src + 4 * EV * x);
+                        for (int x = 0; x < KC; x++) kf[c][x] = *(const kvec*)(src + (unsigned long long)(4 * c) * p.kpr + 4 * EV * x);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < NB; c++) {
+                        const T* src = row_of(kbase, kid[c], min(key0 + KG * (r >> 2) + 4 * c + (r & 3), w.hi - 1), p.kpp, p.kpr) + g * EV;
+#pragma unroll
+                        for (int x = 0; x < KC; x++) kf[c][x] = *(const kvec*)(src + 4 * EV * x);
+                    }
                 }
             };
             u32 vbad = 0;  // the lane's V keys on pages the cache does not have
             auto load_v = [&](int i) __attribute__((always_inline)) {
                 const int key0 = key_of(i);
-                vbad = 0;
-                if (runs) {
-                    const int key = min(key0 + KG * g, (w.hi - 1) / KG * KG), row = key - div_by(key, p.S) * (int)p.S.d;
-                    const T* src = vbase + page_of(vid[0]) * p.vpp + row * p.vpr + r * VC;
-                    if ((u32)vid[0] >= (u32)p.P) vbad = ~0u;
+                if constexpr (RUNS) {
+                    const T* src = row_of(vbase, vid[0], min(key0 + KG * g, (w.hi - 1) / KG * KG), p.vpp, p.vpr) + r * VC;
+                    vbad = (u32)vid[0] < (u32)p.P ? 0 : ~0u;
 #pragma unroll
-                    for (int i = 0; i < KG; i++)
+                    for (int e = 0; e < KG; e++)
 #pragma unroll
-                        for (int h = 0; h < VH; h++) vf[i][h] = *(const vvec*)(src + i * p.vpr + 16 * VC * h);
+                        for (int h = 0; h < VH; h++) vf[e][h] = *(const vvec*)(src + (unsigned long long)e * p.vpr + 16 * VC * h);
                 } else {
+                    vbad = 0;
 #pragma unroll
-                    for (int i = 0; i < KG; i++) {
-                        const int key = min(key0 + KG * g + i, w.hi - 1), row = key - div_by(key, p.S) * (int)p.S.d;
-                        const T* src = vbase + page_of(vid[i]) * p.vpp + row * p.vpr + r * VC;
-                        if ((u32)vid[i] >= (u32)p.P) vbad |= 1u << i;
+                    for (int e = 0; e < KG; e++) {
+                        const T* src = row_of(vbase, vid[e], min(key0 + KG * g + e, w.hi - 1), p.vpp, p.vpr) + r * VC;
+                        vbad |= (u32)vid[e] < (u32)p.P ? 0 : 1u << e;
 #pragma unroll
-                        for (int h = 0; h < VH; h++) vf[i][h] = *(const vvec*)(src + 16 * VC * h);
+                        for (int h = 0; h < VH; h++) vf[e][h] = *(const vvec*)(src + 16 * VC * h);
                     }
                 }
             };
@@ -428,26 +481,32 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
                             see[m] |= ok ? 1u << e : 0;
                         }
                     }
-                    // Values at keys that the sequence does not have become zeros; those of the others are looked at.
-                    bool odd = false;
+                    // Values at keys that no row sees become zeros. Where all rows are of one token that is all; else the others are looked at.
+                    u32 seen = 0;
 #pragma unroll
-                    for (int e = 0; e < KG; e++) {
-                        const bool there = key0 + KG * g + e < w.hi && !(bad >> e & 1);
+                    for (int m = 0; m < MB; m++) seen |= see[m];
 #pragma unroll
-                        for (int h = 0; h < VH; h++) {
-                            if (!there) vf[e][h] = (vvec){};
+                    for (int o = 1; o < 16; o <<= 1) seen |= __shfl_xor(seen, o);
 #pragma unroll
-                            for (int x = 0; x < (int)(sizeof(vvec) / 4); x++) {
-                                const u32 word = FP32 ? __float_as_uint(vf[e][h][x]) : (u32)vf[e][h][x];
-                                if constexpr (FP32) odd |= (word & 0x7f800000u) == 0x7f800000u;
-                                else {
-                                    constexpr u32 E = std::is_same<T, half_t>::value ? 0x7c00u : 0x7f80u;
-                                    odd |= (word & E) == E || (word >> 16 & E) == E;
+                    for (int e = 0; e < KG; e++)
+#pragma unroll
+                        for (int h = 0; h < VH; h++)
+                            if (!(seen >> e & 1)) vf[e][h] = (vvec){};
+                    if (n0 != n1) {
+                        bool odd = false;
+#pragma unroll
+                        for (int e = 0; e < KG; e++)
+#pragma unroll
+                            for (int h = 0; h < VH; h++)
+#pragma unroll
+                                for (int x = 0; x < (int)(sizeof(vvec) / 4); x++) {
+                                    const auto element = vf[e][h][x];  // (the bit cast of a vector's element itself reads element 0)
+                                    const u32 word = __builtin_bit_cast(u32, element);
+                                    constexpr u32 E = FP32 ? 0x7f800000u : std::is_same<T, half_t>::value ? 0x7c00u : 0x7f80u;
+                                    odd |= (word & E) == E || (!FP32 && (word >> 16 & E) == E);
                                 }
-                            }
-                        }
+                        split = __any(odd);
                     }
-                    split = __any(odd);
                 }
                 // Softmax.
                 u4v pf[MB];
@@ -723,9 +782,9 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
 #pragma unroll
             for (int c = 0; c < CP; c++) {
                 const int r = CR * (4 * c + wave), lr = r + ln / (D / 8), key = min(key_of(i) + lr, w.hi - 1), kr = key - div_by(key, p.S) * (int)p.S.d;
-                const long at = (u32)id[c] < (u32)p.P ? id[c] : 0;
-                dma16_at(kbase + at * p.kpp + kr * p.kpr + k_chunk(ln, lr) * 8, smem + stage * L::TILE + r * ROW);
-                dma16_at(vbase + at * p.vpp + kr * p.vpr + v_chunk(ln, lr) * 8, smem + L::V + stage * L::TILE + r * ROW);
+                const u32 at = (u32)id[c] < (u32)p.P ? id[c] : 0;
+                dma16_at(kbase + (row_at(at, p.kpp, kr, p.kpr) + k_chunk(ln, lr) * 8), smem + stage * L::TILE + r * ROW);
+                dma16_at(vbase + (row_at(at, p.vpp, kr, p.vpr) + v_chunk(ln, lr) * 8), smem + L::V + stage * L::TILE + r * ROW);
             }
         };
         // The same for a tile without an end and with none but pages that exist, whose rows of a copy lie in one page (RUNS).
@@ -741,9 +800,9 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
 #pragma unroll
                 for (int c = 0; c < CP; c++) {
                     const int r = CR * (4 * c + wave), key = key_of(i) + r, kr = key - div_by(key, p.S) * (int)p.S.d;
-                    const long page = uniform(id[c]);
-                    dma16(uniform(kbase + page * p.kpp + kr * p.kpr), k_off, smem + stage * L::TILE + r * ROW);
-                    dma16(uniform(vbase + page * p.vpp + kr * p.vpr), v_off, smem + L::V + stage * L::TILE + r * ROW);
+                    const u32 page = (u32)uniform(id[c]);
+                    dma16(uniform(kbase + row_at(page, p.kpp, kr, p.kpr)), k_off, smem + stage * L::TILE + r * ROW);
+                    dma16(uniform(vbase + row_at(page, p.vpp, kr, p.vpr)), v_off, smem + L::V + stage * L::TILE + r * ROW);
                 }
         };
         bool holes = false;  // whether the cache lacks any page of the run's part
@@ -1127,27 +1186,29 @@ __global__ __launch_bounds__(256) void merge_kernel(PagedArgs p) {
     const Cut cut = ((const Cut*)p.ws)[blockIdx.x];
     const int tr = blockIdx.y * 4 + wave, row = cut.r0 + tr;
     if (cut.more == 0 || row >= cut.rows) return;
+    const int more = min(cut.more, p.grid - 1 - (int)blockIdx.x);
+    auto part_of = [&](int i) __attribute__((always_inline)) { return (const float*)partial<MT, D>(p, blockIdx.x + i, i == 0); };
     float top = -__builtin_inff(), sum = 0.f, y[D / 16];
+    for (int i = lane; i <= more; i += 64) top = fmaxf(top, part_of(i)[MT * D + tr]);
+    top = rows_max(row_max16(top));
+    const float base = top == -__builtin_inff() ? 0.f : top;
+    for (int i = lane; i <= more; i += 64) sum = __builtin_fmaf(part_of(i)[MT * D + MT + tr], __builtin_amdgcn_exp2f(part_of(i)[MT * D + tr] - base), sum);
+    sum = rows_sum(row_sum16(sum));
 #pragma unroll
     for (int e = 0; e < D / 16; e++) y[e] = 0.f;
-    const int more = min(cut.more, p.grid - 1 - (int)blockIdx.x);
+#pragma unroll 4
     for (int i = g; i <= more; i += 4) {
-        const float* part = partial<MT, D>(p, blockIdx.x + i, i == 0);
-        const float m = part[MT * D + tr], l = part[MT * D + MT + tr], now = fmaxf(top, m);
-        const float a = top == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(top - now), b = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - now);
-        top = now;
-        sum = __builtin_fmaf(sum, a, l * b);
+        const float* part = part_of(i);
+        const float a = __builtin_amdgcn_exp2f(part[MT * D + tr] - base);
 #pragma unroll
         for (int e = 0; e < D / 16; e += 4) {
             const f4 z = *(const f4*)(part + tr * D + c + e);
 #pragma unroll
-            for (int k = 0; k < 4; k++) y[e + k] = __builtin_fmaf(y[e + k], a, z[k] * b);
+            for (int k = 0; k < 4; k++) y[e + k] = __builtin_fmaf(z[k], a, y[e + k]);
         }
     }
-    const float all = rows_max(top), a = top == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(top - all);
-    sum = rows_sum(sum * a);
 #pragma unroll
-    for (int e = 0; e < D / 16; e++) y[e] = rows_sum(y[e] * a);
+    for (int e = 0; e < D / 16; e++) y[e] = rows_sum(y[e]);
     if (g == 0) {
         const int token = div_by(row, p.G), head = cut.kvh * (int)p.G.d + row - token * (int)p.G.d;
         T* out = (T*)p.o + (long)(cut.first + token) * p.sot + head * p.soh + c;
@@ -1169,7 +1230,7 @@ static int make_plan(long T, long B, long H, long Hkv, long D, int type, Plan* p
     // Rows of a sequence and KV head, on average.
     const long rows = T * (H / Hkv) / B;
     plan->mt = rows <= 16 ? 16 : rows <= 32 || type == RDA_FP32 ? 32 : 128;
-    plan->grid = plan->mt == 32 || (plan->mt == 128 && D == 128) ? 512 : 768;
+    plan->grid = D == 128 || plan->mt == 32 ? 512 : 768;
     if ((T * (H / Hkv) / plan->mt + 1) * B >= 1L << 31) return RDA_ERR_INVALID;
     plan->workspace = (size_t)plan->grid * sizeof(Cut) + (size_t)plan->grid * 2 * plan->mt * (D + 2) * 4;
     return 0;
@@ -1180,8 +1241,9 @@ static int launch_rows(const PagedArgs& a, void* stream) {
     constexpr int OP = D + 4;
     const size_t o = 4 * 16 * OP * 4, sums = (size_t)(a.B + 1) * 4, lds = o > sums ? o : sums;
     const bool mod = a.cap > 0.f || a.slopes;
-    if (mod) hipLaunchKernelGGL((rows_kernel<T, D, MB, true>), dim3(a.grid), dim3(256), lds, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((rows_kernel<T, D, MB, false>), dim3(a.grid), dim3(256), lds, (hipStream_t)stream, a);
+    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.grid), dim3(256), lds, (hipStream_t)stream, a); };
+    if (a.S.d % RowsTile<T>::KG == 0) mod ? launch(rows_kernel<T, D, MB, true, true>) : launch(rows_kernel<T, D, MB, false, true>);
+    else mod ? launch(rows_kernel<T, D, MB, true, false>) : launch(rows_kernel<T, D, MB, false, false>);
     if (const hipError_t e = hipGetLastError()) return (int)e;
     hipLaunchKernelGGL((merge_kernel<T, D, 16 * MB>), dim3(a.grid, 4 * MB), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
@@ -1192,7 +1254,7 @@ static int launch_tiles(const PagedArgs& a, void* stream) {
     const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.grid), dim3(256), lds, (hipStream_t)stream, a); };
     const bool mod = a.cap > 0.f || a.slopes;
     // Rows of a copy from one scalar base: in one page, the lanes' offsets within 32 bits.
-    if (a.S.d % 8 == 0 && a.kpr < 1L << 24 && a.vpr < 1L << 24) mod ? launch(tiles_kernel<T, D, true, true>) : launch(tiles_kernel<T, D, false, true>);
+    if (a.S.d % 8 == 0 && a.kpr < 1u << 24 && a.vpr < 1u << 24) mod ? launch(tiles_kernel<T, D, true, true>) : launch(tiles_kernel<T, D, false, true>);
     else mod ? launch(tiles_kernel<T, D, true, false>) : launch(tiles_kernel<T, D, false, false>);
     if (const hipError_t e = hipGetLastError()) return (int)e;
     hipLaunchKernelGGL((merge_kernel<T, D, 128>), dim3(a.grid, 32), dim3(256), 0, (hipStream_t)stream, a);
@@ -1231,6 +1293,8 @@ int rda_paged_attn(const void* q, void* out, const void* k_pages, const void* v_
         return RDA_ERR_INVALID;
     // Units of a KV head in 32 bits, whatever the lengths.
     if ((T * (H / Hkv) / plan.mt + B) * (N * S / 64 + 1) >= 1L << 32) return RDA_ERR_INVALID;
+    for (int i : {13, 14, 16, 17})
+        if (dims[i] < 0 || dims[i] >= 1L << 32) return RDA_ERR_INVALID;
     PagedArgs a;
     a.q = q; a.o = out; a.k = k_pages; a.v = v_pages;
     a.table = table; a.starts = starts; a.lengths = lengths; a.prefix = prefix;
@@ -1240,11 +1304,14 @@ int rda_paged_attn(const void* q, void* out, const void* k_pages, const void* v_
     a.S = make_div((int)S); a.G = make_div((int)(H / Hkv));
     a.pitch = dims[6];
     a.sqt = dims[9]; a.sqh = dims[10]; a.sot = dims[11]; a.soh = dims[12];
-    a.kpp = dims[13]; a.kpr = dims[14]; a.kph = dims[15]; a.vpp = dims[16]; a.vpr = dims[17]; a.vph = dims[18];
+    a.kpp = (u32)dims[13]; a.kpr = (u32)dims[14]; a.kph = dims[15]; a.vpp = (u32)dims[16]; a.vpr = (u32)dims[17]; a.vph = dims[18];
     a.scale = softcap > 0.f ? scale / softcap * 2.f * LOG2E : scale * LOG2E;
     a.cap = softcap * LOG2E;
     a.window = window;
-    a.grid = plan.grid;
+    // No more workgroups than units there can be: a short table of few sequences needs none that finds no work.
+    const long least = plan.mt == 128 ? 32 : type == RDA_FP32 ? 64 : 128, units = (T * (H / Hkv) / plan.mt + B) * ((N * S + least - 1) / least) * Hkv;
+    a.grid = (int)(units < plan.grid ? units : plan.grid);
+    a.runs = make_div(a.grid);
     a.fill = fill;
     const auto heads = [&](auto x) {
         using X = decltype(x);
