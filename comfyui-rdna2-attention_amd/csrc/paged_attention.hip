@@ -755,7 +755,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
         const WorkTile w = uniform(make_tile<MT, UK>(p, run.b, run.j));
         const int u0 = run.unit, u1 = min(w.units, u0 + run.count), n = w.hi > w.lo ? u1 - u0 : 0;
         const bool whole = u0 == 0 && u1 == w.units;
-        const int* table = uniform(p.table + run.b * p.pitch);
+        const int* table = p.table + run.b * p.pitch;
         const T* kbase = uniform((const T*)p.k + run.kvh * p.kph);
         const T* vbase = uniform((const T*)p.v + run.kvh * p.vph);
         const int key_first = w.lo + u0 * UK;
@@ -777,14 +777,14 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
 #pragma unroll
             for (int c = 0; c < CP; c++) id[c] = table[div_by(min(key_of(i) + CR * (4 * c + wave) + ln / (D / 8), w.hi - 1), p.S)];
         };
-        auto issue = [&](int i, int stage) __attribute__((always_inline)) {
+        auto issue = [&](int i, u32 st) __attribute__((always_inline)) {
             const int ln = lane_again();
 #pragma unroll
             for (int c = 0; c < CP; c++) {
                 const int r = CR * (4 * c + wave), lr = r + ln / (D / 8), key = min(key_of(i) + lr, w.hi - 1), kr = key - div_by(key, p.S) * (int)p.S.d;
                 const u32 at = (u32)id[c] < (u32)p.P ? id[c] : 0;
-                dma16_at(kbase + (row_at(at, p.kpp, kr, p.kpr) + k_chunk(ln, lr) * 8), smem + stage * L::TILE + r * ROW);
-                dma16_at(vbase + (row_at(at, p.vpp, kr, p.vpr) + v_chunk(ln, lr) * 8), smem + L::V + stage * L::TILE + r * ROW);
+                dma16_at(kbase + (row_at(at, p.kpp, kr, p.kpr) + k_chunk(ln, lr) * 8), smem + st + r * ROW);
+                dma16_at(vbase + (row_at(at, p.vpp, kr, p.vpr) + v_chunk(ln, lr) * 8), smem + L::V + st + r * ROW);
             }
         };
         // The same for a tile without an end and with none but pages that exist, whose rows of a copy lie in one page (RUNS).
@@ -794,15 +794,15 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
 #pragma unroll
                 for (int c = 0; c < CP; c++) id[c] = table[div_by(key_of(i) + CR * (4 * c + wave), p.S)];
         };
-        auto issue_plain = [&](int i, int stage) __attribute__((always_inline)) {
-            if constexpr (!RUNS) issue(i, stage);
+        auto issue_plain = [&](int i, u32 st) __attribute__((always_inline)) {
+            if constexpr (!RUNS) issue(i, st);
             else
 #pragma unroll
                 for (int c = 0; c < CP; c++) {
                     const int r = CR * (4 * c + wave), key = key_of(i) + r, kr = key - div_by(key, p.S) * (int)p.S.d;
                     const u32 page = (u32)uniform(id[c]);
-                    dma16(uniform(kbase + row_at(page, p.kpp, kr, p.kpr)), k_off, smem + stage * L::TILE + r * ROW);
-                    dma16(uniform(vbase + row_at(page, p.vpp, kr, p.vpr)), v_off, smem + L::V + stage * L::TILE + r * ROW);
+                    dma16(uniform(kbase + row_at(page, p.kpp, kr, p.kpr)), k_off, smem + st + r * ROW);
+                    dma16(uniform(vbase + row_at(page, p.vpp, kr, p.vpr)), v_off, smem + L::V + st + r * ROW);
                 }
         };
         bool holes = false;  // whether the cache lacks any page of the run's part
@@ -824,7 +824,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
             issue(0, 0);
 #pragma unroll
             for (int c = 0; c < CP; c++) id[c] = second[c];
-            if (n > 1) issue(1, 1);
+            if (n > 1) issue(1, L::TILE);
             if (n > 2) fetch(2);
         }
 
@@ -840,7 +840,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
             }
             for (int i = 0; i < n; i++) {
                 if (i + 2 < n) {
-                    issue(i + 2, (i + 2) % 3);
+                    issue(i + 2, (u32)((i + 2) % 3 * L::TILE));
                     if (i + 3 < n) fetch(i + 3);
                 }
                 wait_copies();
@@ -873,21 +873,21 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
             }
             asm volatile("" : "+v"(k_base), "+v"(v_base));
 
-            auto qk = [&](auto stage, float (&out)[16], auto&& hook) __attribute__((always_inline)) {
-                const u32 st = (u32)((int)stage * L::TILE);
-                u32 kb = k_base;
+            // `st`: the offset of the tile's stage (the xors above leave a stage's bits alone).
+            auto qk = [&](u32 st, float (&out)[16], auto&& hook) __attribute__((always_inline)) {
+                u32 kb = k_base + st;
                 asm volatile("" : "+v"(kb));
                 f16v acc = {};
                 u4v ka[KS / 2];
 #pragma unroll
-                for (int x = 0; x < KS / 2; x++) ka[x] = lds_u4((kb ^ (u32)(32 * x)) + st);
+                for (int x = 0; x < KS / 2; x++) ka[x] = lds_u4(kb ^ (u32)(32 * x));
                 __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_s_setprio(1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int x = 0; x < KS; x++) {
                     acc = product32<T>(ka[x % (KS / 2)], qf[x], acc);
-                    if (x < KS / 2) ka[x] = lds_u4((kb ^ (u32)(32 * (KS / 2 + x))) + st);
+                    if (x < KS / 2) ka[x] = lds_u4(kb ^ (u32)(32 * (KS / 2 + x)));
                     hook(x);
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -915,7 +915,6 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
                 }
             };
             const float scale = MOD ? 1.f : p.scale;
-            float s[16];
             u4v pf[2];  // P of the two 16-key steps
             // Part k (of eight) of the P of scores x: registers 2 k, 2 k + 1.
             auto exps_into = [&](const float (&x)[16], int k, u4v& d) __attribute__((always_inline)) {
@@ -924,17 +923,17 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
                 l = add_pair<T>(word, l);
                 d[k & 3] = word;
             };
-            auto exps = [&](int k) __attribute__((always_inline)) { exps_into(s, k, pf[k >> 2]); };
+            auto exps = [&](const float (&x)[16], int k) __attribute__((always_inline)) { exps_into(x, k, pf[k >> 2]); };
             auto exps_to = [&](const float (&x)[16], int k, u4v& d) __attribute__((always_inline)) {
                 exps_into(x, k, d);
                 asm volatile("" : "+v"(d), "+v"(l));
             };
             auto no_hook = [](int) {};
             // m moves only where a tile's maximum exceeds it by more than 8.
-            auto move_max = [&]() __attribute__((always_inline)) {
-                float mx = s[0];
+            auto move_max = [&](const float (&x)[16]) __attribute__((always_inline)) {
+                float mx = x[0];
 #pragma unroll
-                for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[r]);
+                for (int r = 1; r < 16; r++) mx = fmaxf(mx, x[r]);
                 const f2 h = both_halves(mx);
                 mx = fmaxf(h[0], h[1]) * scale;
                 if (__any(mx > m + 8.f)) {
@@ -945,22 +944,21 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
                     for (int d = 0; d < DT; d++) o[d] *= a;
                 }
             };
-            auto read_v = [&](u32 vb, u32 st, int j, int d) __attribute__((always_inline)) {
-                const u32 at = (vb ^ (u32)(64 * d)) + st + 16 * j * ROW;
+            auto read_v = [&](u32 vb, int j, int d) __attribute__((always_inline)) {
+                const u32 at = (vb ^ (u32)(64 * d)) + 16 * j * ROW;
                 return __builtin_shufflevector(lds_tr(at), lds_tr(at + 8 * ROW), 0, 1, 2, 3);
             };
-            auto pv = [&](auto stage, auto&& hook) __attribute__((always_inline)) {
-                const u32 st = (u32)((int)stage * L::TILE);
-                u32 vb = v_base;
+            auto pv = [&](u32 st, auto&& hook) __attribute__((always_inline)) {
+                u32 vb = v_base + st;
                 asm volatile("" : "+v"(vb));
                 u4v va[DT];
 #pragma unroll
-                for (int d = 0; d < DT; d++) va[d] = read_v(vb, st, 0, d);
+                for (int d = 0; d < DT; d++) va[d] = read_v(vb, 0, d);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
                     o[d] = product32<T>(va[d], pf[0], o[d]);
-                    va[d] = read_v(vb, st, 1, d);
+                    va[d] = read_v(vb, 1, d);
                     hook(d);
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -976,11 +974,12 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
             int full0 = 0, full1 = 0;
             const int ends = min(n, (w.hi - key_first) / UK);
 
-            // One tile from its scores on, wherever it lies: scores, maximum, P, product, one after the other. Leaves nothing pending.
-            auto plain_step = [&](int i) __attribute__((always_inline)) {
-                const int key0 = key_of(i), stage = i % 3;
+            // One tile from its scores on, wherever it lies: scores, maximum, P, product, one after the other.
+            auto plain_step = [&](int i, u32 st) __attribute__((always_inline)) {
+                const int key0 = key_of(i);
                 const bool masked = i < full0 || i >= full1;
-                qk(stage, s, no_hook);
+                float s[16];
+                qk(st, s, no_hook);
                 bias(s, key0);
                 u32 see = 0xffff;
                 if (masked) {
@@ -993,12 +992,11 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
                         see |= ok ? 1u << r : 0;
                     }
                 }
-                move_max();
+                move_max(s);
 #pragma unroll
-                for (int k = 0; k < 8; k++) exps(k);
+                for (int k = 0; k < 8; k++) exps(s, k);
                 if (masked) {
                     // Values that are not finite, of keys that only some rows see: key by key.
-                    const u32 st = (u32)(stage * L::TILE);
                     bool odd = false;
                     constexpr u32 E = std::is_same<T, half_t>::value ? 0x7c00u : 0x7f80u;
 #pragma unroll
@@ -1012,7 +1010,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
                         for (int j = 0; j < 2; j++)
 #pragma unroll
                             for (int d = 0; d < DT; d++) {
-                                const u4v v = read_v(v_base, st, j, d);
+                                const u4v v = read_v(v_base + st, j, d);
 #pragma unroll 1
                                 for (int kk = 0; kk < 16; kk++) {  // value (kk & 3) + kk / 8 x 4 of the lanes with g = kk / 4 & 1: register 8 j + that
                                     const int e0 = (kk >> 3) * 4 + (kk & 3);
@@ -1026,40 +1024,27 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
                         return;
                     }
                 }
-                pv(stage, no_hook);
+                pv(st, no_hook);
             };
-            // Steps of KS (or 2 DT = KS) products: the four parts of half a tile's exponentials beside every (KS / 4)-th.
+            // A step of the full tiles: tile i's scores are in s, its P's first half in pf[0] and l (before which l was l_old); tile i + 1 is full
+            // too, and its scores go to nxt. Steps of KS (or 2 DT = KS) products: the four parts of half a tile's exponentials beside every
+            // (KS / 4)-th. P is made with the m at hand: a lane's sum that grew by no more than 64 proves that no P was above it; else
+            // the step ends before the product (false), and the tile is taken again by a plain step. (With the maximum moved here, O was
+            // copied between registers in every step: 64 of ~300 instructions.)
             auto beside = [](int x) __attribute__((always_inline)) { return x % (KS / 4) == KS / 4 - 1; };
-            // A step of the full tiles: tile i's scores are in s, its P's first half in pf[0] and l; tile i + 1 is full too. P is first made
-            // with the m at hand; a lane's sum that grew by no more than 64 proves that no P was above it, else the scores are made
-            // again from the tile in LDS, the maximum taken, and P with it.
-            auto settle = [&](auto stage, int i) __attribute__((always_inline)) {
-                if (__builtin_expect(__any(!(l <= l_old + 64.f)), 0)) {
-                    qk(stage, s, no_hook);
-                    bias(s, key_of(i));
-                    l = l_old;
-                    move_max();
-#pragma unroll
-                    for (int k = 0; k < 8; k++) exps(k);
-                }
-            };
-            auto full_step = [&](int i, auto stage) __attribute__((always_inline)) {
-                constexpr int ST = decltype(stage)::value;
-                const std::integral_constant<int, (ST + 1) % 3> next{};
-                issue_plain(i + 2, (ST + 2) % 3);
-                fetch_plain(i + 3);
-                float nxt[16];
-                qk(next, nxt, [&](int x) { if (beside(x)) exps(4 + x / (KS / 4)); });
+            auto full_step = [&](int i, u32 st, u32 st1, u32 st2, const float (&s)[16], float (&nxt)[16]) __attribute__((always_inline)) {
+                if (i + 2 < ends) issue_plain(i + 2, st2);
+                if (i + 3 < ends) fetch_plain(i + 3);
+                qk(st1, nxt, [&](int x) { if (beside(x)) exps(s, 4 + x / (KS / 4)); });
                 bias(nxt, key_of(i + 1));
-                settle(stage, i);
+                if (__builtin_expect(__any(!(l <= l_old + 64.f)), 0)) return false;
                 l_old = l;
                 u4v pn;
-                pv(stage, [&](int x) { if (beside(x)) exps_to(nxt, x / (KS / 4), pn); });
+                pv(st, [&](int x) { if (beside(x)) exps_to(nxt, x / (KS / 4), pn); });
                 pf[0] = pn;
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = nxt[r];
                 wait_copies();
                 __syncthreads();
+                return true;
             };
 
             if (n > 0) {
@@ -1069,32 +1054,52 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
                 if (!holes) {
                     const int upto = min(w.hi, p.window > 0 ? n0 + 1 : max(n0 + 1, w.prefix));
                     full0 = p.window > 0 ? max(n1 - p.window + UK - key_first, 0) / UK : 0;  // the first tile with key0 > n1 - window
-                    full1 = max((upto - key_first) / UK, 0);
+                    full1 = min(max((upto - key_first) / UK, 0), n);
                 }
             }
+            // Pairs of full steps i, i + 1 up to `last`: tiles .. i + 2 full, and copies of tiles without an end only (or none left to copy).
+            const int last = ends == n ? full1 - 3 : min(full1 - 3, ends - 5);
+            u32 st = 0, st1 = L::TILE, st2 = 2 * L::TILE;  // the stages of tiles i, i + 1, i + 2
+            auto turn_stages = [&]() __attribute__((always_inline)) {
+                const u32 x = st;
+                st = st1;
+                st1 = st2;
+                st2 = x;
+            };
             for (int i = 0; i < n;) {
-                // Triples of full steps: tiles i .. i + 3 full, copies up to tile i + 4 and entries up to i + 5 of tiles without an end.
-                const int last = min(full1 - 4, ends - 6);
-                if (i % 3 == 0 && i >= full0 && i <= last) {
-                    qk(std::integral_constant<int, 0>{}, s, no_hook);
-                    bias(s, key_of(i));
-                    move_max();
+                bool copied = false;  // whether tile i + 2 is on its way already
+                if (i >= full0 && i <= last) {
+                    float sa[16], sb[16];
+                    qk(st, sa, no_hook);
+                    bias(sa, key_of(i));
+                    move_max(sa);
                     l_old = l;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) exps(k);
-                    for (; i <= last; i += 3) {
-                        full_step(i, std::integral_constant<int, 0>{});
-                        full_step(i + 1, std::integral_constant<int, 1>{});
-                        full_step(i + 2, std::integral_constant<int, 2>{});
+                    for (int k = 0; k < 4; k++) exps(sa, k);
+                    while (true) {
+                        if (!full_step(i, st, st1, st2, sa, sb)) {
+                            copied = true;
+                            break;
+                        }
+                        i++;
+                        turn_stages();
+                        if (!full_step(i, st, st1, st2, sb, sa)) {
+                            copied = true;
+                            break;
+                        }
+                        i++;
+                        turn_stages();
+                        if (i > last) break;
                     }
                     l = l_old;  // tile i is begun again
                 }
-                if (i + 2 < n) {
-                    issue(i + 2, (i + 2) % 3);
+                if (!copied && i + 2 < n) {
+                    issue(i + 2, st2);
                     if (i + 3 < n) fetch(i + 3);
                 }
-                plain_step(i);
+                plain_step(i, st);
                 i++;
+                turn_stages();
                 wait_copies();
                 __syncthreads();
             }
