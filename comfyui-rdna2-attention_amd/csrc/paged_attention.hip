@@ -282,6 +282,21 @@ __device__ __forceinline__ float capped(float e, float cap) {
     return cap * t;
 }
 
+// D / 16 consecutive values of a row, divided by the row's sum; a row that saw nothing (its sum 0) is 0.
+template <class T, int D>
+__device__ __forceinline__ void store_row(T* out, const float (&y)[D / 16], float sum) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if constexpr (D == 128) {
+        f8 x;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = y[e] * inv;
+        store8(out, x);
+    } else {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        *(t4*)out = __builtin_convertvector((f4){y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv}, t4);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ few rows
 
 // Rows kernel: tiles of 16 MB rows, for single tokens and short chunks (and fp32), bound by the keys and values read. Its four waves take
@@ -652,9 +667,7 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
                 if (w.r0 + tr <= w.r1) {
                     const int token = div_by(w.r0 + tr, p.G), head = run.kvh * (int)p.G.d + w.r0 + tr - token * (int)p.G.d;
                     T* out = (T*)p.o + (long)(w.first + token) * p.sot + head * p.soh + c;
-                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-                    for (int e = 0; e < D / 16; e++) out[e] = sum == 0.f ? (T)0.f : (T)(y[e] * inv);
+                    store_row<T, D>(out, y, sum);
                 }
             } else {
                 float* part = partial<MT, D>(p, block, u0 == 0);
@@ -738,7 +751,7 @@ __device__ __forceinline__ int lane_again() {
 }
 
 template <class T, int D, bool MOD, bool RUNS>
-__global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs p) {
+__global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(PagedArgs p) {
     constexpr int MT = 128, UK = 32, ROW = 2 * D, KS = D / 16, DT = D / 32;  // KS: products of a score block; DT: of a 16-key step with V
     constexpr int CP = D / 64, CR = 1024 / ROW;  // a wave's copies of K per tile; rows of a copy
     using L = TilesLds<D>;
@@ -896,13 +909,19 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
 #pragma unroll
                 for (int r = 0; r < 16; r++) out[r] = acc[r];
             };
-            // Register r of a lane: key 8 (r / 4) + 4 g + r % 4 of the tile. See: bit r set where the lane's row sees it.
-            auto see_key = [&](int key, int at) __attribute__((always_inline)) {
-                bool ok = key < w.hi && ((key <= at && (p.window <= 0 || at - key < p.window)) || key < w.prefix);
-                if (ok && holes) ok = (u32)table[div_by(key, p.S)] < (u32)p.P;
-                return ok;
+            // The keys of a tile that the lane's row sees, a bit each.
+            auto seen_keys = [&](int key0) __attribute__((always_inline)) {
+                auto below = [&](int key) __attribute__((always_inline)) { return (u32)((1ull << min(max(key - key0, 0), 32)) - 1); };
+                const int ln = lane_again(), at = w.p0 + div_by(min(wr0 + (ln & 31), w.r1), p.G);
+                u32 seen = below(min(at + 1, w.hi));
+                if (p.window > 0) seen &= ~below(at - p.window + 1);
+                seen |= below(w.prefix);  // at most hi
+                if (holes) {
+                    const int key = min(key0 + (ln & 31), w.hi - 1);
+                    seen &= (u32)__ballot((u32)table[div_by(key, p.S)] < (u32)p.P);
+                }
+                return seen;
             };
-            auto position_again = [&](int ln) __attribute__((always_inline)) { return w.p0 + div_by(min(wr0 + (ln & 31), w.r1), p.G); };
             auto bias = [&](float (&x)[16], int key0) __attribute__((always_inline)) {
                 if constexpr (MOD) {
                     const float d0 = (float)(pos - key0 - 4 * g);
@@ -979,18 +998,17 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
                 const int key0 = key_of(i);
                 const bool masked = i < full0 || i >= full1;
                 float s[16];
+                u32 seen = ~0u;
+                if (masked) {
+                    seen = seen_keys(key0);
+                    if (!__any(seen != 0)) return;
+                }
                 qk(st, s, no_hook);
                 bias(s, key0);
-                u32 see = 0xffff;
                 if (masked) {
-                    const int ln = lane_again(), at = position_again(ln);
-                    see = 0;
+                    const u32 mine = seen >> (4 * (lane_again() >> 5));  // register r: key 8 (r / 4) + 4 g + r % 4
 #pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const bool ok = see_key(key0 + 8 * (r >> 2) + 4 * (ln >> 5) + (r & 3), at);
-                        if (!ok) s[r] = -__builtin_inff();
-                        see |= ok ? 1u << r : 0;
-                    }
+                    for (int r = 0; r < 16; r++) s[r] = mine >> (8 * (r >> 2) + (r & 3)) & 1 ? s[r] : -__builtin_inff();
                 }
                 move_max(s);
 #pragma unroll
@@ -1001,7 +1019,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
                     constexpr u32 E = std::is_same<T, half_t>::value ? 0x7c00u : 0x7f80u;
 #pragma unroll
                     for (int x = 0; x < L::TILE / 1024; x++) {
-                        const u4v v = lds_u4(smem_u + L::V + st + x * 1024 + lane * 16);
+                        const u4v v = lds_u4(smem_u + L::V + st + x * 1024 + lane_again() * 16);
 #pragma unroll
                         for (int e = 0; e < 4; e++) odd |= (v[e] & E) == E || (v[e] >> 16 & E) == E;
                     }
@@ -1012,13 +1030,13 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
                             for (int d = 0; d < DT; d++) {
                                 const u4v v = read_v(v_base + st, j, d);
 #pragma unroll 1
-                                for (int kk = 0; kk < 16; kk++) {  // value (kk & 3) + kk / 8 x 4 of the lanes with g = kk / 4 & 1: register 8 j + that
+                                for (int kk = 0; kk < 16; kk++) {  // value (kk & 3) + kk / 8 x 4 of the lanes with g = kk / 4 & 1
                                     const int e0 = (kk >> 3) * 4 + (kk & 3);
                                     u4v one;
 #pragma unroll
-                                    for (int e = 0; e < 4; e++) one[e] = (kk >> 2 & 1) == g && e0 >> 1 == e ? v[e] & (kk & 1 ? 0xffff0000u : 0xffffu) : 0;
+                                    for (int e = 0; e < 4; e++) one[e] = (kk >> 2 & 1) == (lane_again() >> 5) && e0 >> 1 == e ? v[e] & (kk & 1 ? 0xffff0000u : 0xffffu) : 0;
                                     const f16v x = product32<T>(one, pf[j], (f16v){});
-                                    if (__shfl(see >> (8 * j + e0) & 1, (kk >> 2 & 1) * 32 + lq)) o[d] += x;
+                                    if (seen >> (16 * j + kk) & 1) o[d] += x;
                                 }
                             }
                         return;
@@ -1175,11 +1193,13 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void tiles_kernel(PagedArgs 
     if (threadIdx.x == 0) ((Cut*)p.ws)[block] = cut;
 }
 
-// Adds up the parts of the tiles that the runs cut: workgroup (x, y) takes rows 4 y .. 4 y + 3 of the tile that run x began and did not
-// end, a wave per row; lanes 16 i .. 16 i + 15 take every fourth part from the i-th on, then the four sums meet. Also zeroes the rows
-// of no sequence, where the output was made for the call.
+// Adds up the parts of the tiles that the runs cut: workgroups (x, *) those of the tile that run x began and did not end, 16 lanes to a
+// row. Of few rows (MT <= 32: single tokens, whose caches are cut into many parts) a wave takes one, each group of 16 lanes every fourth
+// part, and the four sums meet; of 128 (cut in two or three) a wave takes four. Also zeroes the rows of no sequence, where the output was
+// made for the call.
 template <class T, int D, int MT>
 __global__ __launch_bounds__(256) void merge_kernel(PagedArgs p) {
+    constexpr bool MANY = MT <= 32;  // parts
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = (lane & 15) * (D / 16);
     if (p.fill && blockIdx.y == 0) {
         const int head = min(max(p.starts[0], 0), p.T), tail = min(max(p.starts[p.B], head), p.T);
@@ -1189,22 +1209,30 @@ __global__ __launch_bounds__(256) void merge_kernel(PagedArgs p) {
         }
     }
     const Cut cut = ((const Cut*)p.ws)[blockIdx.x];
-    const int tr = blockIdx.y * 4 + wave, row = cut.r0 + tr;
+    const int tr = MANY ? blockIdx.y * 4 + wave : blockIdx.y * 16 + wave * 4 + g, row = cut.r0 + tr;
     if (cut.more == 0 || row >= cut.rows) return;
     const int more = min(cut.more, p.grid - 1 - (int)blockIdx.x);
     auto part_of = [&](int i) __attribute__((always_inline)) { return (const float*)partial<MT, D>(p, blockIdx.x + i, i == 0); };
     float top = -__builtin_inff(), sum = 0.f, y[D / 16];
-    for (int i = lane; i <= more; i += 64) top = fmaxf(top, part_of(i)[MT * D + tr]);
-    top = rows_max(row_max16(top));
-    const float base = top == -__builtin_inff() ? 0.f : top;
-    for (int i = lane; i <= more; i += 64) sum = __builtin_fmaf(part_of(i)[MT * D + MT + tr], __builtin_amdgcn_exp2f(part_of(i)[MT * D + tr] - base), sum);
-    sum = rows_sum(row_sum16(sum));
+    float base;
+    if constexpr (MANY) {
+        for (int i = lane; i <= more; i += 64) top = fmaxf(top, part_of(i)[MT * D + tr]);
+        top = rows_max(row_max16(top));
+        base = top == -__builtin_inff() ? 0.f : top;
+        for (int i = lane; i <= more; i += 64) sum = __builtin_fmaf(part_of(i)[MT * D + MT + tr], __builtin_amdgcn_exp2f(part_of(i)[MT * D + tr] - base), sum);
+        sum = rows_sum(row_sum16(sum));
+    } else {
+#pragma unroll 4
+        for (int i = 0; i <= more; i++) top = fmaxf(top, part_of(i)[MT * D + tr]);
+        base = top;
+    }
 #pragma unroll
     for (int e = 0; e < D / 16; e++) y[e] = 0.f;
 #pragma unroll 4
-    for (int i = g; i <= more; i += 4) {
+    for (int i = MANY ? g : 0; i <= more; i += MANY ? 4 : 1) {
         const float* part = part_of(i);
         const float a = __builtin_amdgcn_exp2f(part[MT * D + tr] - base);
+        if constexpr (!MANY) sum = __builtin_fmaf(part[MT * D + MT + tr], a, sum);
 #pragma unroll
         for (int e = 0; e < D / 16; e += 4) {
             const f4 z = *(const f4*)(part + tr * D + c + e);
@@ -1212,15 +1240,14 @@ __global__ __launch_bounds__(256) void merge_kernel(PagedArgs p) {
             for (int k = 0; k < 4; k++) y[e + k] = __builtin_fmaf(z[k], a, y[e + k]);
         }
     }
+    if constexpr (MANY) {
 #pragma unroll
-    for (int e = 0; e < D / 16; e++) y[e] = rows_sum(y[e]);
-    if (g == 0) {
-        const int token = div_by(row, p.G), head = cut.kvh * (int)p.G.d + row - token * (int)p.G.d;
-        T* out = (T*)p.o + (long)(cut.first + token) * p.sot + head * p.soh + c;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-        for (int e = 0; e < D / 16; e++) out[e] = sum == 0.f ? (T)0.f : (T)(y[e] * inv);
+        for (int e = 0; e < D / 16; e++) y[e] = rows_sum(y[e]);
+        if (g != 0) return;
     }
+    const int token = div_by(row, p.G), head = cut.kvh * (int)p.G.d + row - token * (int)p.G.d;
+    T* out = (T*)p.o + (long)(cut.first + token) * p.sot + head * p.soh + c;
+    store_row<T, D>(out, y, sum);
 }
 
 // ------------------------------------------------------------------------------------------------ launches
@@ -1235,7 +1262,7 @@ static int make_plan(long T, long B, long H, long Hkv, long D, int type, Plan* p
     // Rows of a sequence and KV head, on average.
     const long rows = T * (H / Hkv) / B;
     plan->mt = rows <= 16 ? 16 : rows <= 32 || type == RDA_FP32 ? 32 : 128;
-    plan->grid = D == 128 || plan->mt == 32 ? 512 : 768;
+    plan->grid = (D == 128 && plan->mt == 16) || plan->mt == 32 ? 512 : 768;
     if ((T * (H / Hkv) / plan->mt + 1) * B >= 1L << 31) return RDA_ERR_INVALID;
     plan->workspace = (size_t)plan->grid * sizeof(Cut) + (size_t)plan->grid * 2 * plan->mt * (D + 2) * 4;
     return 0;
@@ -1262,7 +1289,7 @@ static int launch_tiles(const PagedArgs& a, void* stream) {
     if (a.S.d % 8 == 0 && a.kpr < 1u << 24 && a.vpr < 1u << 24) mod ? launch(tiles_kernel<T, D, true, true>) : launch(tiles_kernel<T, D, false, true>);
     else mod ? launch(tiles_kernel<T, D, true, false>) : launch(tiles_kernel<T, D, false, false>);
     if (const hipError_t e = hipGetLastError()) return (int)e;
-    hipLaunchKernelGGL((merge_kernel<T, D, 128>), dim3(a.grid, 32), dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL((merge_kernel<T, D, 128>), dim3(a.grid, 8), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 template <class T, int D>
@@ -1315,7 +1342,8 @@ int rda_paged_attn(const void* q, void* out, const void* k_pages, const void* v_
     a.window = window;
     // No more workgroups than units there can be: a short table of few sequences needs none that finds no work.
     const long least = plan.mt == 128 ? 32 : type == RDA_FP32 ? 64 : 128, units = (T * (H / Hkv) / plan.mt + B) * ((N * S + least - 1) / least) * Hkv;
-    a.grid = (int)(units < plan.grid ? units : plan.grid);
+    const int most = plan.mt == 128 && D == 128 && (softcap > 0.f || slopes) ? 512 : plan.grid;  // that kernel's registers leave two workgroups to a CU
+    a.grid = (int)(units < most ? units : most);
     a.runs = make_div(a.grid);
     a.fill = fill;
     const auto heads = [&](auto x) {
