@@ -45,7 +45,9 @@ struct PagedArgs {
 
 // ------------------------------------------------------------------------------------------------ the order of the work
 
-// A tile: rows r0 .. r1 of a sequence and the keys lo .. hi that any of them sees, in units of UK from lo (a multiple of UK).
+// A tile: rows r0 .. r1 of a sequence and the keys lo .. hi that any of them sees, in units of UK from lo (a multiple of UK). Its `units` are
+// AHEAD more than those of its keys, for what a tile costs before its first key; a run that would end or begin within the first AHEAD ends
+// or begins at the tile's start.
 struct WorkTile {
     int first, rows;  // the sequence's first row of q; its rows (tokens x heads)
     int r0, r1;       // the tile's rows, r1 included
@@ -59,7 +61,12 @@ __device__ __forceinline__ int seq_rows(const PagedArgs& p, int b, int& first) {
     const int end = min(max(p.starts[b + 1], first), p.T);
     return (end - first) * (int)p.G.d;
 }
-template <int MT, int UK>
+// What a tile costs before its first key, in units (us, units 0 / 6 / 8 / 12 / 18: 24 heads x 4096 causal tokens 281 / 228 / 221 / 219 / 213, a
+// chunk of 1001 beside 30 single tokens 95 / 76 / 74 / 75 / 75, 20 ragged chunks over caches 187 / 143 / 140 / 143 / 148; with changed scores,
+// whose units take twice as long, 0 / 6 / 12: 2 x 4096 capped 308 / 310 / 326, 5 biased prompts 79 / 83 / 89. Of 16 rows, units 0 / 1 / 2: 61
+// single tokens 144.7 / 140.3 / 142.0, 32 sequences of 5 tokens 130 / 123 / 130).
+__host__ __device__ constexpr int ahead(int mt, bool mod) { return mt == 128 ? (mod ? 2 : 8) : 1; }
+template <int MT, int UK, int AHEAD>
 __device__ __forceinline__ WorkTile make_tile(const PagedArgs& p, int b, int j) {
     WorkTile t;
     t.rows = seq_rows(p, b, t.first);
@@ -72,7 +79,7 @@ __device__ __forceinline__ WorkTile make_tile(const PagedArgs& p, int b, int j) 
     const int n0 = t.p0 + div_by(t.r0, p.G), n1 = t.p0 + div_by(max(t.r1, 0), p.G);
     t.hi = min(t.keys, max(n1 + 1, t.prefix));
     t.lo = p.window > 0 && t.prefix == 0 && n0 >= p.window ? (n0 - p.window + 1) / UK * UK : 0;
-    t.units = max((t.hi - t.lo + UK - 1) / UK, 1);  // a tile without keys is one unit: its rows are written too
+    t.units = AHEAD + max((t.hi - t.lo + UK - 1) / UK, 1);  // a tile without keys is one unit: its rows are written too
     return t;
 }
 
@@ -135,28 +142,45 @@ __device__ __forceinline__ u32 cut_run(const PagedArgs& p, u32 per_head, int blo
     run.count = (int)min((unsigned long long)run.quota, total - u0);
     return (u32)(u0 - (unsigned long long)run.kvh * per_head);
 }
+template <int AHEAD>
+__device__ __forceinline__ void begin_at_tile(Run& run) {
+    if (run.count > 0 && run.unit <= AHEAD) {
+        run.count += run.unit;
+        run.unit = 0;
+    }
+}
 // smem: B + 1 tile sums; shared: NT + 8 words.
-template <int MT, int UK, int NT>
+template <int MT, int UK, int AHEAD, int NT>
 __device__ __forceinline__ Run find_run(const PagedArgs& p, int* smem, u32* shared, int block) {
     const int t = threadIdx.x;
     u32* red = shared + NT;
     Run run = {};
-    // Up to 64 sequences of a tile each at most (a batch of single tokens): every wave by itself, a sequence per lane. (With a lane for
-    // each tile and the general search, a call of one token took 3 us longer.)
+    // Up to 64 sequences of up to 64 tiles together: every wave by itself, a lane for each. (The search below takes 3 us of a workgroup's time.)
     if (p.B <= 64) {
-        const int lane = t & 63, b = min(lane, p.B - 1);
+        const int lane = t & 63;
         int first;
-        const int rows = lane < p.B ? seq_rows(p, b, first) : 0;
-        if (!__any(rows > MT)) {
-            const u32 units = rows > 0 ? make_tile<MT, UK>(p, b, 0).units : 0, upto = scan_wave(units);
+        const u32 tiles = lane < p.B ? (u32)(seq_rows(p, lane, first) + MT - 1) / MT : 0, end = scan_wave(tiles);
+        if ((u32)__builtin_amdgcn_readlane((int)end, 63) <= 64) {
+            int b = lane;  // the lane's tile's sequence: the first whose tiles end past it
+            if (__any(lane < p.B && tiles != 1)) {
+                b = 0;
+#pragma unroll
+                for (int o = 32; o; o >>= 1)
+                    if ((int)__shfl(end, b + o - 1) <= lane) b += o;
+            }
+            const int before = (int)__shfl(end - tiles, min(b, 63)), all = __builtin_amdgcn_readlane((int)end, 63);
+            const u32 units = lane < all ? make_tile<MT, UK, AHEAD>(p, b, lane - before).units : 0, upto = scan_wave(units);
             const u32 s = cut_run(p, (u32)__builtin_amdgcn_readlane((int)upto, 63), block, run);
             if (run.count == 0) return run;
-            run.b = uniform((int)__builtin_ctzll(__ballot(upto > s)));
+            const int at = uniform((int)__builtin_ctzll(__ballot(upto > s)));
             run.kvh = uniform(run.kvh);
             run.count = uniform(run.count);
             run.quota = (u32)uniform((int)run.quota);
-            run.unit = uniform((int)(s - (u32)__builtin_amdgcn_readlane((int)(upto - units), run.b)));
-            run.tiles = 1;
+            run.b = __builtin_amdgcn_readlane(b, at);
+            run.j = at - __builtin_amdgcn_readlane(before, at);
+            run.tiles = __builtin_amdgcn_readlane((int)tiles, run.b);
+            run.unit = uniform((int)(s - (u32)__builtin_amdgcn_readlane((int)(upto - units), at)));
+            begin_at_tile<AHEAD>(run);
             return run;
         }
     }
@@ -190,7 +214,7 @@ __device__ __forceinline__ Run find_run(const PagedArgs& p, int* smem, u32* shar
     u32 units = 0;
     for (int i = t0; i < t1; i++) {
         while (smem[b + 1] <= i) b++;
-        units += make_tile<MT, UK>(p, b, i - smem[b]).units;
+        units += make_tile<MT, UK, AHEAD>(p, b, i - smem[b]).units;
     }
     const u32 upto = scan_block<NT>(units, red), from = upto - units;
     if (t == NT - 1) red[4] = upto;
@@ -203,7 +227,7 @@ __device__ __forceinline__ Run find_run(const PagedArgs& p, int* smem, u32* shar
         int bb = bt;
         for (int i = t0; i < t1; i++) {
             while (smem[bb + 1] <= i) bb++;
-            const u32 n = make_tile<MT, UK>(p, bb, i - smem[bb]).units;
+            const u32 n = make_tile<MT, UK, AHEAD>(p, bb, i - smem[bb]).units;
             if (s < at + n) {
                 shared[0] = bb;
                 shared[1] = i - smem[bb];
@@ -222,6 +246,7 @@ __device__ __forceinline__ Run find_run(const PagedArgs& p, int* smem, u32* shar
     run.tiles = uniform((int)shared[3]);
     run.count = run.tiles ? uniform(run.count) : 0;  // no tiles: sums past 32 bits (starts that fall)
     run.quota = (u32)uniform((int)run.quota);
+    begin_at_tile<AHEAD>(run);
     __syncthreads();
     return run;
 }
@@ -324,7 +349,7 @@ template <class T, int D, int MB, bool MOD, bool RUNS>
 __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(PagedArgs p) {
     using R = RowsTile<T>;
     constexpr bool FP32 = R::FP32;
-    constexpr int KT = R::KT, KG = R::KG, UK = R::UK, MT = 16 * MB;
+    constexpr int KT = R::KT, KG = R::KG, UK = R::UK, MT = 16 * MB, AHEAD = ahead(MT, MOD);
     constexpr int NB = KG / 4;              // score blocks of 16 keys
     constexpr int EV = 16 / sizeof(T);      // values of a 16-byte vector
     constexpr int KC = D / (4 * EV);        // 16-byte vectors of a lane's part of a K row
@@ -339,13 +364,14 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
     const int t = threadIdx.x, lane = t & 63, g = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int block = work_block(p.grid);
-    Run run = find_run<MT, UK, 256>(p, (int*)smem, shared, block);
+    Run run = find_run<MT, UK, AHEAD, 256>(p, (int*)smem, shared, block);
     Cut cut = {};
 
     while (run.count > 0) {
-        const WorkTile w = uniform(make_tile<MT, UK>(p, run.b, run.j));
-        const int u0 = run.unit, u1 = min(w.units, u0 + run.count), n = u1 - u0;
-        const bool whole = u0 == 0 && u1 == w.units;
+        const WorkTile w = uniform(make_tile<MT, UK, AHEAD>(p, run.b, run.j));
+        if (run.unit + run.count <= AHEAD) break;  // the next run's
+        const bool begins = run.unit == 0, last_part = run.unit + run.count >= w.units, whole = begins && last_part;
+        const int u0 = begins ? 0 : run.unit - AHEAD, u1 = min(w.units, run.unit + run.count) - AHEAD, n = u1 - u0;
         const int* table = p.table + run.b * p.pitch;
         const T* kbase = (const T*)p.k + run.kvh * p.kph;
         const T* vbase = (const T*)p.v + run.kvh * p.vph;
@@ -670,7 +696,7 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
                     store_row<T, D>(out, y, sum);
                 }
             } else {
-                float* part = partial<MT, D>(p, block, u0 == 0);
+                float* part = partial<MT, D>(p, block, begins);
 #pragma unroll
                 for (int e = 0; e < D / 16; e += 4) *(f4*)(part + tr * D + c + e) = (f4){y[e], y[e + 1], y[e + 2], y[e + 3]};
                 if (c == 0) {
@@ -680,14 +706,14 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
             }
         }
         __syncthreads();
-        if (u0 == 0 && u1 < w.units) {
-            cut.more = (int)((w.units - u1 + run.quota - 1) / run.quota);
+        if (begins && !last_part) {
+            cut.more = (int)((w.units - run.count + run.quota - 1) / run.quota);
             cut.kvh = run.kvh;
             cut.first = w.first;
             cut.rows = w.rows;
             cut.r0 = w.r0;
         }
-        run.count -= n;
+        run.count -= min(w.units - run.unit, run.count);
         run.unit = 0;
         if (run.count > 0) next_tile<MT>(p, run);
     }
@@ -752,22 +778,23 @@ __device__ __forceinline__ int lane_again() {
 
 template <class T, int D, bool MOD, bool RUNS>
 __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(PagedArgs p) {
-    constexpr int MT = 128, UK = 32, ROW = 2 * D, KS = D / 16, DT = D / 32;  // KS: products of a score block; DT: of a 16-key step with V
+    constexpr int MT = 128, UK = 32, AHEAD = ahead(MT, MOD), ROW = 2 * D, KS = D / 16, DT = D / 32;  // KS: products of a score block; DT: of a 16-key step with V
     constexpr int CP = D / 64, CR = 1024 / ROW;  // a wave's copies of K per tile; rows of a copy
     using L = TilesLds<D>;
     extern __shared__ __attribute__((aligned(256))) char smem[];
     const int lane = threadIdx.x & 63, g = lane >> 5, lq = lane & 31;
     const int wave = uniform((int)(threadIdx.x >> 6));
     const int block = work_block(p.grid);
-    Run run = find_run<MT, UK, 256>(p, (int*)smem, (u32*)(smem + L::SHARED), block);
-    int* flag = (int*)(smem + L::SHARED) + 256 + 8;
+    Run run = find_run<MT, UK, AHEAD, 256>(p, (int*)smem, (u32*)(smem + L::SHARED), block);
+    int* flags = (int*)(smem + L::SHARED) + 256 + 8;  // a wave's: whether the cache lacks a page that it looked up
     Cut cut = {};
     const u32 smem_u = lds_addr(smem);
 
     while (run.count > 0) {
-        const WorkTile w = uniform(make_tile<MT, UK>(p, run.b, run.j));
-        const int u0 = run.unit, u1 = min(w.units, u0 + run.count), n = w.hi > w.lo ? u1 - u0 : 0;
-        const bool whole = u0 == 0 && u1 == w.units;
+        const WorkTile w = uniform(make_tile<MT, UK, AHEAD>(p, run.b, run.j));
+        if (run.unit + run.count <= AHEAD) break;  // the next run's
+        const bool begins = run.unit == 0, last_part = run.unit + run.count >= w.units, whole = begins && last_part;
+        const int u0 = begins ? 0 : run.unit - AHEAD, u1 = min(w.units, run.unit + run.count) - AHEAD, n = w.hi > w.lo ? u1 - u0 : 0;
         const int* table = p.table + run.b * p.pitch;
         const T* kbase = uniform((const T*)p.k + run.kvh * p.kph);
         const T* vbase = uniform((const T*)p.v + run.kvh * p.vph);
@@ -825,12 +852,6 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
 #pragma unroll
             for (int c = 0; c < CP; c++) first[c] = id[c];
             fetch(min(1, n - 1));
-            const int e0 = div_by(key_first, p.S), e1 = div_by(min(key_first + n * UK, w.hi) - 1, p.S);
-            bool hole = false;
-            for (int e = e0 + (int)threadIdx.x; e <= e1; e += 256) hole |= (u32)table[e] >= (u32)p.P;
-            if (threadIdx.x == 0) *flag = 0;
-            __syncthreads();
-            if (hole) *flag = 1;
             int second[CP];
 #pragma unroll
             for (int c = 0; c < CP; c++) second[c] = id[c], id[c] = first[c];
@@ -839,6 +860,11 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
             for (int c = 0; c < CP; c++) id[c] = second[c];
             if (n > 1) issue(1, L::TILE);
             if (n > 2) fetch(2);
+            const int e1 = div_by(min(key_first + n * UK, w.hi) - 1, p.S);
+            bool hole = false;
+            for (int e = div_by(key_first, p.S) + (int)threadIdx.x; e <= e1; e += 256) hole |= (u32)table[e] >= (u32)p.P;
+            hole = __any(hole);
+            if (lane_again() == 0) flags[wave] = hole;
         }
 
         f16v o[DT];
@@ -993,26 +1019,23 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
             int full0 = 0, full1 = 0;
             const int ends = min(n, (w.hi - key_first) / UK);
 
-            // One tile from its scores on, wherever it lies: scores, maximum, P, product, one after the other.
-            auto plain_step = [&](int i, u32 st) __attribute__((always_inline)) {
-                const int key0 = key_of(i);
-                const bool masked = i < full0 || i >= full1;
-                float s[16];
-                u32 seen = ~0u;
-                if (masked) {
-                    seen = seen_keys(key0);
-                    if (!__any(seen != 0)) return;
-                }
-                qk(st, s, no_hook);
-                bias(s, key0);
+            // A tile's first part, wherever it lies: its scores, masked where not every row sees every key, the maximum, and the first half of P;
+            // and its second, with one look at values that only some rows see.
+            float sa[16], sb[16];
+            auto begin_tile = [&](int i, u32 st, u32 seen, bool masked) __attribute__((always_inline)) {
+                qk(st, sa, no_hook);
+                bias(sa, key_of(i));
                 if (masked) {
                     const u32 mine = seen >> (4 * (lane_again() >> 5));  // register r: key 8 (r / 4) + 4 g + r % 4
 #pragma unroll
-                    for (int r = 0; r < 16; r++) s[r] = mine >> (8 * (r >> 2) + (r & 3)) & 1 ? s[r] : -__builtin_inff();
+                    for (int r = 0; r < 16; r++) sa[r] = mine >> (8 * (r >> 2) + (r & 3)) & 1 ? sa[r] : -__builtin_inff();
                 }
-                move_max(s);
+                move_max(sa);
+                l_old = l;
 #pragma unroll
-                for (int k = 0; k < 8; k++) exps(s, k);
+                for (int k = 0; k < 4; k++) exps(sa, k);
+            };
+            auto end_tile = [&](u32 st, u32 seen, bool masked) __attribute__((always_inline)) {
                 if (masked) {
                     // Values that are not finite, of keys that only some rows see: key by key.
                     bool odd = false;
@@ -1023,7 +1046,7 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
 #pragma unroll
                         for (int e = 0; e < 4; e++) odd |= (v[e] & E) == E || (v[e] >> 16 & E) == E;
                     }
-                    if (__any(odd)) {
+                    if (__builtin_expect(__any(odd), 0)) {
 #pragma unroll
                         for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -1068,7 +1091,7 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
             if (n > 0) {
                 wait_copies();
                 __syncthreads();
-                holes = uniform(*flag) != 0;
+                holes = uniform(flags[0] | flags[1] | flags[2] | flags[3]) != 0;
                 if (!holes) {
                     const int upto = min(w.hi, p.window > 0 ? n0 + 1 : max(n0 + 1, w.prefix));
                     full0 = p.window > 0 ? max(n1 - p.window + UK - key_first, 0) / UK : 0;  // the first tile with key0 > n1 - window
@@ -1085,37 +1108,48 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
                 st2 = x;
             };
             for (int i = 0; i < n;) {
-                bool copied = false;  // whether tile i + 2 is on its way already
-                if (i >= full0 && i <= last) {
-                    float sa[16], sb[16];
-                    qk(st, sa, no_hook);
-                    bias(sa, key_of(i));
-                    move_max(sa);
-                    l_old = l;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) exps(sa, k);
-                    while (true) {
-                        if (!full_step(i, st, st1, st2, sa, sb)) {
-                            copied = true;
-                            break;
-                        }
-                        i++;
-                        turn_stages();
-                        if (!full_step(i, st, st1, st2, sb, sa)) {
-                            copied = true;
-                            break;
-                        }
-                        i++;
-                        turn_stages();
-                        if (i > last) break;
-                    }
-                    l = l_old;  // tile i is begun again
-                }
-                if (!copied && i + 2 < n) {
+                const bool masked = i < full0 || i >= full1;
+                u32 seen = ~0u;
+                if (masked) seen = seen_keys(key_of(i));
+                bool full = i >= full0 && i <= last, copied = false;  // whether tile i + 2 is on its way
+                if (!full && i + 2 < n) {
                     issue(i + 2, st2);
                     if (i + 3 < n) fetch(i + 3);
+                    copied = true;
                 }
-                plain_step(i, st);
+                if (__any(seen != 0)) {
+                    while (true) {
+                        begin_tile(i, st, seen, masked);
+                        bool done = true, taken = true;  // taken: the tile's maximum is
+                        while (full) {
+                            taken = false;
+                            done = full_step(i, st, st1, st2, sa, sb);
+                            if (!done) break;
+                            i++;
+                            turn_stages();
+                            done = full_step(i, st, st1, st2, sb, sa);
+                            if (!done) break;
+                            i++;
+                            turn_stages();
+                            full = i <= last;
+                        }
+                        if (done) {
+                            if (!copied && i + 2 < n) {
+                                issue(i + 2, st2);
+                                if (i + 3 < n) fetch(i + 3);
+                            }
+                            copied = true;
+#pragma unroll
+                            for (int k = 4; k < 8; k++) exps(sa, k);
+                            if (taken || !__any(!(l <= l_old + 64.f))) break;
+                        }
+                        // P above the maximum at hand (a full step's look, or the last tile's after full steps): the tile again, its copies made.
+                        l = l_old;
+                        copied = true;
+                        full = false;
+                    }
+                    end_tile(st, seen, masked);
+                }
                 i++;
                 turn_stages();
                 wait_copies();
@@ -1154,7 +1188,7 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
                     }
                 }
             } else {
-                float* part = partial<MT, D>(p, block, u0 == 0);
+                float* part = partial<MT, D>(p, block, begins);
 #pragma unroll
                 for (int half = 0; half < D / 64; half++) {  // 64 values of fp32 at a time
 #pragma unroll
@@ -1179,14 +1213,14 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
             }
         }
         __syncthreads();
-        if (u0 == 0 && u1 < w.units) {
-            cut.more = (int)((w.units - u1 + run.quota - 1) / run.quota);
+        if (begins && !last_part) {
+            cut.more = (int)((w.units - run.count + run.quota - 1) / run.quota);
             cut.kvh = run.kvh;
             cut.first = w.first;
             cut.rows = w.rows;
             cut.r0 = w.r0;
         }
-        run.count -= u1 - u0;
+        run.count -= min(w.units - run.unit, run.count);
         run.unit = 0;
         if (run.count > 0) next_tile<MT>(p, run);
     }
@@ -1324,7 +1358,7 @@ int rda_paged_attn(const void* q, void* out, const void* k_pages, const void* v_
         !vector_rows(v_pages, dims + 16, 3, type))
         return RDA_ERR_INVALID;
     // Units of a KV head in 32 bits, whatever the lengths.
-    if ((T * (H / Hkv) / plan.mt + B) * (N * S / 64 + 1) >= 1L << 32) return RDA_ERR_INVALID;
+    if ((T * (H / Hkv) / plan.mt + B) * (N * S / 32 + 1 + ahead(plan.mt, false)) >= 1L << 32) return RDA_ERR_INVALID;
     for (int i : {13, 14, 16, 17})
         if (dims[i] < 0 || dims[i] >= 1L << 32) return RDA_ERR_INVALID;
     PagedArgs a;
@@ -1341,7 +1375,7 @@ int rda_paged_attn(const void* q, void* out, const void* k_pages, const void* v_
     a.cap = softcap * LOG2E;
     a.window = window;
     // No more workgroups than units there can be: a short table of few sequences needs none that finds no work.
-    const long least = plan.mt == 128 ? 32 : type == RDA_FP32 ? 64 : 128, units = (T * (H / Hkv) / plan.mt + B) * ((N * S + least - 1) / least) * Hkv;
+    const long least = plan.mt == 128 ? 32 : type == RDA_FP32 ? 64 : 128, units = (T * (H / Hkv) / plan.mt + B) * ((N * S + least - 1) / least + ahead(plan.mt, false)) * Hkv;
     const int most = plan.mt == 128 && D == 128 && (softcap > 0.f || slopes) ? 512 : plan.grid;  // that kernel's registers leave two workgroups to a CU
     a.grid = (int)(units < most ? units : most);
     a.runs = make_div(a.grid);
