@@ -974,15 +974,17 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
                 asm volatile("" : "+v"(d), "+v"(l));
             };
             auto no_hook = [](int) {};
-            // m moves only where a tile's maximum exceeds it by more than 8.
+            // m moves only where a row's maximum of a tile exceeds it by more than 2: a lane's 16 values of P then add up to at most 64, which full
+            // steps (below) look for. (With more than 8, as in the rows kernel, rows whose first keys score low went on at 6 to 8 above m, and
+            // took each tile twice: 2 x 4096 in a window of 2048, whose rows begin with few keys, ran half of its workgroups at half speed.)
             auto move_max = [&](const float (&x)[16]) __attribute__((always_inline)) {
                 float mx = x[0];
 #pragma unroll
                 for (int r = 1; r < 16; r++) mx = fmaxf(mx, x[r]);
                 const f2 h = both_halves(mx);
                 mx = fmaxf(h[0], h[1]) * scale;
-                if (__any(mx > m + 8.f)) {
-                    const float mn = mx > m + 8.f ? mx : m, a = __builtin_amdgcn_exp2f(m - mn);
+                if (__any(mx > m + 2.f)) {
+                    const float mn = fmaxf(m, mx), a = __builtin_amdgcn_exp2f(m - mn);
                     m = mn;
                     l *= a;
 #pragma unroll
