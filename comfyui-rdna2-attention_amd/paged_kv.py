@@ -9,7 +9,7 @@ import torch
 
 from . import _lib
 from .hip_attention import Kernels
-from .rotary import TYPES, rows_ready, same_device, vector_rows
+from .rotary import TYPES, Sizes, rows_ready, same_device, vector_rows
 
 HEADS = (64, 128)  # head dims of `attention`
 MAX_SEQUENCES = 8192
@@ -37,7 +37,11 @@ class Cache:
             raise ValueError("Cache takes k and v with a contiguous last dimension and rows on 16-byte boundaries")
         if k.device != v.device:
             raise ValueError("Cache takes k and v on one device")
-        self.k, self.v = k, v
+        self._k, self._v = k, v
+        self.sizes = (k.dtype, k.shape, k.stride(), v.stride())
+
+    k = property(lambda self: self._k, doc="The pages of the keys.")
+    v = property(lambda self: self._v, doc="The pages of the values.")
 
 
 class Batch:
@@ -57,16 +61,32 @@ class Batch:
             raise ValueError("Batch takes a table with contiguous rows, and contiguous starts and lengths")
         if not table.device == starts.device == lengths.device:
             raise ValueError("Batch takes its tensors on one device")
-        self.table, self.starts, self.lengths = table, starts, lengths
+        self._table, self._starts, self._lengths = table, starts, lengths
+        self.sizes = (table.shape, table.stride(0))
+
+    def _replace(name):
+        def put(self, t):  # also what batch.lengths += 1 does, with the tensor itself
+            old = getattr(self, name)
+            if t is not old and (t.dtype != old.dtype or t.shape != old.shape or t.stride() != old.stride() or t.device != old.device):
+                raise ValueError(f"Batch keeps the type, shape, strides and device of its {name[1:]}")
+            setattr(self, name, t)
+        return property(lambda self: getattr(self, name), put)
+
+    table, starts, lengths = _replace("_table"), _replace("_starts"), _replace("_lengths")
+    del _replace
 
 
 def _sizes(what, cache, batch):
     """(sequences, pages per sequence, table pitch, pages, page size), checked."""
-    B, N = batch.table.shape
+    (B, N), pitch = batch.sizes
     P, S = cache.k.shape[:2]
     if N * S > MAX_KEYS:
         raise ValueError(f"{what} takes tables of at most {MAX_KEYS} tokens a sequence")
-    return B, N, batch.table.stride(0), P, S
+    return B, N, pitch, P, S
+
+
+_append_sizes, _attention_sizes = Sizes(), Sizes()
+_workspaces = {}  # bytes by sizes
 
 
 def append(cache, batch, k, v, rotary=None, q=None, q_out=None):
@@ -75,39 +95,62 @@ def append(cache, batch, k, v, rotary=None, q=None, q_out=None):
     and v are fp16, bf16 or fp32, of the cache's type or another: rounded to it once, after the turn. q (tokens, heads, D), if
     given, is turned in the same launch into q_out (the cache's type; None: in place) -- what attention takes. Rows of no
     sequence are left as they were in q_out, as is the cache where a position is negative, past the table or on a page that it does not
-    have. Two tokens on one row of one page: either may remain. Returns q_out."""
+    have. Two tokens on one row of one page: either may remain. q_out is q itself or does not overlap q, k and v. Returns q_out."""
+    kc, vc = cache._k, cache._v
+    if q is not None:
+        if q_out is None:
+            q_out = q
+        if q.data_ptr() % 16 and q_out is not q:
+            q = q.clone(memory_format=torch.contiguous_format)
+    if k.data_ptr() % 16 or v.data_ptr() % 16:
+        k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
+    key = (cache.sizes, batch.sizes, k.dtype, k.shape, k.stride(), v.dtype, v.shape, v.stride(), 0 if rotary is None else rotary.dim,
+           None if q is None else (q.dtype, q.shape, q.stride()), None if q_out is None else (q_out.dtype, q_out.shape, q_out.stride()))
+    dims = _append_sizes.get(key)
+    if dims is None:
+        k, v, q, dims = _check_append(cache, batch, k, v, rotary, q, q_out, key)
+    same_device("append", kc, batch._table, k, v, q, q_out, None if rotary is None else rotary.turns)
+    if q_out is not None and q_out.data_ptr() % 16:
+        raise ValueError(Q_OUT_ERROR)
+    if k.shape[0] == 0:
+        return q_out
+    _lib.check(get_kernels().paged_append(None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), None if q is None else q_out.data_ptr(),
+                                          kc.data_ptr(), vc.data_ptr(), batch._table.data_ptr(), batch._starts.data_ptr(), batch._lengths.data_ptr(),
+                                          None if rotary is None else rotary.turns.data_ptr(), 1.0 if rotary is None else rotary.factor,
+                                          0 if rotary is None else rotary.interleaved, TYPES[k.dtype], TYPES[kc.dtype], dims, _lib.raw_stream()))
+    return q_out
+
+
+Q_OUT_ERROR = "append's q_out has q's shape and the cache's type, a contiguous last dimension and rows on 16-byte boundaries"
+
+
+def _check_append(cache, batch, k, v, rotary, q, q_out, key):
+    """(k, v and q, copied where the kernel cannot address them; the size arguments) of an append call, or ValueError."""
     kc, vc = cache.k, cache.v
-    _, S, Hkv, D = kc.shape
+    _, _, Hkv, D = kc.shape
     if k.dim() != 3 or k.dtype not in TYPES or k.shape[1:] != (Hkv, D) or v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError(f"append takes k and v as (tokens, {Hkv}, {D}) of one type: fp16, bf16 or fp32")
     if D > 256 or (rotary is not None and rotary.dim > D):
         raise ValueError("append takes heads of at most 256 values, and no more rotated ones than these")
     T, H = k.shape[0], 0
     if q is not None:
-        if q_out is None:
-            q_out = q
         H = q.shape[1] if q.dim() == 3 else 0
         if q.dim() != 3 or q.dtype != k.dtype or q.shape[0] != T or q.shape[2] != D or H == 0:
             raise ValueError(f"append takes q as ({T}, heads, {D}) of k's type")
         if q_out.shape != q.shape or q_out.dtype != kc.dtype or not (T == 0 or rows_ready(q_out)):
-            raise ValueError("append's q_out has q's shape and the cache's type, a contiguous last dimension and rows on 16-byte boundaries")
+            raise ValueError(Q_OUT_ERROR)
     elif q_out is not None:
         raise ValueError("append takes q_out with q only")
     B, N, pitch, P, S = _sizes("append", cache, batch)
-    same_device("append", kc.device, batch.table, k, v, q, q_out, None if rotary is None else rotary.turns)
     if H + 2 * Hkv > 65535:
         raise ValueError("append takes at most 65535 heads")
-    if T == 0:
-        return q_out
-    k, v = vector_rows(k), vector_rows(v)
-    src = None if q is None else vector_rows(q)
-    dims = _lib.long_array([T, H, Hkv, D, 0 if rotary is None else rotary.dim, B, N, pitch, P, S, *((0, 0) if q is None else src.stride()[:2]), *k.stride()[:2],
-                            *v.stride()[:2], *((0, 0) if q is None else q_out.stride()[:2]), *kc.stride()[:3], *vc.stride()[:3]])
-    _lib.check(get_kernels().paged_append(None if q is None else src.data_ptr(), k.data_ptr(), v.data_ptr(), None if q is None else q_out.data_ptr(),
-                                          kc.data_ptr(), vc.data_ptr(), batch.table.data_ptr(), batch.starts.data_ptr(), batch.lengths.data_ptr(),
-                                          None if rotary is None else rotary.turns.data_ptr(), 1.0 if rotary is None else rotary.factor,
-                                          0 if rotary is None else rotary.interleaved, TYPES[k.dtype], TYPES[kc.dtype], dims, _lib.raw_stream()))
-    return q_out
+    ready = T == 0 or all(rows_ready(t) for t in (k, v) + (() if q is None else (q,)))
+    if not ready:
+        k, v, q = vector_rows(k), vector_rows(v), None if q is None else vector_rows(q)
+    none = (0, 0)
+    values = [T, H, Hkv, D, 0 if rotary is None else rotary.dim, B, N, pitch, P, S, *(none if q is None else q.stride()[:2]), *k.stride()[:2], *v.stride()[:2],
+              *(none if q is None else q_out.stride()[:2]), *kc.stride()[:3], *vc.stride()[:3]]
+    return k, v, q, _append_sizes.keep(key, values) if ready else _lib.long_array(values)
 
 
 def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slopes=None, prefix=None):
@@ -115,38 +158,64 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     A token at position n (its own key included) sees the keys j <= n; with window > 0 those with n - j < window; with prefix (int32,
     one per sequence) also those j < prefix[b], ahead of it or behind the window. Scores are scale q.k (scale None: D^-0.5); with
     softcap > 0, softcap tanh(scale q.k / softcap); with slopes (fp32, one per head), less slopes[h] |n - j|. heads is a multiple of
-    the cache's KV heads, which they share in order. A token that sees nothing gets 0. Returns out (q's shape; rows of no sequence
-    left as they were), or a new tensor, with those rows 0. out does not overlap q."""
+    the cache's KV heads, which they share in order. A token that sees nothing gets 0. Returns out (q's shape, not overlapping q; rows of no
+    sequence left as they were), or a new tensor, with those rows 0."""
+    kc, vc = cache._k, cache._v
+    fill = out is None
+    if fill:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    key = (cache.sizes, batch.sizes, q.dtype, q.shape, q.stride(), out.dtype, out.shape, out.stride(),
+           None if slopes is None else (slopes.dtype, slopes.shape, slopes.stride()), None if prefix is None else (prefix.dtype, prefix.shape, prefix.stride()))
+    dims = _attention_sizes.get(key)
+    if dims is None:
+        q, dims = _check_attention(cache, batch, q, out, slopes, prefix, key)
+    if not softcap >= 0.0 or not 0 <= window < 2 ** 31:
+        raise ValueError("attention takes softcap >= 0 and 0 <= window < 2^31 (0: none)")
+    same_device("attention", kc, batch._table, q, out, slopes, prefix)
+    if q.numel() == 0:
+        return out
+    address = out.data_ptr()
+    if address % 16:
+        raise ValueError(OUT_ERROR)
+    if address == q.data_ptr():
+        raise ValueError("attention's out is not q: rows are written while others' queries are still read")
+    T, H, Hkv, D, B = dims[:5]
+    type_ = TYPES[q.dtype]
+    k = get_kernels()
+    sizes = (T, B, H, Hkv, D, type_)
+    size = _workspaces.get(sizes)
+    if size is None:
+        size = _workspaces[sizes] = k.paged_attn_workspace(*sizes)
+    workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    _lib.check(k.paged_attn(q.data_ptr(), address, kc.data_ptr(), vc.data_ptr(), batch._table.data_ptr(), batch._starts.data_ptr(), batch._lengths.data_ptr(),
+                            None if prefix is None else prefix.data_ptr(), None if slopes is None else slopes.data_ptr(), workspace.data_ptr(),
+                            D ** -0.5 if scale is None else scale, softcap, window, fill, type_, dims, _lib.raw_stream()))
+    return out
+
+
+OUT_ERROR = "attention's out has q's shape and type, a contiguous last dimension and rows on 16-byte boundaries"
+
+
+def _check_attention(cache, batch, q, out, slopes, prefix, key):
+    """(q, copied where the kernel cannot address it; the size arguments) of an attention call, or ValueError."""
     kc, vc = cache.k, cache.v
-    _, S, Hkv, D = kc.shape
+    _, _, Hkv, D = kc.shape
     if q.dim() != 3 or q.dtype != kc.dtype or D not in HEADS or q.shape[2] != D or q.shape[1] == 0 or q.shape[1] % Hkv:
         raise ValueError(f"attention takes q as (tokens, a multiple of {Hkv} heads, {D}) of the cache's type {kc.dtype}, head dim 64 or 128")
     T, H = q.shape[:2]
     B, N, pitch, P, S = _sizes("attention", cache, batch)
-    fill = out is None
-    if fill:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not (T == 0 or rows_ready(out)):
-        raise ValueError("attention's out has q's shape and type, a contiguous last dimension and rows on 16-byte boundaries")
-    elif T and out.data_ptr() == q.data_ptr():
-        raise ValueError("attention's out is not q: rows are written while others' queries are still read")
-    if not softcap >= 0.0 or window < 0 or window >= 2 ** 31:
-        raise ValueError("attention takes softcap >= 0 and 0 <= window < 2^31 (0: none)")
+    if out.shape != q.shape or out.dtype != q.dtype or not (T == 0 or rows_ready(out)):
+        raise ValueError(OUT_ERROR)
     if slopes is not None and (slopes.dtype != torch.float32 or slopes.numel() != H or not slopes.is_contiguous()):
         raise ValueError(f"attention takes slopes as {H} contiguous fp32 values")
     if prefix is not None and (prefix.dtype != torch.int32 or prefix.numel() != B or not prefix.is_contiguous()):
         raise ValueError(f"attention takes prefix as {B} contiguous int32 values")
     if T * (H // Hkv) >= 2 ** 31:
         raise ValueError("attention takes fewer than 2^31 rows of tokens and heads per KV head")
-    same_device("attention", kc.device, batch.table, q, out, slopes, prefix)
-    if T == 0:
-        return out
-    q = vector_rows(q)
-    type_ = TYPES[q.dtype]
-    kernels_ = get_kernels()
-    workspace = torch.empty(kernels_.paged_attn_workspace(T, B, H, Hkv, D, type_), dtype=torch.uint8, device=q.device)
-    dims = _lib.long_array([T, H, Hkv, D, B, N, pitch, P, S, *q.stride()[:2], *out.stride()[:2], *kc.stride()[:3], *vc.stride()[:3]])
-    _lib.check(kernels_.paged_attn(q.data_ptr(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), batch.table.data_ptr(), batch.starts.data_ptr(),
-                                   batch.lengths.data_ptr(), None if prefix is None else prefix.data_ptr(), None if slopes is None else slopes.data_ptr(),
-                                   workspace.data_ptr(), D ** -0.5 if scale is None else scale, softcap, window, int(fill), type_, dims, _lib.raw_stream()))
-    return out
+    ready = T == 0 or rows_ready(q)
+    if not ready:
+        q = vector_rows(q)
+    values = [T, H, Hkv, D, B, N, pitch, P, S, *q.stride()[:2], *out.stride()[:2], *kc.stride()[:3], *vc.stride()[:3]]
+    return q, _attention_sizes.keep(key, values) if ready else _lib.long_array(values)

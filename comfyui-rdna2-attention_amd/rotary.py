@@ -104,13 +104,29 @@ def rows_ready(t):
     return True
 
 
-def same_device(what, device, *tensors):
-    """Raises ValueError unless every tensor is on `device`, and it is the current one: the kernels run on its current stream."""
+def same_device(what, *tensors):
+    """Raises ValueError unless every tensor (None: none) is on the current GPU: the kernels run on its current stream."""
+    device = -1
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what} takes tensors of one device, not {device} and {t.device}")
-    if device.type != "cuda" or device.index != torch.cuda.current_device():
-        raise ValueError(f"{what} runs on the current GPU; its tensors are on {device}")
+        if t is not None:
+            d = t.get_device()
+            if device == -1:
+                device = d if d >= 0 and d == torch._C._cuda_getDevice() else -2
+            if d != device:
+                raise ValueError(f"{what} runs on the current GPU; its tensors are on {', '.join(sorted({str(x.device) for x in tensors if x is not None}))}")
+
+
+class Sizes(dict):
+    """The size arguments of an operator's calls by their tensors' types, shapes and strides: checked and packed once for each."""
+
+    def keep(self, key, values):
+        if len(self) >= 4096:
+            self.clear()
+        self[key] = value = _lib.long_array(values)
+        return value
+
+
+_rotate_sizes = Sizes()
 
 
 def rotate(x, positions, rotary, out=None, inverse=False):
@@ -119,24 +135,41 @@ def rotate(x, positions, rotary, out=None, inverse=False):
     turn in 32, rounded once. Values past rotary.dim are copied. inverse turns back: the gradient of x for a gradient of the result
     (and, where rotary.factor is 1, x itself). Any strides of x with a contiguous last dimension (other heads-first
     layouts are views of these shapes); out, if given, is x itself or does not overlap it. Returns out, or a new contiguous tensor."""
-    if x.dim() not in (3, 4) or x.dtype not in TYPES or x.shape[-1] % 16 or not rotary.dim <= x.shape[-1] <= MAX_HEAD:
-        raise ValueError(f"rotate takes (tokens, heads, D) or (batch, length, heads, D) in fp16, bf16 or fp32, D a multiple of 16 from {rotary.dim} "
-                         f"to {MAX_HEAD}, not {tuple(x.shape)} {x.dtype}")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != x.shape[:-2]:
-        raise ValueError(f"rotate takes int32 or int64 positions of shape {tuple(x.shape[:-2])}, not {tuple(positions.shape)} {positions.dtype}")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or not (out.numel() == 0 or rows_ready(out)):
-        raise ValueError("rotate's out has x's shape and type, a contiguous last dimension and rows on 16-byte boundaries")
-    same_device("rotate", x.device, positions, rotary.turns, out)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    positions = positions.contiguous()
+    key = (x.dtype, x.shape, x.stride(), out.dtype, out.shape, out.stride(), positions.dtype, positions.shape, rotary.dim)
+    dims = _rotate_sizes.get(key)
+    if dims is None:
+        x, dims = _check_rotate(x, positions, rotary, out, key)
+    same_device("rotate", x, positions, rotary.turns, out)
+    if out.data_ptr() % 16:
+        raise ValueError(OUT_ERROR)
     if x.numel() == 0:
         return out
-    if x.shape[-2] > 65535:
-        raise ValueError("rotate takes at most 65535 heads")
-    x, positions = vector_rows(x), positions.contiguous()
-    B, L = (1, x.shape[0]) if x.dim() == 3 else x.shape[:2]
-    sx, so = x.stride(), out.stride()
-    dims = _lib.long_array([B, L, x.shape[-2], x.shape[-1], rotary.dim, *(sx[:3] if x.dim() == 4 else (0, *sx[:2])), *(so[:3] if x.dim() == 4 else (0, *so[:2]))])
-    _lib.check(get_kernels().rotate_positions(x.data_ptr(), out.data_ptr(), positions.data_ptr(), int(positions.dtype == torch.int64), rotary.turns.data_ptr(),
+    _lib.check(get_kernels().rotate_positions(x.data_ptr(), out.data_ptr(), positions.data_ptr(), positions.dtype is torch.int64, rotary.turns.data_ptr(),
                                               rotary.factor, rotary.interleaved + 2 * bool(inverse), TYPES[x.dtype], dims, _lib.raw_stream()))
     return out
+
+
+OUT_ERROR = "rotate's out has x's shape and type, a contiguous last dimension and rows on 16-byte boundaries"
+
+
+def _check_rotate(x, positions, rotary, out, key):
+    """(x, copied where the kernel cannot address it; the size arguments) of a rotate call, or ValueError."""
+    if x.dim() not in (3, 4) or x.dtype not in TYPES or x.shape[-1] % 16 or not rotary.dim <= x.shape[-1] <= MAX_HEAD or x.shape[-2] > 65535:
+        raise ValueError(f"rotate takes (tokens, heads, D) or (batch, length, heads, D) in fp16, bf16 or fp32, D a multiple of 16 from {rotary.dim} "
+                         f"to {MAX_HEAD}, at most 65535 heads, not {tuple(x.shape)} {x.dtype}")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != x.shape[:-2]:
+        raise ValueError(f"rotate takes int32 or int64 positions of shape {tuple(x.shape[:-2])}, not {tuple(positions.shape)} {positions.dtype}")
+    if out.shape != x.shape or out.dtype != x.dtype or not (out.numel() == 0 or rows_ready(out)):
+        raise ValueError(OUT_ERROR)
+    ready = x.numel() == 0 or rows_ready(x)
+    if not ready:
+        x = x.clone(memory_format=torch.contiguous_format)
+    B, L = (1, x.shape[0]) if x.dim() == 3 else x.shape[:2]
+    sx, so = x.stride(), out.stride()
+    values = [B, L, x.shape[-2], x.shape[-1], rotary.dim, *(sx[:3] if x.dim() == 4 else (0, *sx[:2])), *(so[:3] if x.dim() == 4 else (0, *so[:2]))]
+    return x, _rotate_sizes.keep(key, values) if ready else _lib.long_array(values)

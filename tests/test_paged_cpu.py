@@ -94,6 +94,20 @@ def test_cache_and_batch_refusals():
             paged_kv.Batch(*bad)
 
 
+def test_handles_keep_what_was_checked():
+    cache, batch = handles()
+    batch.lengths += 3
+    assert batch.lengths.tolist() == [3, 3]
+    batch.starts = torch.ones(3, dtype=torch.int32)
+    assert batch.starts.tolist() == [1, 1, 1]
+    for name, t in (("lengths", torch.zeros(3, dtype=torch.int32)), ("starts", torch.zeros(3)), ("table", torch.zeros(2, 4, dtype=torch.int32)),
+                    ("lengths", torch.zeros(4, dtype=torch.int32)[::2])):
+        with pytest.raises(ValueError):
+            setattr(batch, name, t)
+    with pytest.raises(AttributeError):
+        cache.k = cache.v
+
+
 def handles(dtype=torch.float32, D=64):
     cache = paged_kv.Cache(torch.zeros(4, 8, 2, D, dtype=dtype), torch.zeros(4, 8, 2, D, dtype=dtype))
     return cache, paged_kv.Batch(torch.zeros(2, 3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
@@ -111,8 +125,7 @@ def test_append_refusals():
             paged_kv.append(cache, batch, **bad)
     with pytest.raises(ValueError, match="current GPU"):
         paged_kv.append(cache, batch, k, k, q=q, q_out=o)
-    wide = paged_kv.Batch(torch.zeros(1, 1, dtype=torch.int32).expand(1, 1), torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
-    wide.table = types.SimpleNamespace(shape=(1, 2 ** 28), stride=lambda i: 2 ** 28)
+    wide = types.SimpleNamespace(sizes=((1, 2 ** 28), 2 ** 28))
     with pytest.raises(ValueError, match="at most 2147418112 tokens"):
         paged_kv.append(cache, wide, k, k)
 
