@@ -61,11 +61,11 @@ __device__ __forceinline__ int seq_rows(const PagedArgs& p, int b, int& first) {
     const int end = min(max(p.starts[b + 1], first), p.T);
     return (end - first) * (int)p.G.d;
 }
-// What a tile costs before its first key, in units (us, units 0 / 6 / 8 / 12 / 18: 24 heads x 4096 causal tokens 281 / 228 / 221 / 219 / 213, a
-// chunk of 1001 beside 30 single tokens 95 / 76 / 74 / 75 / 75, 20 ragged chunks over caches 187 / 143 / 140 / 143 / 148; with changed scores,
-// whose units take twice as long, 0 / 6 / 12: 2 x 4096 capped 308 / 310 / 326, 5 biased prompts 79 / 83 / 89. Of 16 rows, units 0 / 1 / 2: 61
-// single tokens 144.7 / 140.3 / 142.0, 32 sequences of 5 tokens 130 / 123 / 130).
-__host__ __device__ constexpr int ahead(int mt, bool mod) { return mt == 128 ? (mod ? 2 : 8) : 1; }
+// What a tile costs before its first key, in units: us at 0 / 6 / 8 / 12 units for 24 heads x 4096 causal tokens 281 / 228 / 208 / 200, for a
+// chunk of 1001 beside 30 single tokens 95 / 76 / 74 / 74, for 20 ragged chunks over caches 187 / 143 / 135 / 137 (at 10: 143); with changed
+// scores, whose units take longer, at 1 / 2 / 4 / 6: 2 x 4096 capped in a window 258 / 246 / 223 / 222, 5 biased prompts 71 / 71 / 71 / 74. Tiles of
+// 16 rows at 0 / 1 / 2: 61 single tokens of ragged lengths 144.7 / 140.3 / 142.0, 32 sequences of 5 tokens 130 / 123 / 130.
+__host__ __device__ constexpr int ahead(int mt, bool mod) { return mt == 128 ? (mod ? 4 : 8) : 1; }
 template <int MT, int UK, int AHEAD>
 __device__ __forceinline__ WorkTile make_tile(const PagedArgs& p, int b, int j) {
     WorkTile t;
@@ -1295,9 +1295,15 @@ struct Plan {
 static int make_plan(long T, long B, long H, long Hkv, long D, int type, Plan* plan) {
     if (T <= 0 || B <= 0 || B > MAX_SEQUENCES || Hkv <= 0 || H <= 0 || H % Hkv || (D != 64 && D != 128) || type < RDA_FP16 || type > RDA_FP32) return RDA_ERR_INVALID;
     if (T * (H / Hkv) >= 1L << 31) return RDA_ERR_INVALID;
-    // Rows of a sequence and KV head, on average.
+    // Tiles of 16, 32 or 128 rows by the rows of a sequence and KV head, on average (a lower or higher number in one of them costs time only),
+    // us 16 / 32 / 128: 32 sequences over 4096 keys, of 16 rows 113 / 121 / 142, 32 rows 130 / 125 / 144, 64 rows 249 / 140 / 157, 96 rows
+    // 368 / 324 / 172. Where all tiles of 128 rows together are few, each is cut into many parts, which cost more than the keys that
+    // tiles of 32 read again: over 8192 keys, 128-row tiles x KV heads 16 (24 tokens of one sequence) 34 / 68, 32 (128 tokens) 67.7 / 66.1, 48
+    // (192) 84 / 73; over 4096 keys, 32 (4 x 24 tokens) 43 / 63, 48 (2 x 96) 54 / 59, 64 (4 x 48) 70 / 61. fp32 keeps 16 rows, whose
+    // matrix products bound it (32 sequences of 16 rows 186, in tiles of 32 rows 242; 32 rows 238 / 247; 512 tokens over 512 105 / 110).
     const long rows = T * (H / Hkv) / B;
-    plan->mt = rows <= 16 ? 16 : rows <= 32 || type == RDA_FP32 ? 32 : 128;
+    plan->mt = rows <= 16 || type == RDA_FP32 ? 16 : rows <= 64 || B * ((rows + 127) / 128) * Hkv <= 40 ? 32 : 128;
+    // What the chip holds at a time: two or three workgroups on each of 256 CUs, by registers (three of the 64-dim and of the 128-row kernels).
     plan->grid = (D == 128 && plan->mt == 16) || plan->mt == 32 ? 512 : 768;
     if ((T * (H / Hkv) / plan->mt + 1) * B >= 1L << 31) return RDA_ERR_INVALID;
     plan->workspace = (size_t)plan->grid * sizeof(Cut) + (size_t)plan->grid * 2 * plan->mt * (D + 2) * 4;
@@ -1332,7 +1338,9 @@ template <class T, int D>
 static int launch_paged(const PagedArgs& a, const Plan& plan, void* stream) {
     if constexpr (sizeof(T) == 2)
         if (plan.mt == 128) return launch_tiles<T, D>(a, stream);
-    return plan.mt == 16 ? launch_rows<T, D, 1>(a, stream) : launch_rows<T, D, 2>(a, stream);
+    if constexpr (sizeof(T) == 2)
+        if (plan.mt == 32) return launch_rows<T, D, 2>(a, stream);
+    return launch_rows<T, D, 1>(a, stream);
 }
 
 static bool vector_rows(const void* p, const long* strides, int n, int type) {
