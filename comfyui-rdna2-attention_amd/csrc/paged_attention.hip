@@ -1040,14 +1040,19 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
             auto end_tile = [&](u32 st, u32 seen, bool masked) __attribute__((always_inline)) {
                 if (masked) {
                     // Values that are not finite, of keys that only some rows see: key by key.
-                    bool odd = false;
-                    constexpr u32 E = std::is_same<T, half_t>::value ? 0x7c00u : 0x7f80u;
+                    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+                    constexpr unsigned short E = std::is_same<T, half_t>::value ? 0x7c00 : 0x7f80;
+                    us2 most = {0, 0};
 #pragma unroll
                     for (int x = 0; x < L::TILE / 1024; x++) {
-                        const u4v v = lds_u4(smem_u + L::V + st + x * 1024 + lane_again() * 16);
+                        const u4v v = lds_u4(smem_u + L::V + st + x * 1024 + lane_again() * 16) & 0x7fff7fffu;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) odd |= (v[e] & E) == E || (v[e] >> 16 & E) == E;
+                        for (int e = 0; e < 4; e++) {
+                            const u32 word = v[e];
+                            most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, word));
+                        }
                     }
+                    const bool odd = most[0] >= E || most[1] >= E;
                     if (__builtin_expect(__any(odd), 0)) {
 #pragma unroll
                         for (int j = 0; j < 2; j++)
