@@ -23,6 +23,7 @@
 #include "paged.h"
 
 #define LOG2E 1.4426950408889634f
+#define LEAST -3.402823466e38f  // the lowest finite number
 #define MAX_SEQUENCES 8192
 #define MAX_KEYS ((1L << 31) - (1L << 16))  // of a sequence: a tile past its end keeps 32-bit key numbers
 
@@ -732,7 +733,7 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
 //   its base is then scalar, else each lane has its own. Table entries are fetched one step before the copies they are for, and have
 //   arrived by the barrier that ends it.
 // * Tiles at the ends of what the wave's rows see are masked, by a branch that the other tiles skip. Scores are replaced by -inf, and m
-//   starts at -1e30, so that a row without keys so far has P = 0.
+//   starts at the lowest finite number, so that a row without keys so far has P = 0.
 // * Keys past the sequence's end are copies of its last row, and those on pages that the cache does not have rows of page 0; masked
 //   tiles whose values are not all finite add them key by key to the rows that see them.
 template <int D>
@@ -870,7 +871,7 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
         f16v o[DT];
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d] = (f16v){};
-        float m = -1e30f, l = 0.f, l_old = 0.f;
+        float m = LEAST, l = 0.f, l_old = 0.f;
 
         if (!active) {  // no rows: the wave copies its part
             if (n > 0) {
@@ -1388,6 +1389,8 @@ int rda_paged_attn(const void* q, void* out, const void* k_pages, const void* v_
     a.kpp = (u32)dims[13]; a.kpr = (u32)dims[14]; a.kph = dims[15]; a.vpp = (u32)dims[16]; a.vpr = (u32)dims[17]; a.vph = dims[18];
     a.scale = softcap > 0.f ? scale / softcap * 2.f * LOG2E : scale * LOG2E;
     a.cap = softcap * LOG2E;
+    // Normal, positive and finite: masked scores are -inf before they meet the scale.
+    if (!(a.scale >= 1.2e-38f && a.scale <= 3e38f && a.cap <= 3e38f)) return RDA_ERR_INVALID;
     a.window = window;
     // No more workgroups than units there can be: a short table of few sequences needs none that finds no work.
     const long least = plan.mt == 128 ? 32 : type == RDA_FP32 ? 64 : 128, units = (T * (H / Hkv) / plan.mt + B) * ((N * S + least - 1) / least + ahead(plan.mt, false)) * Hkv;

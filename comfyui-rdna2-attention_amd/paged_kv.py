@@ -157,7 +157,7 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     """Attention of the batch's new tokens q (tokens, heads, D), the cache's type, D 64 or 128, over the cached keys of their sequences.
     A token at position n (its own key included) sees the keys j <= n; with window > 0 those with n - j < window; with prefix (int32,
     one per sequence) also those j < prefix[b], ahead of it or behind the window. Scores are scale q.k (scale None: D^-0.5); with
-    softcap > 0, softcap tanh(scale q.k / softcap); with slopes (fp32, one per head), less slopes[h] |n - j|. heads is a multiple of
+    softcap > 0, softcap tanh(scale q.k / softcap); with slopes (fp32, one per head, finite), less slopes[h] |n - j|. heads is a multiple of
     the cache's KV heads, which they share in order. A token that sees nothing gets 0. Returns out (q's shape, not overlapping q; rows of no
     sequence left as they were), or a new tensor, with those rows 0."""
     kc, vc = cache._k, cache._v
@@ -171,8 +171,10 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     dims = _attention_sizes.get(key)
     if dims is None:
         q, dims = _check_attention(cache, batch, q, out, slopes, prefix, key)
-    if not softcap >= 0.0 or not 0 <= window < 2 ** 31:
-        raise ValueError("attention takes softcap >= 0 and 0 <= window < 2^31 (0: none)")
+    if scale is None:
+        scale = cache._k.shape[3] ** -0.5
+    if not 0.0 <= softcap < 1e30 or not 1e-30 < (scale / softcap if softcap else scale) < 1e30 or not 0 <= window < 2 ** 31:
+        raise ValueError("attention takes a positive scale, softcap >= 0 (0: none), neither beyond 1e30, and 0 <= window < 2^31 (0: none)")
     same_device("attention", kc, batch._table, q, out, slopes, prefix)
     if q.numel() == 0:
         return out
@@ -191,7 +193,7 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
     _lib.check(k.paged_attn(q.data_ptr(), address, kc.data_ptr(), vc.data_ptr(), batch._table.data_ptr(), batch._starts.data_ptr(), batch._lengths.data_ptr(),
                             None if prefix is None else prefix.data_ptr(), None if slopes is None else slopes.data_ptr(), workspace.data_ptr(),
-                            D ** -0.5 if scale is None else scale, softcap, window, fill, type_, dims, _lib.raw_stream()))
+                            scale, softcap, window, fill, type_, dims, _lib.raw_stream()))
     return out
 
 
@@ -212,6 +214,8 @@ def _check_attention(cache, batch, q, out, slopes, prefix, key):
         raise ValueError(f"attention takes slopes as {H} contiguous fp32 values")
     if prefix is not None and (prefix.dtype != torch.int32 or prefix.numel() != B or not prefix.is_contiguous()):
         raise ValueError(f"attention takes prefix as {B} contiguous int32 values")
+    if max(*kc.stride()[:2], *vc.stride()[:2]) >= 2 ** 32:
+        raise ValueError("attention takes a cache whose pages and rows are less than 2^32 values apart")
     if T * (H // Hkv) >= 2 ** 31:
         raise ValueError("attention takes fewer than 2^31 rows of tokens and heads per KV head")
     ready = T == 0 or rows_ready(q)

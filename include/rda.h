@@ -219,7 +219,7 @@ int rda_paged_append(const void* q, const void* k, const void* v, void* q_out, v
 
 /* Attention of rows q (T, H, D) over a paged cache as appended to, D 64 or 128, all of one type: row t of sequence b, at position n as
  * above, sees keys j < min(lengths[b], N S) with j <= n (window > 0: and n - j < window), or j < prefix[b] (prefix NULL: none). Scores
- * are scale q.k; with softcap > 0, softcap tanh(scale q.k / softcap); with slopes [H] (or NULL), less slopes[h] |n - j|. Rows that see
+ * are scale q.k (scale positive); with softcap > 0, softcap tanh(scale q.k / softcap); with slopes [H] (or NULL), less slopes[h] |n - j|. Rows that see
  * nothing are 0; rows of no sequence are left as they were, or set to 0 with fill = 1. At most 8192 sequences. dims: T, H, Hkv, D, B,
  * N, the table's row pitch, P, S, strides (t, h) of q, of out, and (page, row, head) of k_pages, v_pages. workspace:
  * rda_paged_attn_workspace bytes of the same sizes, its contents of no account before and after; calls that overlap take one each.

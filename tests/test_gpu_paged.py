@@ -141,6 +141,45 @@ def test_values_that_are_not_finite(dev, type_, new, length):
     check(got[at:, :2][..., keep], ref[at:, :2][..., keep], off[at:, :2][..., keep], t)
 
 
+@pytest.mark.parametrize("new,length", [(1, 300), (40, 40), (100, 400)])
+@pytest.mark.parametrize("type_", ["bf16", "fp32"])
+def test_scores_far_from_zero(dev, type_, new, length):
+    """Scores near -10^35 and 10^35: the softmax is of their differences, wherever they lie. q sees keys as +-10^17 (1 + steps of 1/8): products
+    exact in both types, and one key's score above all others by more than 2^100."""
+    t = TYPES[type_]
+    g = gen(new)
+    table, starts, lengths, pages = batch_of([(new, length)], 16, g)
+    step = torch.randint(0, 4, (pages, 16, 1, 1), generator=g)
+    k = (2.0 ** 57 * (1 + step / 8)).expand(pages, 16, 1, 64).to(t).contiguous()
+    v = torch.randn(pages, 16, 1, 64, generator=g).to(t)
+    q = torch.full((new, 2, 64), 2.0 ** 57).to(t)
+    q[:, 1] = -q[:, 1]
+    got = paged_kv.attention(paged_kv.Cache(k.to(dev), v.to(dev)), paged_kv.Batch(table.to(dev), starts.to(dev), lengths.to(dev)), q.to(dev)).cpu()
+    ref, off, _ = attended(q, k, v, table, starts, lengths)
+    # Equal scores stay equal (the same operations on the same values) and all others' weights are 0: a mean of values, in 32 bits and P = 1.
+    bound = length * 2.0 ** -23 * v.double().abs().max() + rounding(ref, t)
+    assert ((got.double() - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("type_", ["bf16", "fp16"])
+def test_maximum_that_rises_slowly(dev, type_):
+    """Scores that grow with the key's position, by any amount a tile: rows whose maximum keeps moving, or stays just below what moves it."""
+    g = gen(77)
+    t = TYPES[type_]
+    for slope in (0.02, 0.05, 0.11, 0.3, 1.0):
+        table, starts, lengths, pages = batch_of([(140, 900)], 16, g)
+        k = torch.randn(pages, 16, 2, 64, generator=g) * 0.1
+        for n in range(900):
+            k[int(table[0, n // 16]), n % 16, :, 0] = slope * n
+        v = torch.randn(pages, 16, 2, 64, generator=g)
+        q = torch.randn(140, 8, 64, generator=g) * 0.1
+        q[..., 0] = 1.0
+        k, v, q = k.to(t), v.to(t), q.to(t)
+        got = paged_kv.attention(paged_kv.Cache(k.to(dev), v.to(dev)), paged_kv.Batch(table.to(dev), starts.to(dev), lengths.to(dev)), q.to(dev))
+        ref, off, _ = attended(q, k, v, table, starts, lengths)
+        check(got, ref, off, t)
+
+
 def test_many_sequences(dev):
     """More sequences than a workgroup has threads, most of them short, some empty."""
     g = gen(11)

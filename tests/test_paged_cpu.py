@@ -135,7 +135,8 @@ def test_attention_refusals():
     q = torch.zeros(3, 4, 64)
     f, i = torch.zeros(4), torch.zeros(2, dtype=torch.int32)
     for bad in (dict(q=q.half()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q[0]), dict(q=q[:, :0]), dict(q=q, out=q), dict(q=q, out=q[:2].clone()),
-                dict(q=q, out=q.half()), dict(q=q, out=torch.zeros(3, 4, 128)[..., ::2]), dict(q=q, softcap=-1.0), dict(q=q, softcap=float("nan")),
+                dict(q=q, out=q.half()), dict(q=q, out=torch.zeros(3, 4, 128)[..., ::2]), dict(q=q, softcap=-1.0), dict(q=q, softcap=float("nan")), dict(q=q, scale=0.0), dict(q=q, scale=-0.1), dict(q=q, scale=float("inf")), dict(q=q, scale=float("nan")),
+                dict(q=q, softcap=1e-35), dict(q=q, softcap=float("inf")),
                 dict(q=q, window=-1), dict(q=q, window=2 ** 31), dict(q=q, slopes=f[:3]), dict(q=q, slopes=f.half()), dict(q=q, slopes=torch.zeros(8)[::2]),
                 dict(q=q, prefix=i[:1]), dict(q=q, prefix=i.long()), dict(q=q, prefix=torch.zeros(4, dtype=torch.int32)[::2])):
         with pytest.raises(ValueError):
@@ -152,14 +153,15 @@ def test_entry_points_reject_before_any_launch():
     lib = _lib.declare(ctypes.CDLL(_lib.LIB_PATH))
     a = 1 << 20
 
-    def attn(type_=1, window=0, softcap=0.0, q=a, ws=a, **change):
+    def attn(type_=1, window=0, softcap=0.0, q=a, ws=a, scale=0.1, **change):
         d = dict(T=4, H=8, Hkv=2, D=128, B=2, N=4, pitch=4, P=9, S=16, sqt=1024, sqh=128, sot=1024, soh=128, kp=4096, kr=256, kh=128, vp=4096, vr=256, vh=128)
         d.update(change)
-        return lib.rda_paged_attn(q, a, a, a, a, a, a, None, None, ws, 0.1, softcap, window, 0, type_, _lib.long_array(list(d.values())), None)
+        return lib.rda_paged_attn(q, a, a, a, a, a, a, None, None, ws, scale, softcap, window, 0, type_, _lib.long_array(list(d.values())), None)
 
     for bad in (dict(T=0), dict(H=7), dict(H=0), dict(Hkv=0), dict(D=96), dict(B=0), dict(B=8193), dict(N=0), dict(P=0), dict(S=0), dict(N=1 << 27), dict(sqt=1028),
                 dict(soh=132), dict(kr=252), dict(vh=4), dict(q=a + 8), dict(ws=a + 8), dict(type_=3), dict(type_=-1), dict(window=-1), dict(softcap=-1.0),
-                dict(softcap=float("nan")), dict(T=1 << 30)):
+                dict(softcap=float("nan")), dict(T=1 << 30), dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=1e-39),
+                dict(kp=1 << 32), dict(vr=1 << 32)):
         assert attn(**bad) == 1, bad
     assert lib.rda_paged_attn_workspace(4, 2, 8, 2, 128, 1) > 0 and lib.rda_paged_attn_workspace(4, 2, 8, 3, 128, 1) == 0
 
