@@ -963,27 +963,27 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
             const float scale = MOD ? 1.f : p.scale;
             u4v pf[2];  // P of the two 16-key steps
             // Part k (of eight) of the P of scores x: registers 2 k, 2 k + 1.
-            auto exps_into = [&](const float (&x)[16], int k, u4v& d) __attribute__((always_inline)) {
-                const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * k], scale, -m)), b = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * k + 1], scale, -m));
+            auto exps_into = [&](const float (&x)[16], int k, u4v& d, float by) __attribute__((always_inline)) {
+                const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * k], by, -m)), b = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * k + 1], by, -m));
                 const u32 word = pair_of<T>(a, b);
                 l = add_pair<T>(word, l);
                 d[k & 3] = word;
             };
-            auto exps = [&](const float (&x)[16], int k) __attribute__((always_inline)) { exps_into(x, k, pf[k >> 2]); };
+            auto exps = [&](const float (&x)[16], int k, float by) __attribute__((always_inline)) { exps_into(x, k, pf[k >> 2], by); };
             auto exps_to = [&](const float (&x)[16], int k, u4v& d) __attribute__((always_inline)) {
-                exps_into(x, k, d);
+                exps_into(x, k, d, scale);
                 asm volatile("" : "+v"(d), "+v"(l));
             };
             auto no_hook = [](int) {};
             // m moves only where a row's maximum of a tile exceeds it by more than 2: a lane's 16 values of P then add up to at most 64, which full
             // steps (below) look for. (With more than 8, as in the rows kernel, rows whose first keys score low went on at 6 to 8 above m, and
             // took each tile twice: 2 x 4096 in a window of 2048, whose rows begin with few keys, ran half of its workgroups at half speed.)
-            auto move_max = [&](const float (&x)[16]) __attribute__((always_inline)) {
+            auto move_max = [&](const float (&x)[16], float by) __attribute__((always_inline)) {
                 float mx = x[0];
 #pragma unroll
                 for (int r = 1; r < 16; r++) mx = fmaxf(mx, x[r]);
                 const f2 h = both_halves(mx);
-                mx = fmaxf(h[0], h[1]) * scale;
+                mx = fmaxf(h[0], h[1]) * by;
                 if (__any(mx > m + 2.f)) {
                     const float mn = fmaxf(m, mx), a = __builtin_amdgcn_exp2f(m - mn);
                     m = mn;
@@ -1024,19 +1024,34 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
 
             // A tile's first part, wherever it lies: its scores, masked where not every row sees every key, the maximum, and the first half of P;
             // and its second, with one look at values that only some rows see.
-            float sa[16], sb[16];
+            // x scale - m in one rounding is off by half a step of x scale: nothing for scores of attention, but 2^(x scale - m) would leave fp32's range
+            // where scores pass 2^24. A wave that meets one of 4096 or more scales its scores first from then on, and takes no full steps.
+            float sa[16], sb[16], by = scale;
+            bool large = false;
             auto begin_tile = [&](int i, u32 st, u32 seen, bool masked) __attribute__((always_inline)) {
                 qk(st, sa, no_hook);
                 bias(sa, key_of(i));
+                if constexpr (!MOD) {
+                    if (!large) {
+                        float a = 0.f;
+#pragma unroll
+                        for (int r = 0; r < 16; r++) a = fmaxf(a, fabsf(sa[r]));
+                        large = __any(a * scale >= 4096.f);
+                        by = large ? 1.f : scale;
+                    }
+                    if (__builtin_expect(large, 0))
+#pragma unroll
+                        for (int r = 0; r < 16; r++) sa[r] *= scale;
+                }
                 if (masked) {
                     const u32 mine = seen >> (4 * (lane_again() >> 5));  // register r: key 8 (r / 4) + 4 g + r % 4
 #pragma unroll
                     for (int r = 0; r < 16; r++) sa[r] = mine >> (8 * (r >> 2) + (r & 3)) & 1 ? sa[r] : -__builtin_inff();
                 }
-                move_max(sa);
+                move_max(sa, by);
                 l_old = l;
 #pragma unroll
-                for (int k = 0; k < 4; k++) exps(sa, k);
+                for (int k = 0; k < 4; k++) exps(sa, k, by);
             };
             auto end_tile = [&](u32 st, u32 seen, bool masked) __attribute__((always_inline)) {
                 if (masked) {
@@ -1084,7 +1099,7 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
             auto full_step = [&](int i, u32 st, u32 st1, u32 st2, const float (&s)[16], float (&nxt)[16]) __attribute__((always_inline)) {
                 if (i + 2 < ends) issue_plain(i + 2, st2);
                 if (i + 3 < ends) fetch_plain(i + 3);
-                qk(st1, nxt, [&](int x) { if (beside(x)) exps(s, 4 + x / (KS / 4)); });
+                qk(st1, nxt, [&](int x) { if (beside(x)) exps(s, 4 + x / (KS / 4), scale); });
                 bias(nxt, key_of(i + 1));
                 if (__builtin_expect(__any(!(l <= l_old + 64.f)), 0)) return false;
                 l_old = l;
@@ -1128,6 +1143,7 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
                 if (__any(seen != 0)) {
                     while (true) {
                         begin_tile(i, st, seen, masked);
+                        full = full && !large;
                         bool done = true, taken = true;  // taken: the tile's maximum is
                         while (full) {
                             taken = false;
@@ -1148,7 +1164,7 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
                             }
                             copied = true;
 #pragma unroll
-                            for (int k = 4; k < 8; k++) exps(sa, k);
+                            for (int k = 4; k < 8; k++) exps(sa, k, by);
                             if (taken || !__any(!(l <= l_old + 64.f))) break;
                         }
                         // P above the maximum at hand (a full step's look, or the last tile's after full steps): the tile again, its copies made.

@@ -55,10 +55,10 @@ def appended(k, v, k_pages, v_pages, table, starts, lengths, rotary):
 
 def attended(q, k_pages, v_pages, table, starts, lengths, scale=None, softcap=0.0, window=0, slopes=None, prefix=None):
     """paged_kv.attention in 64 bits and the bound on what its arithmetic is off by before the last rounding, both (tokens, heads, D),
-    rows of no sequence 0; and which rows belong to a sequence."""
+    rows of no sequence 0; and which rows belong to a sequence. Tokens together where every value that any of them sees is finite, else one
+    by one, with only what that one sees."""
     T, H, D = q.shape
     P, S, Hkv, _ = k_pages.shape
-    u = 2.0 ** -24 if q.dtype == torch.float32 else torch.finfo(q.dtype).eps / 2
     scale = D ** -0.5 if scale is None else scale
     out, off = torch.zeros(T, H, D, dtype=torch.float64), torch.zeros(T, H, D, dtype=torch.float64)
     mine = torch.zeros(T, dtype=torch.bool)
@@ -70,33 +70,53 @@ def attended(q, k_pages, v_pages, table, starts, lengths, scale=None, softcap=0.
         there = (page >= 0) & (page < P)
         page = torch.where(there, page, 0)
         K, V = k_pages[page, j % S].double(), v_pages[page, j % S].double()  # (keys, Hkv, D)
-        for i in range(new):
-            n = p0 + i
-            see = j <= n
-            if window:
-                see &= n - j < window
-            if prefix is not None:
-                see |= j < int(prefix[b])
-            see &= there
-            if not see.any():
-                continue
-            Ks, Vs = K[see].repeat_interleave(H // Hkv, 1), V[see].repeat_interleave(H // Hkv, 1)  # (seen, H, D)
-            qi = q[first + i].double()
-            x = torch.einsum("hd,jhd->hj", qi, Ks) * scale
-            size = torch.einsum("hd,jhd->hj", qi.abs(), Ks.abs()) * abs(scale)
-            # Scores: D products and sums and the scale in 32 bits; tanh's and the bias's own roundings.
-            delta = (D + 4) * 2.0 ** -24 * size.amax(1, keepdim=True)
-            if softcap:
-                x = softcap * torch.tanh(x / softcap)
-                delta = delta + softcap * 4e-7 * (1 if q.dtype != torch.float32 else 0.5)
-            if slopes is not None:
-                gap = (n - j[see]).abs().double()
-                x = x - slopes.double()[:, None] * gap
-                delta = delta + 2.0 ** -23 * (slopes.double()[:, None] * gap).amax(1, keepdim=True)
-            delta = delta + 2.0 ** -23 * x.abs().amax(1, keepdim=True) + 2.0 ** -21  # to the log2 domain, less the maximum; 2^x
-            w = torch.softmax(x, 1)
-            out[first + i] = torch.einsum("hj,jhd->hd", w, Vs)
-            spread = torch.einsum("hj,jhd->hd", w, Vs.abs())
-            # Each weight is off by delta and its rounding, in the numerator and in the sum; sums of `seen` terms in 32 bits.
-            off[first + i] = spread * 2 * (delta + (u if q.dtype != torch.float32 else 0) + int(see.sum()) * 2.0 ** -24) * 1.01
+        n = torch.arange(p0, p0 + new)[:, None]
+        see = j <= n
+        if window:
+            see &= n - j < window
+        if prefix is not None:
+            see |= j < int(prefix[b])
+        see &= there
+        if not see.any():
+            continue
+        used = see.any(0)
+        K, V, see, j = K[used], V[used], see[:, used], j[used]
+        rows = slice(first, first + new)
+        if torch.isfinite(K).all() and torch.isfinite(V).all():
+            out[rows], off[rows] = _rows(q[rows], K, V, see, n, j, scale, softcap, slopes)
+        else:
+            for i in range(new):
+                one, s = slice(first + i, first + i + 1), see[i]
+                if s.any():
+                    out[one], off[one] = _rows(q[one], K[s], V[s], see[i:i + 1, s], n[i:i + 1], j[s], scale, softcap, slopes)
     return out, off, mine
+
+
+def _rows(q, K, V, see, n, j, scale, softcap, slopes):
+    """Attention of q (rows, heads, D) over K, V (keys, Hkv, D), row i over the keys of see[i], and its bound."""
+    R, H, D = q.shape
+    Hkv, keys = K.shape[1], K.shape[0]
+    low = q.dtype != torch.float32
+    u = torch.finfo(q.dtype).eps / 2 if low else 0.0
+    grouped = lambda t: t.view(R, Hkv, H // Hkv, -1).permute(1, 2, 0, 3).reshape(Hkv, -1, t.shape[-1])  # noqa: E731
+    back = lambda t: t.view(Hkv, H // Hkv, R, -1).permute(2, 0, 1, 3).reshape(R, H, -1)  # noqa: E731
+    Kt, Vt = K.permute(1, 2, 0).contiguous(), V.permute(1, 0, 2).contiguous()
+    qd = grouped(q.double())
+    x = back(torch.bmm(qd, Kt)) * scale  # (rows, heads, keys)
+    size = back(torch.bmm(qd.abs(), Kt.abs())) * scale
+    hidden = ~see[:, None]
+    # Scores: D products and sums and the scale in 32 bits; tanh's and the bias's own roundings.
+    delta = (D + 4) * 2.0 ** -24 * size.masked_fill(hidden, 0).amax(2, keepdim=True)
+    if softcap:
+        x = softcap * torch.tanh(x / softcap)
+        delta = delta + softcap * 4e-7 * (1 if low else 0.5)
+    if slopes is not None:
+        bias = slopes.double()[None, :, None] * (n - j).abs().double()[:, None]
+        x = x - bias
+        delta = delta + 2.0 ** -23 * bias.abs().masked_fill(hidden, 0).amax(2, keepdim=True)
+    delta = delta + 2.0 ** -23 * x.abs().masked_fill(hidden, 0).amax(2, keepdim=True) + 2.0 ** -21  # to the log2 domain, less the maximum; 2^x
+    some = see.any(1)[:, None, None]
+    w = torch.softmax(torch.where(some, x.masked_fill(hidden, -math.inf), 0.0), 2) * some
+    out, spread = back(torch.bmm(grouped(w), Vt)), back(torch.bmm(grouped(w), Vt.abs()))
+    # Each weight is off by delta and its rounding, in the numerator and in the sum; sums of the keys' terms in 32 bits.
+    return out, spread * 2 * (delta + u + keys * 2.0 ** -24) * 1.01

@@ -47,7 +47,13 @@ def check(got, ref, off, dtype, rows=None):
                            f"worst {float(((got - ref).abs() / bound)[bad].nan_to_num(9e9).max()):.2f} of the bound")
 
 
-def attend(dev, type_, D, heads, kv, page, seqs, seed, rows_behind=0, garbage=float("nan"), table_edit=None, view=None, **options):
+def tile_rows(T, B, heads, kv, D, type_):
+    """Rows of the tiles that a call's sizes choose, by the workspace they take: 16, 32 or 128."""
+    size = paged_kv.get_kernels().paged_attn_workspace(T, B, heads, kv, D, {"fp16": 0, "bf16": 1, "fp32": 2}[type_])
+    return {(grid * (32 + 2 * mt * (D + 2) * 4)): mt for mt in (16, 32, 128) for grid in (512, 768)}[size]
+
+
+def attend(dev, type_, D, heads, kv, page, seqs, seed, rows_behind=0, tiles=None, garbage=float("nan"), table_edit=None, view=None, **options):
     g = gen(seed)
     t = TYPES[type_]
     table, starts, lengths, pages = batch_of(seqs, page, g)
@@ -58,6 +64,7 @@ def attend(dev, type_, D, heads, kv, page, seqs, seed, rows_behind=0, garbage=fl
         table_edit(table)
     T = int(starts[-1]) + rows_behind
     q = torch.randn(T, heads, D, generator=g).to(t)
+    assert tiles is None or type_ == "fp32" or tile_rows(T, len(seqs), heads, kv, D, type_) == tiles
     print(f"attention {type_} D={D} heads={heads}/{kv} page={page} seqs={seqs[:6]}{'...' if len(seqs) > 6 else ''} {options}", flush=True)
     on = lambda x: x.to(dev) if isinstance(x, torch.Tensor) else x  # noqa: E731
     kd, vd = on(k), on(v)
@@ -90,6 +97,67 @@ def test_attention(dev, type_, heads, kv, D, page, name):
     attend(dev, type_, D, heads, kv, page, BATCHES[name], seed=len(name) + heads + page)
 
 
+# Enough KV heads for tiles of 128 rows: groups of 1, 2 and 5, pages that are and are not whole runs of 8 keys.
+WIDE = [(48, 24, 64, 16), (24, 24, 128, 24), (70, 14, 128, 8), (30, 30, 64, 7), (24, 24, 128, 13), (44, 22, 128, 64)]
+
+
+@pytest.mark.parametrize("seqs", [[(200, 200)], [(130, 1000)], [(1, 300), (260, 391), (0, 50), (1, 2), (0, 0), (297, 297)], [(150, 151), (129, 640)]])
+@pytest.mark.parametrize("heads,kv,D,page", WIDE)
+@pytest.mark.parametrize("type_", ["fp16", "bf16"])
+def test_wide_attention(dev, type_, heads, kv, D, page, seqs):
+    attend(dev, type_, D, heads, kv, page, seqs, seed=heads + page, tiles=128)
+
+
+@pytest.mark.parametrize("options", ["window1", "window7", "window100", "window150", "prefix", "prefix-window", "softcap", "slopes", "all", "scale"])
+@pytest.mark.parametrize("type_,heads,kv,D,page", [("bf16", 24, 24, 128, 16), ("fp16", 48, 24, 64, 20), ("fp16", 72, 24, 128, 8), ("bf16", 26, 26, 64, 32)])
+def test_wide_scores(dev, type_, heads, kv, D, page, options):
+    seqs = [(130, 390), (90, 90), (3, 200), (275, 333)]
+    slopes = torch.linspace(-0.01, 0.5, heads)
+    prefix = torch.tensor([0, 50, 210, 300], dtype=torch.int32)
+    o = {"window1": dict(window=1), "window7": dict(window=7), "window100": dict(window=100), "window150": dict(window=150), "prefix": dict(prefix=prefix),
+         "prefix-window": dict(prefix=prefix, window=20), "softcap": dict(softcap=2.0), "slopes": dict(slopes=slopes),
+         "all": dict(prefix=prefix, window=64, softcap=30.0, slopes=slopes), "scale": dict(scale=0.7)}[options]
+    attend(dev, type_, D, heads, kv, page, seqs, seed=3, tiles=128, **o)
+
+
+@pytest.mark.parametrize("page", [8, 20])
+@pytest.mark.parametrize("D", [64, 128])
+def test_wide_rows_that_see_nothing(dev, D, page):
+    """As below, in tiles of 128 rows: rows before the sequence's first position, and pages that the cache does not have, among whole ones."""
+    got = attend(dev, "bf16", D, 24, 24, page, [(200, 120), (90, 0), (100, 220)], seed=4, tiles=128)
+    assert not got[:80].any() and not got[200:290].any() and got[80:200].any(-1).all()
+
+    def edit(table):
+        table[0, :] = -1
+        table[1, 1] = 10 ** 9
+        table[2, 3:] = torch.where(torch.arange(table.shape[1] - 3) % 4 == 1, -5, table[2, 3:])
+    got = attend(dev, "fp16", D, 24, 24, page, [(100, 160), (133, 133), (140, 400), (1, 170)], seed=5, table_edit=edit, tiles=128)
+    assert not got[:100].any()
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_wide_random(dev, seed):
+    """Seeded random batches in tiles of 128 rows."""
+    g = gen(1900 + seed)
+    pick = lambda *a: a[int(torch.randint(0, len(a), (1,), generator=g))]  # noqa: E731
+    upto = lambda n: int(torch.randint(0, n + 1, (1,), generator=g))  # noqa: E731
+    kv = pick(21, 24, 42)
+    heads = kv * pick(1, 2, 3)
+    seqs = [(new, new + upto(pick(10, 200, 700))) for new in [130 + upto(200)] + [pick(1, 100 + upto(150), upto(90) + 60) for _ in range(1 + upto(2))]]
+    o = {}
+    if upto(2) == 0:
+        o["window"] = 1 + upto(250)
+    if upto(3) == 0:
+        o["softcap"] = 5.0
+    if upto(3) == 0:
+        o["slopes"] = torch.rand(heads, generator=g)
+    if upto(3) == 0:
+        o["prefix"] = torch.randint(0, 250, (len(seqs),), generator=g, dtype=torch.int32)
+    rows = sum(n for n, _ in seqs) * (heads // kv) // len(seqs)
+    D = pick(64, 128)
+    attend(dev, pick("fp16", "bf16"), D, heads, kv, pick(1, 7, 8, 12, 16, 48, 256), seqs, seed=seed, rows_behind=upto(2), tiles=128 if rows > 64 else None, **o)
+
+
 @pytest.mark.parametrize("options", ["window1", "window7", "window100", "prefix", "prefix-window", "softcap", "slopes", "all", "scale"])
 @pytest.mark.parametrize("type_,D,page", [("bf16", 128, 16), ("fp16", 64, 20), ("fp32", 128, 16), ("fp32", 64, 3)])
 def test_scores(dev, type_, D, page, options):
@@ -118,8 +186,8 @@ def test_rows_that_see_nothing(dev, type_):
 
 
 @pytest.mark.parametrize("type_", TYPES)
-@pytest.mark.parametrize("new,length", [(40, 40), (9, 300), (150, 150)])
-def test_values_that_are_not_finite(dev, type_, new, length):
+@pytest.mark.parametrize("new,length,copies", [(40, 40, 1), (9, 300, 1), (150, 150, 1), (150, 150, 12), (200, 330, 12)])
+def test_values_that_are_not_finite(dev, type_, new, length, copies):
     """inf and NaN in the keys and values of later tokens do not reach the rows that do not see them; rows that do see them get them."""
     g = gen(new)
     t = TYPES[type_]
@@ -130,30 +198,33 @@ def test_values_that_are_not_finite(dev, type_, new, length):
     v[int(table[0, bad // 16]), bad % 16, 0, 5] = float("nan")
     v[int(table[0, bad // 16]), bad % 16, 1, 70] = float("inf")
     k[int(table[0, (bad + 1) // 16]), (bad + 1) % 16, 1] = float("nan")
-    print(f"not finite {type_} {new} of {length}", flush=True)
+    k, v, q = k.repeat(1, 1, copies, 1), v.repeat(1, 1, copies, 1), q.repeat(1, copies, 1)  # 12: tiles of 128 rows
+    print(f"not finite {type_} {new} of {length} x {copies}", flush=True)
+    assert type_ == "fp32" or tile_rows(new, 1, 4 * copies, 2 * copies, 128, type_) == (128 if copies > 1 else 32)
     got = paged_kv.attention(paged_kv.Cache(k.to(dev), v.to(dev)), paged_kv.Batch(table.to(dev), starts.to(dev), lengths.to(dev)), q.to(dev)).cpu()
     ref, off, _ = attended(q, k, v, table, starts, lengths)
     at = bad - (length - new)
     check(got, ref, off, t, rows=slice(0, at))
     assert torch.isfinite(got[:at]).all()
-    assert got[at:, :2, 5].isnan().all() and (got[at, 2:, 70] == float("inf")).all() and got[at + 1:, 2:].isnan().all()
+    nan, inf = [h for h in range(4 * copies) if h % 4 < 2], [h for h in range(4 * copies) if h % 4 >= 2]
+    assert got[at:, nan, 5].isnan().all() and (got[at, inf, 70] == float("inf")).all() and got[at + 1:, inf].isnan().all()
     keep = [d for d in range(128) if d != 5]
-    check(got[at:, :2][..., keep], ref[at:, :2][..., keep], off[at:, :2][..., keep], t)
+    check(got[at:, nan][..., keep], ref[at:, nan][..., keep], off[at:, nan][..., keep], t)
 
 
-@pytest.mark.parametrize("new,length", [(1, 300), (40, 40), (100, 400)])
+@pytest.mark.parametrize("new,length,kv", [(1, 300, 1), (40, 40, 1), (100, 400, 1), (130, 400, 24)])
 @pytest.mark.parametrize("type_", ["bf16", "fp32"])
-def test_scores_far_from_zero(dev, type_, new, length):
+def test_scores_far_from_zero(dev, type_, new, length, kv):
     """Scores near -10^35 and 10^35: the softmax is of their differences, wherever they lie. q sees keys as +-10^17 (1 + steps of 1/8): products
     exact in both types, and one key's score above all others by more than 2^100."""
     t = TYPES[type_]
     g = gen(new)
     table, starts, lengths, pages = batch_of([(new, length)], 16, g)
-    step = torch.randint(0, 4, (pages, 16, 1, 1), generator=g)
-    k = (2.0 ** 57 * (1 + step / 8)).expand(pages, 16, 1, 64).to(t).contiguous()
-    v = torch.randn(pages, 16, 1, 64, generator=g).to(t)
-    q = torch.full((new, 2, 64), 2.0 ** 57).to(t)
-    q[:, 1] = -q[:, 1]
+    step = torch.randint(0, 4, (pages, 16, kv, 1), generator=g)
+    k = (2.0 ** 57 * (1 + step / 8)).expand(pages, 16, kv, 64).to(t).contiguous()
+    v = torch.randn(pages, 16, kv, 64, generator=g).to(t)
+    q = torch.full((new, 2 * kv, 64), 2.0 ** 57).to(t)
+    q[:, 1::2] = -q[:, 1::2]
     got = paged_kv.attention(paged_kv.Cache(k.to(dev), v.to(dev)), paged_kv.Batch(table.to(dev), starts.to(dev), lengths.to(dev)), q.to(dev)).cpu()
     ref, off, _ = attended(q, k, v, table, starts, lengths)
     # Equal scores stay equal (the same operations on the same values) and all others' weights are 0: a mean of values, in 32 bits and P = 1.
@@ -161,18 +232,19 @@ def test_scores_far_from_zero(dev, type_, new, length):
     assert ((got.double() - ref).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("kv", [2, 24])
 @pytest.mark.parametrize("type_", ["bf16", "fp16"])
-def test_maximum_that_rises_slowly(dev, type_):
+def test_maximum_that_rises_slowly(dev, type_, kv):
     """Scores that grow with the key's position, by any amount a tile: rows whose maximum keeps moving, or stays just below what moves it."""
     g = gen(77)
     t = TYPES[type_]
     for slope in (0.02, 0.05, 0.11, 0.3, 1.0):
         table, starts, lengths, pages = batch_of([(140, 900)], 16, g)
-        k = torch.randn(pages, 16, 2, 64, generator=g) * 0.1
+        k = torch.randn(pages, 16, kv, 64, generator=g) * 0.1
         for n in range(900):
             k[int(table[0, n // 16]), n % 16, :, 0] = slope * n
-        v = torch.randn(pages, 16, 2, 64, generator=g)
-        q = torch.randn(140, 8, 64, generator=g) * 0.1
+        v = torch.randn(pages, 16, kv, 64, generator=g)
+        q = torch.randn(140, 2 * kv, 64, generator=g) * 0.1
         q[..., 0] = 1.0
         k, v, q = k.to(t), v.to(t), q.to(t)
         got = paged_kv.attention(paged_kv.Cache(k.to(dev), v.to(dev)), paged_kv.Batch(table.to(dev), starts.to(dev), lengths.to(dev)), q.to(dev))
@@ -203,6 +275,7 @@ def test_rows_of_no_sequence(dev):
     ref, off, mine = attended(q, k, v, table, starts, lengths)
     assert mine.tolist() == [False] * 2 + [True] * 3 + [False] * 4
     check(got, ref, off, torch.float16, rows=mine)
+    assert paged_kv.attention(cache, batch, q.to(dev)[:0]).shape == (0, 4, 64)
     left = out.cpu()
     assert (left[~mine] == 7).all() and (left[:, 0] == 7).all() and (left[:, 5] == 7).all()
 
@@ -458,9 +531,10 @@ def test_calls_at_once(dev):
     jobs = []
     for s in range(4):
         g = gen(60 + s)
-        table, starts, lengths, pages = batch_of([(1, 900 + 100 * s), (60, 300), (1, 5)], 16, g)
-        cache = paged_kv.Cache(*(torch.randn(pages, 16, 2, 128, generator=g).half().to(dev) for _ in range(2)))
-        jobs.append((cache, paged_kv.Batch(table.to(dev), starts.to(dev), lengths.to(dev)), torch.randn(62, 8, 128, generator=g).half().to(dev)))
+        kv, seqs = (2, [(1, 900 + 100 * s), (60, 300), (1, 5)]) if s % 2 else (24, [(1, 900), (160, 300 + 50 * s), (140, 140)])
+        table, starts, lengths, pages = batch_of(seqs, 16, g)
+        cache = paged_kv.Cache(*(torch.randn(pages, 16, kv, 128, generator=g).half().to(dev) for _ in range(2)))
+        jobs.append((cache, paged_kv.Batch(table.to(dev), starts.to(dev), lengths.to(dev)), torch.randn(int(starts[-1]), 2 * kv, 128, generator=g).half().to(dev)))
     want = [paged_kv.attention(*j) for j in jobs]
     streams = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()

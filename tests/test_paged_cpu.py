@@ -185,6 +185,21 @@ def test_entry_points_reject_before_any_launch():
         assert append(**bad) == 1, bad
 
 
+def test_tile_rule():
+    """The tiles that sizes choose, by the workspace of their parts: 16 rows for single tokens and fp32, 32 for short chunks and where tiles of
+    128 would be few, else 128."""
+    lib = _lib.declare(ctypes.CDLL(_lib.LIB_PATH))
+
+    def rows(T, B, H, Hkv, D, type_):
+        size = lib.rda_paged_attn_workspace(T, B, H, Hkv, D, type_)
+        return {grid * (32 + 2 * mt * (D + 2) * 4): mt for mt in (16, 32, 128) for grid in (512, 768)}[size]
+
+    assert rows(64, 64, 32, 8, 128, 1) == 16 and rows(1, 1, 64, 4, 64, 0) == 16 and rows(2048, 1, 32, 8, 128, 2) == 16
+    assert rows(32 * 5, 32, 32, 8, 128, 1) == 32 and rows(32 * 16, 32, 32, 8, 64, 0) == 32 and rows(32 * 17, 32, 32, 8, 128, 1) == 128
+    assert rows(160, 1, 32, 8, 128, 1) == 32 and rows(161, 1, 32, 8, 128, 1) == 128  # 5 and 6 tiles x 8 KV heads
+    assert rows(2048, 1, 32, 8, 128, 1) == 128 and rows(1031, 31, 24, 8, 64, 0) == 128
+
+
 def test_reference_against_torch():
     """The 64-bit forms: causal attention of a chunk over cached keys equals torch's with the same mask, in any pages; a turn keeps lengths
     and depends on differences of positions only; appended pages hold the tokens in order."""
