@@ -4,8 +4,9 @@
 // Row n of a sequence (its position) with query head h sees keys j <= n (in a window, those with n - j < window; with a prefix, also
 // j < prefix). Its scores, in the log2 domain, are x = log2(e) (scale q.k), or log2(e) cap tanh(scale q.k / cap), less log2(e)
 // slope_h |n - j|; out = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m) in one pass over the keys, m the running maximum. m moves only when
-// a tile's maximum exceeds it by more than 8: the terms then stay below 2^8, far inside fp16's range, and O is seldom rescaled. A row
-// that sees nothing (or only scores of -inf) is 0.
+// a tile's maximum exceeds it by more than 8 (2 in tiles of 128 rows), so that O is seldom rescaled. For an fp16 cache m stands below the
+// maximum by lift() and the terms are that much larger, near the top of fp16's range: one of 2^-21 of the largest still has all of
+// fp16's bits, where many keys of little weight stand beside one of much. A row that sees nothing (or only scores of -inf) is 0.
 //
 // Work. The query heads of a KV head share its keys: the rows of (sequence, KV head) are its (token, head) pairs in token order, MT
 // to a tile, so that single tokens of a group of heads fill a tile with no key read twice. A tile walks the keys that any of its rows
@@ -279,6 +280,9 @@ template <int MT, int D>
 __device__ __forceinline__ float* partial(const PagedArgs& p, int block, int which) {
     return (float*)(p.ws + (size_t)p.grid * sizeof(Cut)) + ((size_t)block * 2 + which) * MT * (D + 2);
 }
+// How far below the maximum m stands (see the top): with what a tile's maximum may exceed it by, terms reach 2^15.
+template <class T>
+__host__ __device__ constexpr float lift(int mt) { return std::is_same<T, half_t>::value ? (mt == 128 ? 9.f : 7.f) : 0.f; }
 // The offset of a row of a page.
 __device__ __forceinline__ unsigned long long row_at(u32 page, u32 page_stride, u32 row, u32 row_stride) {
     return (unsigned long long)page * page_stride + (unsigned long long)row * row_stride;
@@ -351,6 +355,7 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
     using R = RowsTile<T>;
     constexpr bool FP32 = R::FP32;
     constexpr int KT = R::KT, KG = R::KG, UK = R::UK, MT = 16 * MB, AHEAD = ahead(MT, MOD);
+    constexpr float LIFT = lift<T>(MT);
     constexpr int NB = KG / 4;              // score blocks of 16 keys
     constexpr int EV = 16 / sizeof(T);      // values of a 16-byte vector
     constexpr int KC = D / (4 * EV);        // 16-byte vectors of a lane's part of a K row
@@ -559,7 +564,8 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
 #pragma unroll
                     for (int e = 1; e < KG; e++) mx = fmaxf(mx, s[m][e]);
                     mx = rows_max(mx);
-                    const bool move = mx > m_[m] + 8.f || (m_[m] == -__builtin_inff() && mx > m_[m]);
+                    const bool move = mx > m_[m] + (8.f + LIFT) || (m_[m] == -__builtin_inff() && mx > m_[m]);
+                    mx -= LIFT;
                     if (__any(move)) {
                         const float a = move ? __builtin_amdgcn_exp2f(m_[m] - mx) : 1.f;
                         m_[m] = move ? mx : m_[m];
@@ -781,6 +787,7 @@ template <class T, int D, bool MOD, bool RUNS>
 __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(PagedArgs p) {
     constexpr int MT = 128, UK = 32, AHEAD = ahead(MT, MOD), ROW = 2 * D, KS = D / 16, DT = D / 32;  // KS: products of a score block; DT: of a 16-key step with V
     constexpr int CP = D / 64, CR = 1024 / ROW;  // a wave's copies of K per tile; rows of a copy
+    constexpr float LIFT = lift<T>(MT), MOST = 64.f * (std::is_same<T, half_t>::value ? 512.f : 1.f);  // of a full step's sum of P in a lane: 64 2^LIFT
     using L = TilesLds<D>;
     extern __shared__ __attribute__((aligned(256))) char smem[];
     const int lane = threadIdx.x & 63, g = lane >> 5, lq = lane & 31;
@@ -975,8 +982,8 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
                 asm volatile("" : "+v"(d), "+v"(l));
             };
             auto no_hook = [](int) {};
-            // m moves only where a row's maximum of a tile exceeds it by more than 2: a lane's 16 values of P then add up to at most 64, which full
-            // steps (below) look for. (With more than 8, as in the rows kernel, rows whose first keys score low went on at 6 to 8 above m, and
+            // m moves only where a row's maximum of a tile exceeds it by more than 2: a lane's 16 values of P then add up to at most 64 (2^LIFT), which
+            // full steps (below) look for. (With more than 8, as in the rows kernel, rows whose first keys score low went on at 6 to 8 above m, and
             // took each tile twice: 2 x 4096 in a window of 2048, whose rows begin with few keys, ran half of its workgroups at half speed.)
             auto move_max = [&](const float (&x)[16], float by) __attribute__((always_inline)) {
                 float mx = x[0];
@@ -984,8 +991,8 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
                 for (int r = 1; r < 16; r++) mx = fmaxf(mx, x[r]);
                 const f2 h = both_halves(mx);
                 mx = fmaxf(h[0], h[1]) * by;
-                if (__any(mx > m + 2.f)) {
-                    const float mn = fmaxf(m, mx), a = __builtin_amdgcn_exp2f(m - mn);
+                if (__any(mx > m + (2.f + LIFT))) {
+                    const float mn = fmaxf(m, mx - LIFT), a = __builtin_amdgcn_exp2f(m - mn);
                     m = mn;
                     l *= a;
 #pragma unroll
@@ -1092,7 +1099,7 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
             };
             // A step of the full tiles: tile i's scores are in s, its P's first half in pf[0] and l (before which l was l_old); tile i + 1 is full
             // too, and its scores go to nxt. Steps of KS (or 2 DT = KS) products: the four parts of half a tile's exponentials beside every
-            // (KS / 4)-th. P is made with the m at hand: a lane's sum that grew by no more than 64 proves that no P was above it; else
+            // (KS / 4)-th. P is made with the m at hand: a lane's sum that grew by no more than MOST proves that no P was above it; else
             // the step ends before the product (false), and the tile is taken again by a plain step. (With the maximum moved here, O was
             // copied between registers in every step: 64 of ~300 instructions.)
             auto beside = [](int x) __attribute__((always_inline)) { return x % (KS / 4) == KS / 4 - 1; };
@@ -1101,7 +1108,7 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
                 if (i + 3 < ends) fetch_plain(i + 3);
                 qk(st1, nxt, [&](int x) { if (beside(x)) exps(s, 4 + x / (KS / 4), scale); });
                 bias(nxt, key_of(i + 1));
-                if (__builtin_expect(__any(!(l <= l_old + 64.f)), 0)) return false;
+                if (__builtin_expect(__any(!(l <= l_old + MOST)), 0)) return false;
                 l_old = l;
                 u4v pn;
                 pv(st, [&](int x) { if (beside(x)) exps_to(nxt, x / (KS / 4), pn); });
@@ -1165,7 +1172,7 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
                             copied = true;
 #pragma unroll
                             for (int k = 4; k < 8; k++) exps(sa, k, by);
-                            if (taken || !__any(!(l <= l_old + 64.f))) break;
+                            if (taken || !__any(!(l <= l_old + MOST))) break;
                         }
                         // P above the maximum at hand (a full step's look, or the last tile's after full steps): the tile again, its copies made.
                         l = l_old;

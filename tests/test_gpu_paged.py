@@ -1,5 +1,7 @@
 """paged_kv.append and paged_kv.attention on the GPU against plain 64-bit forms: every type, head layouts, page sizes that end inside
 a tile, sequences from nothing to thousands of keys, masks that leave rows empty, pages that hold NaN where no row may look."""
+import math
+
 import pytest
 import torch
 
@@ -250,6 +252,34 @@ def test_maximum_that_rises_slowly(dev, type_, kv):
         got = paged_kv.attention(paged_kv.Cache(k.to(dev), v.to(dev)), paged_kv.Batch(table.to(dev), starts.to(dev), lengths.to(dev)), q.to(dev))
         ref, off, _ = attended(q, k, v, table, starts, lengths)
         check(got, ref, off, t)
+
+
+@pytest.mark.parametrize("gap", [6.3, 13.7, 18.3, 25.1])
+@pytest.mark.parametrize("type_,new,kv,tiles", [("fp16", 1, 2, 16), ("fp16", 40, 1, 32), ("fp16", 140, 24, 128), ("bf16", 140, 24, 128), ("bf16", 1, 2, 16), ("fp32", 1, 2, 16)])
+def test_light_keys_beside_heavy_ones(dev, type_, new, kv, tiles, gap):
+    """Every 32nd key weighs 2^gap times the others and has value 0, the others 1: a row that sees a heavy and b light keys gives
+    b 2^-gap / (a + b 2^-gap), nothing but the light keys' weights. Each of those is rounded to the type, as is the heavy ones' (2 u), its
+    score has an error of 2^-23 of gap in the log2 domain and 2^x one of 2^-22, sums of n keys n 2^-23; in fp16 a weight that falls below
+    the normal range is off by half of 2^-24, with m lifted 2^7 (2^9) below the maximum at least."""
+    length, t = 2000, TYPES[type_]
+    assert tile_rows(new, 1, kv, kv, 64, type_) == tiles
+    pages = torch.zeros(125, 16, kv, 64)
+    k, v, q = pages.clone(), pages.clone() + 1.0, torch.zeros(new, kv, 64)
+    k[..., 0] = -1.0
+    k[::2, 0] = 0.0
+    v[::2, 0] = 0.0
+    q[..., 0] = 1.0
+    cache = paged_kv.Cache(k.to(t).to(dev), v.to(t).to(dev))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    batch = paged_kv.Batch(torch.arange(125, dtype=torch.int32, device=dev)[None], i32([0, new]), i32([length]))
+    got = paged_kv.attention(cache, batch, q.to(t).to(dev), scale=gap * math.log(2.0)).cpu().double()
+    n = torch.arange(length - new + 1, length + 1, dtype=torch.float64)
+    heavy = (n / 32).ceil()
+    light = (n - heavy) * 2.0 ** -gap
+    ref = (light / (heavy + light))[:, None, None].expand_as(got)
+    u = 0.0 if type_ == "fp32" else torch.finfo(t).eps / 2
+    off = ref * (2 * u + (gap * 2 ** -23 + 2.0 ** -22) * 1.4 + length * 2.0 ** -23) + (31 * 2.0 ** -32 if type_ == "fp16" else 0.0)
+    check(got, ref, off, t)
 
 
 def test_many_sequences(dev):
