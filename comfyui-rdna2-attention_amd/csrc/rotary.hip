@@ -16,6 +16,7 @@
 #define ROW_WAVES 4  // waves, each of a token and a slice of heads, per workgroup
 #define PASSES 4     // heads per lane
 #define MAX_PAIRS 128
+#define MAX_ROWS ((1L << 26) - 64)  // tokens of a call: a grid has fewer than 2^32 threads
 
 // Cosine and sine of a turn's fraction: n f - rint(4 n f) / 4 = y / 4, |y| <= 1/2, then the series at y pi / 2 (at most pi / 4:
 // the first terms left out are below 2e-9 and 1e-10).
@@ -244,9 +245,9 @@ extern "C" {
 int rda_rotate_positions(const void* x, void* y, const void* positions, int wide, const double* turns, float factor, int flags, int type, const long* dims,
                          void* stream) {
     const long B = dims[0], L = dims[1], H = dims[2], D = dims[3], R = dims[4];
-    if (B <= 0 || L <= 0 || H <= 0 || H > 65535 || L >= 1L << 31 || !rotary_ok(turns, D, R) || R == 0) return RDA_ERR_INVALID;
+    if (B <= 0 || L <= 0 || H <= 0 || H > 65535 || !rotary_ok(turns, D, R) || R == 0) return RDA_ERR_INVALID;
     const long groups = (B * L + ROW_WAVES - 1) / ROW_WAVES, slice = 64 / (D / 16) * PASSES;
-    if (B >= 1L << 31 || groups >= 1L << 31 || type < RDA_FP16 || type > RDA_FP32 || !vector_rows(x, dims + 5, 3, type) || !vector_rows(y, dims + 8, 3, type))
+    if (B > MAX_ROWS || L > MAX_ROWS || B * L > MAX_ROWS || type < RDA_FP16 || type > RDA_FP32 || !vector_rows(x, dims + 5, 3, type) || !vector_rows(y, dims + 8, 3, type))
         return RDA_ERR_INVALID;
     const RotateArgs a = {{turns, (int)D, (int)R, flags & 1, factor, flags & 2 ? -1.f : 1.f}, x, y, positions, wide, (int)L, (int)H, B * L,
                           dims[5], dims[6], dims[7], dims[8], dims[9], dims[10]};
@@ -260,7 +261,7 @@ int rda_rotate_positions(const void* x, void* y, const void* positions, int wide
 int rda_paged_append(const void* q, const void* k, const void* v, void* q_out, void* k_pages, void* v_pages, const int* table, const int* starts,
                      const int* lengths, const double* turns, float factor, int interleaved, int type, int cache_type, const long* dims, void* stream) {
     const long T = dims[0], H = dims[1], Hkv = dims[2], D = dims[3], R = dims[4], B = dims[5], N = dims[6], P = dims[8], S = dims[9];
-    if (T <= 0 || T >= 1L << 31 || H < 0 || Hkv <= 0 || H + 2 * Hkv > 65535 || !rotary_ok(turns, D, R) || B <= 0 || B >= 1L << 30 || N <= 0 || P <= 0 || P >= 1L << 31 ||
+    if (T <= 0 || T > MAX_ROWS || H < 0 || Hkv <= 0 || H + 2 * Hkv > 65535 || !rotary_ok(turns, D, R) || B <= 0 || B >= 1L << 30 || N <= 0 || P <= 0 || P >= 1L << 31 ||
         S <= 0 || N > ((1L << 31) - (1L << 16)) / S)
         return RDA_ERR_INVALID;
     if (type < RDA_FP16 || type > RDA_FP32 || cache_type < RDA_FP16 || cache_type > RDA_FP32) return RDA_ERR_INVALID;

@@ -9,7 +9,7 @@ import torch
 
 from . import _lib
 from .hip_attention import Kernels
-from .rotary import TYPES, Sizes, rows_ready, same_device, vector_rows
+from .rotary import MAX_TOKENS, TYPES, Sizes, distinct, rows_ready, same_device, vector_rows
 
 HEADS = (64, 128)  # head dims of `attention`
 MAX_SEQUENCES = 8192
@@ -95,7 +95,8 @@ def append(cache, batch, k, v, rotary=None, q=None, q_out=None):
     and v are fp16, bf16 or fp32, of the cache's type or another: rounded to it once, after the turn. q (tokens, heads, D), if
     given, is turned in the same launch into q_out (the cache's type; None: in place) -- what attention takes. Rows of no
     sequence are left as they were in q_out, as is the cache where a position is negative, past the table or on a page that it does not
-    have. Two tokens on one row of one page: either may remain. q_out is q itself or does not overlap q, k and v. Returns q_out."""
+    have. Two tokens on one row of one page: either may remain. q_out is q itself or does not overlap q, k and v, and
+    none of them overlaps the pages. Returns q_out."""
     kc, vc = cache._k, cache._v
     if q is not None:
         if q_out is None:
@@ -121,7 +122,7 @@ def append(cache, batch, k, v, rotary=None, q=None, q_out=None):
     return q_out
 
 
-Q_OUT_ERROR = "append's q_out has q's shape and the cache's type, a contiguous last dimension and rows on 16-byte boundaries"
+Q_OUT_ERROR = "append's q_out has q's shape and the cache's type, a contiguous last dimension and rows on 16-byte boundaries, each its own"
 
 
 def _check_append(cache, batch, k, v, rotary, q, q_out, key):
@@ -137,11 +138,15 @@ def _check_append(cache, batch, k, v, rotary, q, q_out, key):
         H = q.shape[1] if q.dim() == 3 else 0
         if q.dim() != 3 or q.dtype != k.dtype or q.shape[0] != T or q.shape[2] != D or H == 0:
             raise ValueError(f"append takes q as ({T}, heads, {D}) of k's type")
-        if q_out.shape != q.shape or q_out.dtype != kc.dtype or not (T == 0 or rows_ready(q_out)):
+        if q_out.shape != q.shape or q_out.dtype != kc.dtype or not (T == 0 or (rows_ready(q_out) and distinct(q_out))):
             raise ValueError(Q_OUT_ERROR)
     elif q_out is not None:
         raise ValueError("append takes q_out with q only")
     B, N, pitch, P, S = _sizes("append", cache, batch)
+    if not (distinct(kc) and distinct(vc)):
+        raise ValueError("append takes a cache whose pages, rows and heads are not one memory (an expanded view)")
+    if T > MAX_TOKENS:
+        raise ValueError(f"append takes at most {MAX_TOKENS} tokens")
     if H + 2 * Hkv > 65535:
         raise ValueError("append takes at most 65535 heads")
     ready = T == 0 or all(rows_ready(t) for t in (k, v) + (() if q is None else (q,)))
@@ -189,6 +194,8 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     sizes = (T, B, H, Hkv, D, type_)
     size = _workspaces.get(sizes)
     if size is None:
+        if len(_workspaces) >= 4096:
+            _workspaces.clear()
         size = _workspaces[sizes] = k.paged_attn_workspace(*sizes)
     workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
     _lib.check(k.paged_attn(q.data_ptr(), address, kc.data_ptr(), vc.data_ptr(), batch._table.data_ptr(), batch._starts.data_ptr(), batch._lengths.data_ptr(),
@@ -197,7 +204,7 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     return out
 
 
-OUT_ERROR = "attention's out has q's shape and type, a contiguous last dimension and rows on 16-byte boundaries"
+OUT_ERROR = "attention's out has q's shape and type, a contiguous last dimension and rows on 16-byte boundaries, each its own"
 
 
 def _check_attention(cache, batch, q, out, slopes, prefix, key):
@@ -208,7 +215,7 @@ def _check_attention(cache, batch, q, out, slopes, prefix, key):
         raise ValueError(f"attention takes q as (tokens, a multiple of {Hkv} heads, {D}) of the cache's type {kc.dtype}, head dim 64 or 128")
     T, H = q.shape[:2]
     B, N, pitch, P, S = _sizes("attention", cache, batch)
-    if out.shape != q.shape or out.dtype != q.dtype or not (T == 0 or rows_ready(out)):
+    if out.shape != q.shape or out.dtype != q.dtype or not (T == 0 or (rows_ready(out) and distinct(out))):
         raise ValueError(OUT_ERROR)
     if slopes is not None and (slopes.dtype != torch.float32 or slopes.numel() != H or not slopes.is_contiguous()):
         raise ValueError(f"attention takes slopes as {H} contiguous fp32 values")

@@ -11,6 +11,7 @@ from . import _lib
 from .hip_attention import Kernels
 
 MAX_HEAD = 256
+MAX_TOKENS = 2 ** 26 - 64  # of a call
 LAYOUTS = ("half", "interleaved")
 TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # the library's type codes
 
@@ -104,6 +105,11 @@ def rows_ready(t):
     return True
 
 
+def distinct(t):
+    """Whether no dimension of t repeats one address (expanded views): what a kernel writes has to."""
+    return all(s != 0 or n == 1 for s, n in zip(t.stride(), t.shape))
+
+
 def same_device(what, *tensors):
     """Raises ValueError unless every tensor (None: none) is on the current GPU: the kernels run on its current stream."""
     device = -1
@@ -154,7 +160,7 @@ def rotate(x, positions, rotary, out=None, inverse=False):
     return out
 
 
-OUT_ERROR = "rotate's out has x's shape and type, a contiguous last dimension and rows on 16-byte boundaries"
+OUT_ERROR = "rotate's out has x's shape and type, a contiguous last dimension and rows on 16-byte boundaries, each its own"
 
 
 def _check_rotate(x, positions, rotary, out, key):
@@ -164,7 +170,9 @@ def _check_rotate(x, positions, rotary, out, key):
                          f"to {MAX_HEAD}, at most 65535 heads, not {tuple(x.shape)} {x.dtype}")
     if positions.dtype not in (torch.int32, torch.int64) or positions.shape != x.shape[:-2]:
         raise ValueError(f"rotate takes int32 or int64 positions of shape {tuple(x.shape[:-2])}, not {tuple(positions.shape)} {positions.dtype}")
-    if out.shape != x.shape or out.dtype != x.dtype or not (out.numel() == 0 or rows_ready(out)):
+    if positions.numel() > MAX_TOKENS:
+        raise ValueError(f"rotate takes at most {MAX_TOKENS} tokens")
+    if out.shape != x.shape or out.dtype != x.dtype or not (out.numel() == 0 or (rows_ready(out) and distinct(out))):
         raise ValueError(OUT_ERROR)
     ready = x.numel() == 0 or rows_ready(x)
     if not ready:

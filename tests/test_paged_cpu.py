@@ -94,6 +94,43 @@ def test_cache_and_batch_refusals():
             paged_kv.Batch(*bad)
 
 
+def test_outputs_of_one_memory_are_refused():
+    """Expanded views as outputs: two rows would be written to one place."""
+    rot, pos = rotary.Rotary(64, device="cpu"), torch.zeros(4, dtype=torch.int32)
+    x = torch.zeros(4, 2, 64, dtype=torch.float16)
+    for out in (x[:1].expand(4, 2, 64), x[:, :1].expand(4, 2, 64)):
+        with pytest.raises(ValueError, match="each its own"):
+            rotary.rotate(x, pos, rot, out=out)
+        pages = torch.zeros(3, 8, 2, 64, dtype=torch.float16)
+        cache = paged_kv.Cache(pages, pages.clone())
+        batch = paged_kv.Batch(torch.zeros(1, 3, dtype=torch.int32), torch.tensor([0, 4], dtype=torch.int32), torch.tensor([4], dtype=torch.int32))
+        with pytest.raises(ValueError, match="each its own"):
+            paged_kv.attention(cache, batch, x, out=out)
+        with pytest.raises(ValueError, match="each its own"):
+            paged_kv.append(cache, batch, x, x, q=x, q_out=out)
+    one = paged_kv.Cache(pages[:, :, :1].expand(3, 8, 2, 64), pages)
+    with pytest.raises(ValueError, match="one memory"):
+        paged_kv.append(one, batch, x, x)
+
+
+def test_calls_of_too_many_tokens_are_refused():
+    """A grid has fewer than 2^32 threads; the sizes alone are looked at."""
+    rot, n = rotary.Rotary(16, device="cpu"), rotary.MAX_TOKENS + 1
+    x = torch.zeros(1, 1, 16, dtype=torch.float16).expand(n, 1, 16)
+    with pytest.raises(ValueError, match="at most"):
+        rotary.rotate(x, torch.zeros(1, dtype=torch.int32).expand(n), rot, out=x)
+    pages = torch.zeros(3, 8, 1, 16, dtype=torch.float16)
+    batch = paged_kv.Batch(torch.zeros(1, 3, dtype=torch.int32), torch.tensor([0, 4], dtype=torch.int32), torch.tensor([4], dtype=torch.int32))
+    with pytest.raises(ValueError, match="at most"):
+        paged_kv.append(paged_kv.Cache(pages, pages.clone()), batch, x, x)
+    lib = _lib.declare(ctypes.CDLL(_lib.LIB_PATH))
+    a = 1 << 20
+    for B, L in ((1, n), (n, 1), (1 << 14, 1 << 13), (1 << 40, 1 << 40)):
+        assert lib.rda_rotate_positions(a, a, a, 0, a, 1.0, 0, 0, _lib.long_array([B, L, 1, 16, 16, 16, 16, 16, 16, 16, 16]), None) == 1
+    dims = dict(T=n, H=0, Hkv=1, D=16, R=0, B=1, N=3, pitch=3, P=3, S=8, qt=0, qh=0, kt=16, kh=16, vt=16, vh=16, ot=0, oh=0, kp=128, kr=16, ch=16, vp=128, vr=16, wh=16)
+    assert lib.rda_paged_append(None, a, a, None, a, a, a, a, a, None, 1.0, 0, 0, 0, _lib.long_array(list(dims.values())), None) == 1
+
+
 def test_handles_keep_what_was_checked():
     cache, batch = handles()
     batch.lengths += 3
