@@ -65,7 +65,7 @@ __device__ __forceinline__ int seq_rows(const PagedArgs& p, int b, int& first) {
 }
 // What a tile costs before its first key, in units: us at 0 / 6 / 8 / 12 units for 24 heads x 4096 causal tokens 281 / 228 / 208 / 200, for a
 // chunk of 1001 beside 30 single tokens 95 / 76 / 74 / 74, for 20 ragged chunks over caches 187 / 143 / 135 / 137 (at 10: 143); with changed
-// scores, whose units take longer, at 1 / 2 / 4 / 6: 2 x 4096 capped in a window 258 / 246 / 223 / 222, 5 biased prompts 71 / 71 / 71 / 74. Tiles of
+// scores, whose units take longer, at 3 / 4 / 6: 2 x 4096 capped in a window 225 / 214 / 213, 5 biased prompts 62 / 62 / 63. Tiles of
 // 16 rows at 0 / 1 / 2: 61 single tokens of ragged lengths 144.7 / 140.3 / 142.0, 32 sequences of 5 tokens 130 / 123 / 130.
 __host__ __device__ constexpr int ahead(int mt, bool mod) { return mt == 128 ? (mod ? 4 : 8) : 1; }
 template <int MT, int UK, int AHEAD>
@@ -748,7 +748,8 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
 // A chunk of 2048 tokens, 32 heads over 8 KV heads of 128 bf16, over 14336 cached keys: 546 to 554 us for 515 GFLOP, 0.94 PFLOP/s, 78% of what a library
 // product of 8192^3 reaches. The matrix instructions run in 47% of the cycles (at 1.6 to 1.9 GHz, the chip's power limit) and five other vector
 // instructions stand beside each; the two do not overlap within a wave's SIMD, and add up to nearly all of them. LDS reads meet no bank conflict.
-// Capped scores take three transcendentals each where plain ones take one: 2 x 4096 tokens of 16 heads of 128 in a window of 2048, 103 GFLOP, 215 us.
+// Capped scores take three transcendentals each where plain ones take one: 2 x 4096 tokens of 16 heads of 128 in a window of 2048, 103 GFLOP, 198 us:
+// at two workgroups a CU vector work and products fill ~80% of the cycles (217 us with the whole capped score made before the softmax's product).
 // With D = 64 a score's exponential stands beside half the products. Tiles that are masked cost ~2.4 full ones, a tile's start ~7 us of latency.
 template <int D>
 struct TilesLds {
@@ -964,18 +965,28 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
                 }
                 return seen;
             };
+            // What x is times in the softmax's exponent. Capped scores without a bias stay the -1 / (1 + 2^e) of their tanh (see capped), times 2 cap: that
+            // a row's scores are all cap too low changes nothing. (Where 2 cap passes 4096 they are made whole first, as large scores are, below.)
+            const float scale = !MOD ? p.scale : p.cap > 0.f && !p.slopes && p.cap < 2048.f ? 2.f * p.cap : 1.f;
             auto bias = [&](float (&x)[16], int key0) __attribute__((always_inline)) {
                 if constexpr (MOD) {
-                    const float d0 = (float)(pos - key0 - 4 * g);
+                    if (p.cap > 0.f) {
 #pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        float y = x[r] * p.scale;
-                        if (p.cap > 0.f) y = capped<false>(y, p.cap);
-                        x[r] = __builtin_fmaf(-slope, fabsf(d0 - (float)(8 * (r >> 2) + (r & 3))), y);
+                        for (int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x[r] * p.scale));
+                        if (scale != 1.f) return;
+#pragma unroll
+                        for (int r = 0; r < 16; r++) x[r] = __builtin_fmaf(2.f * p.cap, x[r], p.cap);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; r++) x[r] *= p.scale;
+                    }
+                    if (p.slopes) {
+                        const float d0 = (float)(pos - key0 - 4 * g);
+#pragma unroll
+                        for (int r = 0; r < 16; r++) x[r] = __builtin_fmaf(-slope, fabsf(d0 - (float)(8 * (r >> 2) + (r & 3))), x[r]);
                     }
                 }
             };
-            const float scale = MOD ? 1.f : p.scale;
             u4v pf[2];  // P of the two 16-key steps
             // Part k (of eight) of the P of scores x: registers 2 k, 2 k + 1.
             auto exps_into = [&](const float (&x)[16], int k, u4v& d, float by) __attribute__((always_inline)) {

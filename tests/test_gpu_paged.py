@@ -122,6 +122,16 @@ def test_wide_scores(dev, type_, heads, kv, D, page, options):
     attend(dev, type_, D, heads, kv, page, seqs, seed=3, tiles=128, **o)
 
 
+@pytest.mark.parametrize("softcap,scale", [(0.05, 0.3), (50.0, 0.1), (50.0, 20.0), (1400.0, 5.0), (1500.0, 5.0), (20000.0, 5.0)])
+@pytest.mark.parametrize("type_,heads,kv,D,tiles", [("bf16", 24, 24, 128, 128), ("fp16", 48, 24, 64, 128), ("fp16", 2, 2, 128, 32), ("fp32", 2, 2, 64, 16)])
+def test_caps_low_and_high(dev, type_, heads, kv, D, tiles, softcap, scale):
+    """Caps that every score reaches, that none comes near, and past what the tiles of 128 rows add behind the softmax's own product."""
+    g = gen(int(softcap) + D)
+    slopes = torch.rand(heads, generator=g)
+    for o in ({}, {"slopes": slopes}):
+        attend(dev, type_, D, heads, kv, 16, [(130, 390)] if tiles == 128 else [(40, 390)], seed=D + heads, tiles=tiles, softcap=softcap, scale=scale, **o)
+
+
 @pytest.mark.parametrize("page", [8, 20])
 @pytest.mark.parametrize("D", [64, 128])
 def test_wide_rows_that_see_nothing(dev, D, page):
