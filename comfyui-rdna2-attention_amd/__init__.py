@@ -4,6 +4,7 @@ Drop-in for the reference's kernel modules -- ``hip_attention``, ``int8_gemm``, 
 ``attention`` keep their names, signatures, eligibility checks and fallbacks -- with hand-written gfx950 kernels
 behind a C ABI (librda_gfx950.so, include/rda.h). When ComfyUI is importable the package also registers the two
 nodes of the reference (``RDNA2Attention``, ``RDNA2TextGenerate``) as a thin shim over these modules.
+Beyond the reference, ``rotary`` and ``paged_kv`` serve text models: rotary positions and a key/value cache in pages.
 """
 import logging
 
