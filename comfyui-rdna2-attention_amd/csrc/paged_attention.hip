@@ -295,12 +295,15 @@ __device__ __forceinline__ int work_block(int grid) {
 
 // ------------------------------------------------------------------------------------------------ scores
 
-// log2(e) cap tanh(s / cap) from e = 2 log2(e) scale / cap s: tanh(y) = 1 - 2 / (1 + 2^(2 log2(e) y)). Its error of ~1e-7 cap is far below
-// a 16-bit type's; fp32 takes the odd series up to |y| = 1/4 (to y^9: the next term is below 1e-8 of the first).
-template <bool FP32>
+// log2(e) cap tanh(s / cap) from e = 2 log2(e) scale / cap s: tanh(y) = 1 - 2 / (1 + 2^(2 log2(e) y)). That is off by a few 2^-24 of cap,
+// however small the score: below a 16-bit type's own rounding of P for the caps that models use, but all of the score where the cap is
+// 10^6 times as large. FINE, for fp32 and for caps from HIGH_CAP on, takes the odd series up to |y| = 1/4 (to y^9: the next term is below 1e-8 of
+// the first): off by 2e-6 of the score.
+#define HIGH_CAP 2048.f  // log2(e) cap
+template <bool FINE>
 __device__ __forceinline__ float capped(float e, float cap) {
     const float t = __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(e)), 1.f);
-    if constexpr (FP32) {
+    if constexpr (FINE) {
         const float y = e * 0.34657359027997264f, z = y * y;  // ln(2) / 2
         float s = 62.f / 2835.f;
         s = __builtin_fmaf(s, z, -17.f / 315.f);
@@ -507,13 +510,18 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
                 const bool all = key0 + KT <= w.hi && !__any(bad != 0) && (key0 + KT <= n0 + 1 || key0 + KT <= w.prefix) &&
                                  (p.window <= 0 || n1 - key0 < p.window || key0 + KT <= w.prefix);
                 if constexpr (MOD) {
+                    const auto cap_all = [&](auto fine) __attribute__((always_inline)) {
+#pragma unroll
+                        for (int m = 0; m < MB; m++)
+#pragma unroll
+                            for (int e = 0; e < KG; e++) s[m][e] = capped<decltype(fine)::value>(s[m][e], p.cap);
+                    };
+                    if (FP32 ? p.cap > 0.f : p.cap >= HIGH_CAP) cap_all(std::true_type{});
+                    else if (p.cap > 0.f) cap_all(std::false_type{});
 #pragma unroll
                     for (int m = 0; m < MB; m++)
 #pragma unroll
-                        for (int e = 0; e < KG; e++) {
-                            if (p.cap > 0.f) s[m][e] = capped<FP32>(s[m][e], p.cap);
-                            s[m][e] = __builtin_fmaf(-slope[m], fabsf((float)(pos[m] - (key0 + KG * g + e))), s[m][e]);
-                        }
+                        for (int e = 0; e < KG; e++) s[m][e] = __builtin_fmaf(-slope[m], fabsf((float)(pos[m] - (key0 + KG * g + e))), s[m][e]);
                 }
                 u32 see[MB] = {};
                 bool split = false;  // a value that is not finite and that only some rows see
@@ -966,11 +974,15 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
                 return seen;
             };
             // What x is times in the softmax's exponent. Capped scores without a bias stay the -1 / (1 + 2^e) of their tanh (see capped), times 2 cap: that
-            // a row's scores are all cap too low changes nothing. (Where 2 cap passes 4096 they are made whole first, as large scores are, below.)
-            const float scale = !MOD ? p.scale : p.cap > 0.f && !p.slopes && p.cap < 2048.f ? 2.f * p.cap : 1.f;
+            // a row's scores are all cap too low changes nothing. (From HIGH_CAP on, 2 cap passes 4096 and they are made whole first, as large scores
+            // are, below.)
+            const float scale = !MOD ? p.scale : p.cap > 0.f && !p.slopes && p.cap < HIGH_CAP ? 2.f * p.cap : 1.f;
             auto bias = [&](float (&x)[16], int key0) __attribute__((always_inline)) {
                 if constexpr (MOD) {
-                    if (p.cap > 0.f) {
+                    if (__builtin_expect(p.cap >= HIGH_CAP, 0)) {
+#pragma unroll
+                        for (int r = 0; r < 16; r++) x[r] = capped<true>(x[r] * p.scale, p.cap);
+                    } else if (p.cap > 0.f) {
 #pragma unroll
                         for (int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x[r] * p.scale));
                         if (scale != 1.f) return;

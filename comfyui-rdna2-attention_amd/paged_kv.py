@@ -162,8 +162,9 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     """Attention of the batch's new tokens q (tokens, heads, D), the cache's type, D 64 or 128, over the cached keys of their sequences.
     A token at position n (its own key included) sees the keys j <= n; with window > 0 those with n - j < window; with prefix (int32,
     one per sequence) also those j < prefix[b], ahead of it or behind the window. Scores are scale q.k (scale None: D^-0.5); with
-    softcap > 0, softcap tanh(scale q.k / softcap), to 4e-7 of softcap; with slopes (fp32, one per head, finite), less slopes[h] |n - j|. heads is a multiple of
-    the cache's KV heads, which they share in order. A token that sees nothing gets 0. Returns out (q's shape, not overlapping q; rows of no
+    softcap > 0, softcap tanh(scale q.k / softcap), to 7e-7 of softcap, or, in fp32 and from a softcap of 1420 on, to 2e-6 of the score (so a cap
+    far above the scores changes nothing); with slopes (fp32, one per head, finite), less slopes[h] |n - j|. heads is a multiple of the
+    cache's KV heads, which they share in order. A token that sees nothing gets 0. Returns out (q's shape, not overlapping q; rows of no
     sequence left as they were), or a new tensor, with those rows 0."""
     kc, vc = cache._k, cache._v
     fill = out is None
