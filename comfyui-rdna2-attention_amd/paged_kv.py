@@ -9,7 +9,7 @@ import torch
 
 from . import _lib
 from .hip_attention import Kernels
-from .rotary import MAX_TOKENS, TYPES, Sizes, distinct, rows_ready, same_device, vector_rows
+from .rotary import MAX_TOKENS, TYPES, Sizes, distinct, rows_ready, same_device, vector_rows, written
 
 HEADS = (64, 128)  # head dims of `attention`
 MAX_SEQUENCES = 8192
@@ -119,6 +119,10 @@ def append(cache, batch, k, v, rotary=None, q=None, q_out=None):
                                           kc.data_ptr(), vc.data_ptr(), batch._table.data_ptr(), batch._starts.data_ptr(), batch._lengths.data_ptr(),
                                           None if rotary is None else rotary.turns.data_ptr(), 1.0 if rotary is None else rotary.factor,
                                           0 if rotary is None else rotary.interleaved, TYPES[k.dtype], TYPES[kc.dtype], dims, _lib.raw_stream()))
+    if q is None:
+        written(kc, vc)
+    else:
+        written(kc, vc, q_out)
     return q_out
 
 
@@ -202,6 +206,8 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     _lib.check(k.paged_attn(q.data_ptr(), address, kc.data_ptr(), vc.data_ptr(), batch._table.data_ptr(), batch._starts.data_ptr(), batch._lengths.data_ptr(),
                             None if prefix is None else prefix.data_ptr(), None if slopes is None else slopes.data_ptr(), workspace.data_ptr(),
                             scale, softcap, window, fill, type_, dims, _lib.raw_stream()))
+    if not fill:
+        written(out)
     return out
 
 

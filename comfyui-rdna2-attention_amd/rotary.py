@@ -122,6 +122,12 @@ def same_device(what, *tensors):
                 raise ValueError(f"{what} runs on the current GPU; its tensors are on {', '.join(sorted({str(x.device) for x in tensors if x is not None}))}")
 
 
+def written(*tensors):
+    """Counts a write in the tensors' versions, as torch's own in-place operations do: a kernel's write through an address counts none, and
+    int8_gemv's sibling linears and autograd would take the tensors for unchanged."""
+    torch._C._increment_version(tensors)
+
+
 class Sizes(dict):
     """The size arguments of an operator's calls by their tensors' types, shapes and strides: checked and packed once for each."""
 
@@ -141,7 +147,8 @@ def rotate(x, positions, rotary, out=None, inverse=False):
     turn in 32, rounded once. Values past rotary.dim are copied. inverse turns back: the gradient of x for a gradient of the result
     (and, where rotary.factor is 1, x itself). Any strides of x with a contiguous last dimension (other heads-first
     layouts are views of these shapes); out, if given, is x itself or does not overlap it. Returns out, or a new contiguous tensor."""
-    if out is None:
+    made = out is None
+    if made:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
@@ -157,6 +164,8 @@ def rotate(x, positions, rotary, out=None, inverse=False):
         return out
     _lib.check(get_kernels().rotate_positions(x.data_ptr(), out.data_ptr(), positions.data_ptr(), positions.dtype is torch.int64, rotary.turns.data_ptr(),
                                               rotary.factor, rotary.interleaved + 2 * bool(inverse), TYPES[x.dtype], dims, _lib.raw_stream()))
+    if not made:
+        written(out)
     return out
 
 
