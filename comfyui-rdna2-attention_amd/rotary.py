@@ -138,6 +138,20 @@ class Sizes(dict):
         return value
 
 
+class _Turn(torch.autograd.Function):
+    """rotate where gradients are recorded: linear in x, so that its gradient is the turn back (times the factor), and that one's the turn."""
+
+    @staticmethod
+    def forward(ctx, x, positions, rotary, inverse):
+        ctx.save_for_backward(positions, rotary.turns)
+        ctx.rotary, ctx.inverse = rotary, inverse
+        return rotate(x, positions, rotary, inverse=inverse)
+
+    @staticmethod
+    def backward(ctx, grad):
+        return rotate(grad, ctx.saved_tensors[0], ctx.rotary, inverse=not ctx.inverse), None, None, None
+
+
 _rotate_sizes = Sizes()
 
 
@@ -146,8 +160,13 @@ def rotate(x, positions, rotary, out=None, inverse=False):
     (tokens) or (batch, length), int32 or int64: a pair's angle is its frequency times the position, the product in 64 bits, the
     turn in 32, rounded once. Values past rotary.dim are copied. inverse turns back: the gradient of x for a gradient of the result
     (and, where rotary.factor is 1, x itself). Any strides of x with a contiguous last dimension (other heads-first
-    layouts are views of these shapes); out, if given, is x itself or does not overlap it. Returns out, or a new contiguous tensor."""
+    layouts are views of these shapes); out, if given, is x itself or does not overlap it. Returns out, or a new contiguous tensor, which
+    carries x's gradient where gradients are recorded (an out carries none, and is refused there if x or out requires one)."""
     made = out is None
+    if (x.requires_grad or (not made and out.requires_grad)) and torch.is_grad_enabled():
+        if not made:
+            raise ValueError("rotate records no gradient through out: leave it, or call under torch.no_grad()")
+        return _Turn.apply(x, positions, rotary, inverse)
     if made:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if x.data_ptr() % 16:
