@@ -4,6 +4,8 @@ int8_gemv.attention_decode, whose cache is one contiguous fp32 block per sequenc
 
 A step of a serving loop: write the batch's page table, starts and lengths; `append`; `attention` with the rotated queries. All three
 are device tensors that the kernels read: a captured graph of the two calls stays valid while their contents change.
+
+There is no backward pass: where gradients are recorded, tensors that require one are refused.
 """
 import torch
 
@@ -25,6 +27,13 @@ def get_kernels():
     return kernels
 
 
+def _no_gradient(what, *tensors):
+    """Raises ValueError if any of the tensors (None: none) requires a gradient and gradients are recorded."""
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what} has no backward pass and would drop the gradient of its inputs: call it under torch.no_grad(), or with detached tensors")
+
+
 class Cache:
     """The pages of a layer's keys and values: k and v (pages, page size, KV heads, D), fp16, bf16 or fp32, in any order of
     dimensions in memory but the last, which is contiguous (a (pages, KV heads, page size, D) pool is passed as its
@@ -37,6 +46,8 @@ class Cache:
             raise ValueError("Cache takes k and v with a contiguous last dimension and rows on 16-byte boundaries")
         if k.device != v.device:
             raise ValueError("Cache takes k and v on one device")
+        if k.requires_grad or v.requires_grad:
+            raise ValueError("Cache takes k and v that require no gradient: append writes them")
         self._k, self._v = k, v
         self.sizes = (k.dtype, k.shape, k.stride(), v.stride())
 
@@ -98,6 +109,7 @@ def append(cache, batch, k, v, rotary=None, q=None, q_out=None):
     have. Two tokens on one row of one page: either may remain. q_out is q itself or does not overlap q, k and v, and
     none of them overlaps the pages. Returns q_out."""
     kc, vc = cache._k, cache._v
+    _no_gradient("append", k, v, q, q_out)
     if q is not None:
         if q_out is None:
             q_out = q
@@ -171,6 +183,7 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     cache's KV heads, which they share in order. A token that sees nothing gets 0. Returns out (q's shape, not overlapping q; rows of no
     sequence left as they were), or a new tensor, with those rows 0."""
     kc, vc = cache._k, cache._v
+    _no_gradient("attention", q, slopes, out)
     fill = out is None
     if fill:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
