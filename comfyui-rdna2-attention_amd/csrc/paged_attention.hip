@@ -7,6 +7,9 @@
 // a tile's maximum exceeds it by more than 8 (2 in tiles of 128 rows), so that O is seldom rescaled. For an fp16 cache m stands below the
 // maximum by lift() and the terms are that much larger, near the top of fp16's range: one of 2^-21 of the largest still has all of
 // fp16's bits, where many keys of little weight stand beside one of much. A row that sees nothing (or only scores of -inf) is 0.
+// In 16-bit types the terms are rounded to the type, which the second product's matrix instructions take, and the sum is of the rounded terms, so that
+// the weights in use add up to 1. Beside the output's own rounding that costs little: rms errors are 1.1 times (single tokens, and fp16) to
+// 1.4 times (a bf16 chunk) those of 32-bit terms. Scores, m, l and O are held in 32 bits.
 //
 // Work. The query heads of a KV head share its keys: the rows of (sequence, KV head) are its (token, head) pairs in token order, MT
 // to a tile, so that single tokens of a group of heads fill a tile with no key read twice. A tile walks the keys that any of its rows
@@ -66,7 +69,8 @@ __device__ __forceinline__ int seq_rows(const PagedArgs& p, int b, int& first) {
 // What a tile costs before its first key, in units: us at 0 / 6 / 8 / 12 units for 24 heads x 4096 causal tokens 281 / 228 / 208 / 200, for a
 // chunk of 1001 beside 30 single tokens 95 / 76 / 74 / 74, for 20 ragged chunks over caches 187 / 143 / 135 / 137 (at 10: 143); with changed
 // scores, whose units take longer, at 3 / 4 / 6: 2 x 4096 capped in a window 225 / 214 / 213, 5 biased prompts 62 / 62 / 63. Tiles of
-// 16 rows at 0 / 1 / 2: 61 single tokens of ragged lengths 144.7 / 140.3 / 142.0, 32 sequences of 5 tokens 130 / 123 / 130.
+// 16 rows at 0 / 1 / 2: 61 single tokens of ragged lengths 144.7 / 140.3 / 142.0, 32 sequences of 5 tokens 130 / 123 / 130. (Times of the code that
+// the choice was made on; the 24 heads take 190 now.)
 __host__ __device__ constexpr int ahead(int mt, bool mod) { return mt == 128 ? (mod ? 4 : 8) : 1; }
 template <int MT, int UK, int AHEAD>
 __device__ __forceinline__ WorkTile make_tile(const PagedArgs& p, int b, int j) {
@@ -80,6 +84,8 @@ __device__ __forceinline__ WorkTile make_tile(const PagedArgs& p, int b, int j) 
     t.prefix = p.prefix ? min(max(p.prefix[b], 0), t.keys) : 0;
     const int n0 = t.p0 + div_by(t.r0, p.G), n1 = t.p0 + div_by(max(t.r1, 0), p.G);
     t.hi = min(t.keys, max(n1 + 1, t.prefix));
+    // With a prefix a tile's keys begin at 0, and those between the prefix and the window are walked too, though no row sees them: over 65536 keys
+    // with a window of 4096 a single token takes 14 us, with a prefix of 4 keys as well 59, a chunk of 512 tokens 78 and 513.
     t.lo = p.window > 0 && t.prefix == 0 && n0 >= p.window ? (n0 - p.window + 1) / UK * UK : 0;
     t.units = AHEAD + max((t.hi - t.lo + UK - 1) / UK, 1);  // a tile without keys is one unit: its rows are written too
     return t;
@@ -280,7 +286,8 @@ template <int MT, int D>
 __device__ __forceinline__ float* partial(const PagedArgs& p, int block, int which) {
     return (float*)(p.ws + (size_t)p.grid * sizeof(Cut)) + ((size_t)block * 2 + which) * MT * (D + 2);
 }
-// How far below the maximum m stands (see the top): with what a tile's maximum may exceed it by, terms reach 2^15.
+// How far below the maximum m stands (see the top). In the rows kernel a tile's maximum may exceed that by 8: a term is at most 2^15. In the tiles
+// kernel by 2: a term is at most 2^11, and the sum of a lane's 16 in a full step, which is what the step looks at, 2^15 (MOST).
 template <class T>
 __host__ __device__ constexpr float lift(int mt) { return std::is_same<T, half_t>::value ? (mt == 128 ? 9.f : 7.f) : 0.f; }
 // The offset of a row of a page.
@@ -345,8 +352,8 @@ __device__ __forceinline__ void store_row(T* out, const float (&y)[D / 16], floa
 //
 // K of the next tile is loaded as soon as the scores are computed, V as soon as O is: 16 KiB in flight for each of the CU's eight to twelve
 // waves, where the memory's latency at full rate needs ~32 KiB per CU. 64 single tokens over 8192 bf16 keys (8 KV heads of 128): 370 to 386 us
-// for 2.1 GB, 5.6 to 5.8 TB/s, where a sum of 1 GiB reads at 6.0. 61 over 1 to 16384 keys: 131 us for 657 MB, 5.0 TB/s: a run there is about two
-// tiles, each of which starts and ends with little in flight (~3 us). One fp32 token over 2048 keys: 7 to 9 us of latencies.
+// for 2.1 GB, 5.6 to 5.8 TB/s, where a sum of 1 GiB reads at 6.0. 61 over 1 to 16384 keys: 132 us for 657 MB, 5.0 TB/s: a run there is about two
+// tiles, each of which starts and ends with little in flight (~3 us). One fp32 token over 2048 keys: 8 to 9 us of latencies.
 template <class T>
 struct RowsTile {
     static constexpr bool FP32 = sizeof(T) == 4;
@@ -753,10 +760,10 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
 // * Keys past the sequence's end are copies of its last row, and those on pages that the cache does not have rows of page 0; masked
 //   tiles whose values are not all finite add them key by key to the rows that see them.
 //
-// A chunk of 2048 tokens, 32 heads over 8 KV heads of 128 bf16, over 14336 cached keys: 546 to 554 us for 515 GFLOP, 0.94 PFLOP/s, 78% of what a library
-// product of 8192^3 reaches. The matrix instructions run in 47% of the cycles (at 1.6 to 1.9 GHz, the chip's power limit) and five other vector
+// A chunk of 2048 tokens, 32 heads over 8 KV heads of 128 bf16, over 14336 cached keys: 538 to 554 us for 515 GFLOP, 0.94 PFLOP/s, 69 to 80% of what a
+// library product of 8192^3 reaches (1.18 to 1.37 by the box). The matrix instructions run in 47% of the cycles (at 1.6 to 1.9 GHz, the chip's power limit) and five other vector
 // instructions stand beside each; the two do not overlap within a wave's SIMD, and add up to nearly all of them. LDS reads meet no bank conflict.
-// Capped scores take three transcendentals each where plain ones take one: 2 x 4096 tokens of 16 heads of 128 in a window of 2048, 103 GFLOP, 198 us:
+// Capped scores take three transcendentals each where plain ones take one: 2 x 4096 tokens of 16 heads of 128 in a window of 2048, 103 GFLOP, 190 us:
 // at two workgroups a CU vector work and products fill ~80% of the cycles (217 us with the whole capped score made before the softmax's product).
 // With D = 64 a score's exponential stands beside half the products. Tiles that are masked cost ~2.4 full ones, a tile's start ~7 us of latency.
 template <int D>
@@ -1356,15 +1363,19 @@ struct Plan {
 static int make_plan(long T, long B, long H, long Hkv, long D, int type, Plan* plan) {
     if (T <= 0 || B <= 0 || B > MAX_SEQUENCES || Hkv <= 0 || H <= 0 || H % Hkv || (D != 64 && D != 128) || type < RDA_FP16 || type > RDA_FP32) return RDA_ERR_INVALID;
     if (T * (H / Hkv) >= 1L << 31) return RDA_ERR_INVALID;
-    // Tiles of 16, 32 or 128 rows by the rows of a sequence and KV head, on average (a lower or higher number in one of them costs time only),
-    // us 16 / 32 / 128: 32 sequences over 4096 keys, of 16 rows 113 / 121 / 142, 32 rows 130 / 125 / 144, 64 rows 249 / 140 / 157, 96 rows
+    // Tiles of 16, 32 or 128 rows by the rows of a sequence and KV head, on average. (A lower or higher number in one of them costs time only: a chunk
+    // of 512 tokens over 3584 keys beside 64 single ones over 4096 takes tiles of 32 rows, 286 us where the two alone take 75 + 197, one of 2048 over 2048
+    // beside 255 of them 1017 where they take 152 + 753; beside 30 it takes tiles of 128.) us 16 / 32 / 128: 32 sequences over 4096 keys, of 16 rows 113 / 121 / 142, 32 rows 130 / 125 / 144, 64 rows 249 / 140 / 157, 96 rows
     // 368 / 324 / 172. Where all tiles of 128 rows together are few, each is cut into many parts, which cost more than the keys that
     // tiles of 32 read again: over 8192 keys, 128-row tiles x KV heads 16 (24 tokens of one sequence) 34 / 68, 32 (128 tokens) 67.7 / 66.1, 48
     // (192) 84 / 73; over 4096 keys, 32 (4 x 24 tokens) 43 / 63, 48 (2 x 96) 54 / 59, 64 (4 x 48) 70 / 61. fp32 keeps 16 rows, whose
     // matrix products bound it (32 sequences of 16 rows 186, in tiles of 32 rows 242; 32 rows 238 / 247; 512 tokens over 512 105 / 110).
     const long rows = T * (H / Hkv) / B;
     plan->mt = rows <= 16 || type == RDA_FP32 ? 16 : rows <= 64 || B * ((rows + 127) / 128) * Hkv <= 40 ? 32 : 128;
-    // What the chip holds at a time: two or three workgroups on each of 256 CUs, by registers (three of the 64-dim and of the 128-row kernels).
+    // Two or three workgroups on each of 256 CUs, by registers: two of the tiles of 32 rows and of 128-dim ones of 16, three of 64-dim ones of 16 and of 128
+    // rows (capped or biased 128-dim ones of 128: two, below). Some forms would fit one more (64-dim ones of 16 rows where pages hold whole runs, or in
+    // fp32, and plain bf16 ones of 32). The workspace is sized for this grid, also where a short call launches less of it: at D = 128 in MB 8.5 for tiles
+    // of 16 rows, 17 of 32, 102 of 128, half of it at D = 64 (16 rows: 6.5).
     plan->grid = (D == 128 && plan->mt == 16) || plan->mt == 32 ? 512 : 768;
     if ((T * (H / Hkv) / plan->mt + 1) * B >= 1L << 31) return RDA_ERR_INVALID;
     plan->workspace = (size_t)plan->grid * sizeof(Cut) + (size_t)plan->grid * 2 * plan->mt * (D + 2) * 4;

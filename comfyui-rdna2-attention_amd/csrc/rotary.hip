@@ -19,7 +19,7 @@
 #define MAX_ROWS ((1L << 26) - 64)  // tokens of a call: a grid has fewer than 2^32 threads
 
 // Cosine and sine of a turn's fraction: n f - rint(4 n f) / 4 = y / 4, |y| <= 1/2, then the series at y pi / 2 (at most pi / 4:
-// the first terms left out are below 2e-9 and 1e-10).
+// the first terms left out are below 2e-9 and 1.2e-10).
 __device__ __forceinline__ f2 cos_sin(double position, double turns) {
     const double quarters = 4.0 * (position * turns), whole = rint(quarters);
     const float y = (float)(quarters - whole), z = y * y;

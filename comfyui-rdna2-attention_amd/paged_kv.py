@@ -37,7 +37,7 @@ def _no_gradient(what, *tensors):
 class Cache:
     """The pages of a layer's keys and values: k and v (pages, page size, KV heads, D), fp16, bf16 or fp32, in any order of
     dimensions in memory but the last, which is contiguous (a (pages, KV heads, page size, D) pool is passed as its
-    transpose(1, 2)); rows on 16-byte boundaries. Any page size; multiples of 8 tokens (fp32: 4) are read fastest."""
+    transpose(1, 2)); rows on 16-byte boundaries, no gradient required. Any page size; multiples of 8 tokens (fp32: 4) are read fastest."""
 
     def __init__(self, k, v):
         if k.dim() != 4 or k.shape != v.shape or k.dtype not in TYPES or v.dtype != k.dtype or k.numel() == 0 or k.shape[3] % 16:
@@ -58,9 +58,9 @@ class Cache:
 class Batch:
     """The sequences of a step, all int32 on the device: table (sequences, pages per sequence) -- a sequence's page ids in
     order, entries past its length unread --, starts (sequences + 1) -- its new tokens are rows starts[b] .. starts[b + 1] - 1 of q, k
-    and v --, and lengths (sequences) -- its cached tokens, the new ones included. starts does not fall; rows behind the last sequence
-    (a padded batch) belong to none. A length past the table's capacity counts as the capacity; keys on pages that the
-    cache does not have are masked."""
+    and v --, and lengths (sequences) -- its cached tokens, the new ones included. starts does not fall and ends within those rows; rows behind
+    the last sequence (a padded batch) belong to none. Of a length past the table's capacity only the keys that the table holds are there;
+    positions, and windows with them, follow the length. Keys on pages that the cache does not have are masked."""
 
     def __init__(self, table, starts, lengths):
         if table.dim() != 2 or starts.dim() != 1 or lengths.dim() != 1 or any(t.dtype != torch.int32 for t in (table, starts, lengths)):
@@ -106,7 +106,8 @@ def append(cache, batch, k, v, rotary=None, q=None, q_out=None):
     and v are fp16, bf16 or fp32, of the cache's type or another: rounded to it once, after the turn. q (tokens, heads, D), if
     given, is turned in the same launch into q_out (the cache's type; None: in place) -- what attention takes. Rows of no
     sequence are left as they were in q_out, as is the cache where a position is negative, past the table or on a page that it does not
-    have. Two tokens on one row of one page: either may remain. q_out is q itself or does not overlap q, k and v, and
+    have. Two tokens on one row of one page: either's values may remain, or
+    some of each. q_out is q itself or does not overlap q, k and v, and
     none of them overlaps the pages. Returns q_out."""
     kc, vc = cache._k, cache._v
     _no_gradient("append", k, v, q, q_out)
@@ -181,7 +182,8 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     softcap > 0, softcap tanh(scale q.k / softcap), to 7e-7 of softcap, or, in fp32 and from a softcap of 1420 on, to 2e-6 of the score (so a cap
     far above the scores changes nothing); with slopes (fp32, one per head, finite), less slopes[h] |n - j|. heads is a multiple of the
     cache's KV heads, which they share in order. A token that sees nothing gets 0. Returns out (q's shape, not overlapping q; rows of no
-    sequence left as they were), or a new tensor, with those rows 0."""
+    sequence left as they were), or a new tensor, with those rows 0. Keys between a prefix and the window cost time as if they were seen. A call takes
+    up to 102 MB of workspace from torch's allocator."""
     kc, vc = cache._k, cache._v
     _no_gradient("attention", q, slopes, out)
     fill = out is None
