@@ -115,3 +115,33 @@ def test_gradient_on_the_gpu(dev, type_, layout):
             ref, off = turned(src, positions, rot, inverse)
             assert ((got.cpu().double() - ref).abs() <= off + rounding(ref.abs() + off, type_)).all()
         torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.gpu
+def test_captured_gradient(dev):
+    """A turn and its gradient captured together, replayed while the values, the gradient and the positions change: the eager bits each time."""
+    g = gen(7)
+    rot = rotary.Rotary(64, device=dev)
+    x = torch.randn(9, 4, 64, generator=g).bfloat16().to(dev).requires_grad_()
+    weight, positions = torch.randn(9, 4, 64, generator=g).bfloat16().to(dev), torch.arange(9, dtype=torch.int32, device=dev)
+
+    def step():
+        y = rotary.rotate(x, positions, rot)
+        return y.detach(), torch.autograd.grad(y, x, weight)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, grad = step()
+    for i in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(9, 4, 64, generator=g).bfloat16())
+            weight.copy_(torch.randn(9, 4, 64, generator=g).bfloat16())
+            positions += 1000
+        graph.replay()
+        want = step()
+        assert torch.equal(y, want[0]) and torch.equal(grad, want[1]), i
