@@ -41,3 +41,11 @@ static inline Div make_div(int d) {
     return v;
 }
 __device__ __forceinline__ int div_by(int n, const Div& v) { return (int)((__umulhi((u32)n, v.m) + (u32)n) >> v.s); }
+
+// Values are read and written in vectors of eight: 16-byte aligned bases and strides.
+static bool vector_rows(const void* p, const long* strides, int n, int type) {
+    const long m = type == RDA_FP32 ? 4 : 8;
+    for (int i = 0; i < n; i++)
+        if (strides[i] % m) return false;
+    return ((uintptr_t)p & 15) == 0;
+}
