@@ -54,6 +54,13 @@ SIGNATURES = {
     "rda_rms_norm_rope": (_i, [_p, _p, _p, _i, _i, _i, _i, _l, _l, _l, _f, _p, _l, _p]),
     "rda_rotate_positions": (_i, [_p, _p, _p, _i, _p, _f, _i, _i, _p, _p]),
     "rda_paged_append": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _p, _p]),
+    "rda_norm_rotate": (_i, [_p, _p, _p, _p, _p, _i, _p, _p, _i, _f, _p, _f, _i, _i, _p, _p]),
+    "rda_norm_rotate_back_workspace": (_sz, [_l, _l, _l, _l]),
+    "rda_norm_rotate_back": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _p, _i, _f, _p, _f, _i, _p, _i, _p, _p]),
+    "rda_paged_append_i8": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _f, _i, _p, _p, _i, _f, _i, _i, _p, _p]),
+    "rda_paged_read_i8": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _p]),
+    "rda_paged_attn_i8_workspace": (_sz, [_l, _l, _l, _l, _l, _i]),
+    "rda_paged_attn_i8": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _f, _f, _i, _i, _i, _p, _p]),
     "rda_paged_attn_workspace": (_sz, [_l, _l, _l, _l, _l, _i]),
     "rda_paged_attn": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _f, _f, _i, _i, _i, _p, _p]),
 }

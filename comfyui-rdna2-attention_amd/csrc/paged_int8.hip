@@ -1,0 +1,734 @@
+// A paged key/value cache held in 8 bits: values quantized as they are written, read back, and attention over them.
+//
+// Codes are int8; a block of 16, 32 or 64 consecutive tokens of a KV head has one scale in fp32 for its keys and one for its values: a value is
+// code x scale, the scale the block's largest magnitude / 127. Pages are whole blocks, and blocks are whole groups of 16 tokens, so that 16 aligned keys
+// share a page, a table entry and a scale. A scale that is not finite stands for a block of NaN, which is what values that are not all finite become.
+#include "paged_work.h"
+#include "rotary.h"
+
+#define MAX_KEYS8 ((1L << 31) - (1L << 16))
+
+// ------------------------------------------------------------------------------------------------ appending
+
+struct Append8Args {
+    RotaryArgs r;
+    const void *q, *k, *v;
+    void* qo;
+    signed char *kc, *vc;
+    float *ks, *vs;
+    const int *table, *starts, *lengths;
+    const void *qw, *kw;  // weights of the heads' norms, or null
+    int wtype;
+    float eps;
+    int T, H, Hkv, B, N, P, block, slice;  // tokens of a block (16, 32, 64); heads of a workgroup
+    Div S;
+    long pitch, sqt, sqh, skt, skh, svt, svh, sot, soh, kpp, kpr, kph, vpp, vpr, vph, ksp, ksb, ksh, vsp, vsb, vsh;
+};
+
+// Workgroups (x, *) take a block of one sequence's new tokens each. Sequence b's are the x from first_slot(b) on: with its n new tokens it touches at most
+// (n - 2) / block + 2 blocks, and has n / block rounded down + 2 slots at least, whatever its position, so that no sums over the sequences are needed.
+__device__ __forceinline__ int first_slot(const Append8Args& p, int b) { return min(max(p.starts[b], 0), p.T) / p.block + 2 * b; }
+__device__ __forceinline__ int sequence_of_slot(const Append8Args& p, int slot, int lane) {
+    int at = 0, n = p.B;  // as sequence_of: the number of first slots of 1 .. B at or below slot
+    while (n > 64) {
+        const int step = (n + 63) >> 6, i = (lane + 1) * step;
+        const bool below = i <= n && first_slot(p, at + i) <= slot;
+        const int c = __popcll(__ballot(below));
+        at += c * step;
+        n = min(step - 1, n - c * step);
+    }
+    const bool below = lane < n && first_slot(p, at + 1 + lane) <= slot;
+    return at + __popcll(__ballot(below));
+}
+
+// The largest over the wave's lanes.
+__device__ __forceinline__ u32 wave_max(u32 x) {
+    x = max(x, (u32)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, true));
+    x = max(x, (u32)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true));
+    x = max(x, (u32)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xF, 0xF, true));
+    x = max(x, (u32)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xF, 0xF, true));
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max((u32)a[0], (u32)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max((u32)b[0], (u32)b[1]);
+}
+__device__ __forceinline__ int to_code(float x) { return (int)rintf(fminf(fmaxf(x, -127.f), 127.f)); }
+// Eight quotients as codes.
+__device__ __forceinline__ void store_codes(signed char* p, const f8& x) {
+    *(u2v*)p = (u2v){pack4(to_code(x[0]), to_code(x[1]), to_code(x[2]), to_code(x[3])), pack4(to_code(x[4]), to_code(x[5]), to_code(x[6]), to_code(x[7]))};
+}
+// x / s by 1 / s and one correction, to within an ulp: ties of values that 16 bits hold fall as those of the division do.
+__device__ __forceinline__ f8 over(const f8& x, float s, float by) {
+    f8 y;
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = div_by_scale(x[e], s, by);
+    return y;
+}
+__device__ __forceinline__ f8 load_codes(const signed char* p) {
+    const u2v w = *(const u2v*)p;
+    f8 x;
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = (float)(int)(signed char)(w[i >> 2] >> (8 * (i & 3)));
+    return x;
+}
+#define FLT_TOP 3.402823466e38f
+#define LEAST_SCALE 1e-30f
+
+// One step's keys and values as codes into their blocks, keys normed and turned on the way, and queries normed and turned. A workgroup takes a block
+// and `slice` heads (queries, keys, values in this order): it makes the angles of the block's new tokens once, and takes 16 tokens of a head to a wave, block / 16
+// waves to a head. A block whose first tokens are older keeps a scale at least as large as it had; where the scale grows the older codes are
+// rounded anew to it by the same workgroup, which alone writes the block of that head.
+template <class X, class Q, int PS>
+__global__ __launch_bounds__(256) void append8_kernel(Append8Args p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ u32 most[2][4];
+    f2* cs = (f2*)smem;  // [row of the block][pair]
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int slot = blockIdx.x, b = __builtin_amdgcn_readfirstlane(sequence_of_slot(p, slot, lane));
+    if (b >= p.B) return;
+    const int first = min(max(p.starts[b], 0), p.T), tokens = min(max(p.starts[b + 1], first), p.T) - first;
+    if (tokens == 0) return;
+    const int p0 = max(p.lengths[b], -(1 << 30)) - tokens;             // position of the first new token; negative: no place for it
+    const int shift = p.block == 16 ? 4 : p.block == 32 ? 5 : 6;
+    const int b0 = ((p0 >> shift) + (slot - first_slot(p, b))) << shift;  // the block's first position
+    const int o0 = max(p0 - b0, 0), o1 = min(p0 + tokens - b0, p.block);  // its new rows
+    if (o0 >= o1) return;
+    const int head0 = blockIdx.y * p.slice, head1 = min(head0 + p.slice, p.H + 2 * p.Hkv);
+    const int entry = b0 >= 0 ? div_by(b0, p.S) : p.N;
+    int page = -1;
+    if (entry < p.N) page = p.table[b * p.pitch + entry];
+    const bool there = page >= 0 && page < p.P;
+    const int row0 = there ? b0 - entry * (int)p.S.d : 0, part0 = row0 >> shift;  // the block's first row of the page; its number there
+
+    const int pairs = p.r.R / 2;
+    if (pairs && head0 < p.H + p.Hkv) {
+        for (int i = t; i < (o1 - o0) * pairs; i += 256) {
+            const int row = o0 + i / pairs, pair = i % pairs;
+            const f2 v = cos_sin((double)(b0 + row), p.r.turns[pair]);
+            cs[row * pairs + pair] = (f2){v[0] * p.r.factor, v[1] * p.r.factor};
+        }
+        __syncthreads();
+    }
+    const Place pl = place(p.r, lane);
+    const int per = p.r.D / 16, waves = p.block >> 4, sub = wave & (waves - 1), together = 4 / waves;  // waves of a head; the wave's 16 rows; heads at once
+    int row[PS];
+    bool mine[PS];
+#pragma unroll
+    for (int i = 0; i < PS; i++) {
+        const int x = i * pl.heads + pl.head;
+        row[i] = 16 * sub + x;
+        mine[i] = pl.head < pl.heads && x < 16 && row[i] >= o0 && row[i] < o1;
+    }
+    int turn_of = 0;
+    for (int h0 = head0; h0 < head1; h0 += together, turn_of ^= 1) {
+        const int h = h0 + wave / waves, hk = h - p.H, hv = hk - p.Hkv;
+        const bool active = h < head1;
+        f8 lo[PS], hi[PS];
+        if (active) {
+            const X* src = hk < 0 ? (const X*)p.q + h * p.sqh : hv < 0 ? (const X*)p.k + hk * p.skh : (const X*)p.v + hv * p.svh;
+            const long st = hk < 0 ? p.sqt : hv < 0 ? p.skt : p.svt;
+#pragma unroll
+            for (int i = 0; i < PS; i++) {
+                const X* at = src + (first + b0 - p0 + (mine[i] ? row[i] : o0)) * st;
+                lo[i] = load8(at + pl.at);
+                hi[i] = load8(at + pl.to);
+            }
+            const void* w = hk < 0 ? p.qw : hv < 0 ? p.kw : nullptr;
+            if (w) {
+                const f8 wl = weights8(w, p.wtype, pl.at), wh = weights8(w, p.wtype, pl.to);
+#pragma unroll
+                for (int i = 0; i < PS; i++) {
+                    const float inv = inverse_rms(lo[i], hi[i], p.r.D, p.eps, per, lane);
+                    lo[i] = lo[i] * inv * wl;
+                    hi[i] = hi[i] * inv * wh;
+                }
+            }
+            if (hv < 0 && pl.pair >= 0) {
+#pragma unroll
+                for (int i = 0; i < PS; i++) {
+                    f8 c, s;
+                    angles_of(pl, cs + (mine[i] ? row[i] : o0) * pairs, c, s);
+                    turn(lo[i], hi[i], c, s, p.r.interleaved);
+                }
+            }
+            if (hk < 0) {
+#pragma unroll
+                for (int i = 0; i < PS; i++)
+                    if (mine[i]) {
+                        Q* dst = (Q*)p.qo + (long)(first + b0 - p0 + row[i]) * p.sot + h * p.soh;
+                        store8(dst + pl.at, lo[i]);
+                        store8(dst + pl.to, hi[i]);
+                    }
+            }
+        }
+        if (h0 + together <= p.H) continue;  // queries all (the same for the workgroup)
+        u32 top = 0;  // magnitudes order as their bits do, infinities and NaN above the finite ones
+        if (active && hk >= 0) {
+#pragma unroll
+            for (int i = 0; i < PS; i++)
+                if (mine[i])
+#pragma unroll
+                    for (int e = 0; e < 8; e++) top = max(top, max(__float_as_uint(lo[i][e]) & 0x7fffffffu, __float_as_uint(hi[i][e]) & 0x7fffffffu));
+            top = wave_max(top);
+        }
+        const bool writes = active && hk >= 0 && there;
+        float* scale = nullptr;
+        float had = 0.f;
+        if (writes) {
+            scale = hv < 0 ? p.ks + page * p.ksp + part0 * p.ksb + hk * p.ksh : p.vs + page * p.vsp + part0 * p.vsb + hv * p.vsh;
+            if (o0 > 0) had = *scale;
+        }
+        if (waves > 1) {  // also: every wave has read the scale before one writes it
+            if (lane == 0) most[turn_of][wave] = top;
+            __syncthreads();
+            for (int i = wave & ~(waves - 1), n = i + waves; i < n; i++) top = max(top, most[turn_of][i]);
+        }
+        if (!writes) continue;
+        signed char* codes = hv < 0 ? p.kc + page * p.kpp + row0 * p.kpr + hk * p.kph : p.vc + page * p.vpp + row0 * p.vpr + hv * p.vph;
+        const long cr = hv < 0 ? p.kpr : p.vpr;
+        const float need = fmaxf(__uint_as_float(top) / 127.f, LEAST_SCALE);
+        const bool finite = top < 0x7f800000u && had <= FLT_TOP;
+        const float now = finite ? fmaxf(need, had) : __builtin_nanf(""), by = finite ? 1.f / now : 0.f;
+#pragma unroll
+        for (int i = 0; i < PS; i++) {
+            if (mine[i]) {
+                store_codes(codes + row[i] * cr + pl.at, finite ? over(lo[i], now, by) : (f8){});
+                store_codes(codes + row[i] * cr + pl.to, finite ? over(hi[i], now, by) : (f8){});
+            }
+        }
+        if (o0 > 0 && finite && now != had) {
+            const float shrink = had * by;
+#pragma unroll
+            for (int i = 0; i < PS; i++) {
+                const int x = i * pl.heads + pl.head;
+                if (pl.head < pl.heads && x < 16 && row[i] < o0) {
+                    signed char* at = codes + row[i] * cr;
+                    const f8 a = load_codes(at + pl.at), z = load_codes(at + pl.to);
+                    store_codes(at + pl.at, a * shrink);
+                    store_codes(at + pl.to, z * shrink);
+                }
+            }
+        }
+        if (sub == 0 && lane == 0) *scale = now;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ reading back
+
+struct Read8Args {
+    const signed char *kc, *vc;
+    const float *ks, *vs;
+    const int *table, *starts, *lengths;
+    void *ko, *vo;
+    int T, Hkv, D, B, N, P, shift;
+    Div S;
+    long pitch, kpp, kpr, kph, vpp, vpr, vph, ksp, ksb, ksh, vsp, vsb, vsh;
+};
+
+// Keys and values of a batch's rows as the values that their codes stand for: a wave takes a row, its lanes 16 values each. Rows of no
+// sequence, and of positions that the cache does not have, are 0.
+template <class X>
+__global__ __launch_bounds__(256) void read8_kernel(Read8Args p) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), token = blockIdx.x * 4 + wave;
+    if (token >= p.T) return;
+    const int b = __builtin_amdgcn_readfirstlane(sequence_of(p.starts, p.B, token, lane));
+    int page = -1, row = 0;
+    if (b < p.B && token >= p.starts[b]) {
+        const long n = (long)p.lengths[b] - p.starts[b + 1] + token;
+        const int entry = n >= 0 && n < 1L << 31 ? div_by((int)n, p.S) : p.N;
+        if (entry < p.N) page = p.table[b * p.pitch + entry], row = (int)n - entry * (int)p.S.d;
+    }
+    const bool there = page >= 0 && page < p.P;
+    const int per = p.D / 16, chunks = p.Hkv * per;
+    for (int i = lane; i < 2 * chunks; i += 64) {
+        const bool value = i >= chunks;
+        const int c = value ? i - chunks : i, h = c / per, at = c % per * 16;
+        f8 lo = {}, hi = {};
+        if (there) {
+            const signed char* src = (value ? p.vc + page * p.vpp + row * p.vpr + h * p.vph : p.kc + page * p.kpp + row * p.kpr + h * p.kph) + at;
+            const float scale = value ? p.vs[page * p.vsp + (row >> p.shift) * p.vsb + h * p.vsh] : p.ks[page * p.ksp + (row >> p.shift) * p.ksb + h * p.ksh];
+            const float by = scale <= FLT_TOP ? scale : __builtin_nanf("");
+            lo = load_codes(src) * by;
+            hi = load_codes(src + 8) * by;
+        }
+        X* dst = (X*)(value ? p.vo : p.ko) + ((long)token * p.Hkv + h) * p.D + at;
+        store8(dst, lo);
+        store8(dst + 8, hi);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ attention
+
+struct Attn8Args : PagedArgs {
+    const float *ks, *vs;
+    u32 ksp, ksb, vsp, vsb;  // strides of pages and of blocks of the scales
+    long ksh, vsh;
+    int shift;  // log2 of a block's tokens
+};
+#define LIFT8 7.f  // P stands 2^7 above 2^(x - m), so that it may be 2^15 where m lags by 8
+
+// Codes as fp16: byte b, its sign bit flipped, in the low byte of 0x6400 is 1024 + 128 + code; less 1152 it is the code, exactly.
+__device__ __forceinline__ u32 less_bias(u32 w) {
+    return __builtin_bit_cast(u32, __builtin_bit_cast(h2, w) + (h2){(half_t)-1152.f, (half_t)-1152.f});
+}
+__device__ __forceinline__ u2v widen4(u32 w) {
+    w ^= 0x80808080u;
+    return (u2v){less_bias(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)), less_bias(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u))};
+}
+// Byte j of a and of b as two fp16 codes (j a constant).
+__device__ __forceinline__ u32 widen_pair(u32 a, u32 b, int j) {
+    return less_bias(__builtin_amdgcn_perm(b, a, 0x0c000c00u | (u32)j | (u32)(4 + j) << 16) ^ 0x64806480u);
+}
+__device__ __forceinline__ f4 product16(const u4v& a, const u4v& b, const f4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+// Tiles of 16 MB rows, as rows_kernel of 16-bit caches (paged_attention.hip) has them, in units of 256 keys: a wave's tile is 64 keys, lane
+// group g = l / 16 holding the scores of keys 16 g .. 16 g + 15 (score block c's row 4 g + i stands for key 16 g + 4 c + i), which share a page and a
+// scale of K and of V. All products are of fp16: codes are exact there, and a row of q is brought to a largest magnitude of 2^14 to 2^15 by a power
+// of two that its scores' factor takes back (a bf16 value less than 2^-28 of its row's largest may lose bits). P is what the scale of V leaves of
+// it relative to the largest scale that the row has met, vm: O is in units of vm, and rescaled when that grows, as when the maximum moves. l sums P
+// before both.
+template <class T, int D, int MB, bool MOD>
+__global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
+    constexpr int KT = 64, KG = 16, UK = 4 * KT, MT = 16 * MB, AHEAD = ahead(MT, MOD);
+    constexpr int KC = D / 64;  // 16-byte vectors of a lane's part of a K row
+    constexpr int VC = D / 16;  // consecutive dims of a lane's part of a V row
+    constexpr int OP = D + 4;   // pitch of a row of O in LDS
+    typedef typename std::conditional<VC == 8, u2v, u32>::type vvec;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ u32 shared[256 + 8];
+    __shared__ float ml[2][4][16];
+    const int t = threadIdx.x, lane = t & 63, g = lane >> 4, r = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int block = work_block(p.grid);
+    Run run = find_run<MT, UK, AHEAD, 256>(p, (int*)smem, shared, block);
+    Cut cut = {};
+
+    while (run.count > 0) {
+        const WorkTile w = uniform(make_tile<MT, UK, AHEAD>(p, run.b, run.j));
+        if (run.unit + run.count <= AHEAD) break;  // the next run's
+        const bool begins = run.unit == 0, last_part = run.unit + run.count >= w.units, whole = begins && last_part;
+        const int u0 = begins ? 0 : run.unit - AHEAD, u1 = min(w.units, run.unit + run.count) - AHEAD, n = u1 - u0;
+        const int* table = p.table + run.b * p.pitch;
+        const signed char* kbase = (const signed char*)p.k + run.kvh * p.kph;
+        const signed char* vbase = (const signed char*)p.v + run.kvh * p.vph;
+        const float *ksbase = p.ks + run.kvh * p.ksh, *vsbase = p.vs + run.kvh * p.vsh;
+
+        // Q as the B operand: lane (g, r) has values 64 x + 16 g .. + 15 of row r, as it has of the K rows.
+        u4v qf[MB][KC][2];
+        int pos[MB], pre[MB];
+        float slope[MB], by[MB];  // by: what a product is times, but the key's scale
+#pragma unroll
+        for (int m = 0; m < MB; m++) {
+            const int row = w.r0 + 16 * m + r, rc = min(row, w.r1), token = div_by(rc, p.G), head = run.kvh * (int)p.G.d + rc - token * (int)p.G.d;
+            const T* src = (const T*)p.q + (long)(w.first + token) * p.sqt + head * p.sqh;
+            f8 x[KC][2];
+            float top = 0.f;
+#pragma unroll
+            for (int c = 0; c < KC; c++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    x[c][h] = load8(src + 64 * c + 16 * g + 8 * h);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[c][h][e]));
+                }
+            top = rows_max(top);
+            const int up = top > 0.f && top <= FLT_TOP ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+            by[m] = ldexpf(p.scale, -up);
+#pragma unroll
+            for (int c = 0; c < KC; c++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[c][h][e] = ldexpf(x[c][h][e], up);
+                    qf[m][c][h] = __builtin_bit_cast(u4v, __builtin_convertvector(x[c][h], h8));
+                }
+            pos[m] = row <= w.r1 ? w.p0 + token : -1;
+            pre[m] = row <= w.r1 ? w.prefix : 0;
+            slope[m] = MOD && p.slopes ? p.slopes[head] * LOG2E : 0.f;
+        }
+        const int n0 = uniform(w.p0 + div_by(w.r0, p.G)), n1 = uniform(w.p0 + div_by(w.r1, p.G));
+
+        f4 o[MB][VC];
+        float m_[MB], l_[MB], vm[MB];
+#pragma unroll
+        for (int m = 0; m < MB; m++) {
+#pragma unroll
+            for (int j = 0; j < VC; j++) o[m][j] = (f4){};
+            m_[m] = -__builtin_inff();
+            l_[m] = 0.f;
+            vm[m] = 1e-36f;  // 128 / vm stays finite
+        }
+
+        if (w.hi > w.lo) {
+            const int last = (w.hi - 1) / KG * KG;
+            auto key_of = [&](int i) __attribute__((always_inline)) { return w.lo + (u0 + i) * UK + wave * KT; };
+            int kid, vid;  // table entries of the lane's K rows and of its keys of V
+            auto fetch_ids = [&](int i) __attribute__((always_inline)) {
+                const int key0 = key_of(i);
+                kid = table[div_by(min(key0 + KG * (r >> 2), last), p.S)];
+                vid = table[div_by(min(key0 + KG * g, last), p.S)];
+            };
+            u4v kf[4][KC];
+            vvec vf[KG];
+            float ks = 0.f, vs = 0.f;
+            bool bad = false;  // the lane's keys are on a page that the cache does not have
+            auto load_k = [&](int i) __attribute__((always_inline)) {
+                const int key = min(key_of(i) + KG * (r >> 2), last), row = key - div_by(key, p.S) * (int)p.S.d + (r & 3);
+                const signed char* src = kbase + row_at((u32)kid < (u32)p.P ? (u32)kid : 0, p.kpp, (u32)row, p.kpr) + 16 * g;
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int x = 0; x < KC; x++) kf[c][x] = *(const u4v*)(src + (unsigned long long)(4 * c) * p.kpr + 64 * x);
+            };
+            auto load_v = [&](int i) __attribute__((always_inline)) {
+                const int key = min(key_of(i) + KG * g, last), row = key - div_by(key, p.S) * (int)p.S.d;
+                const u32 page = (u32)vid < (u32)p.P ? (u32)vid : 0;
+                bad = (u32)vid >= (u32)p.P;
+                const signed char* src = vbase + row_at(page, p.vpp, (u32)row, p.vpr) + r * VC;
+#pragma unroll
+                for (int e = 0; e < KG; e++) vf[e] = *(const vvec*)(src + (unsigned long long)e * p.vpr);
+                ks = ksbase[row_at(page, p.ksp, (u32)row >> p.shift, p.ksb)];
+                vs = vsbase[row_at(page, p.vsp, (u32)row >> p.shift, p.vsb)];
+            };
+            fetch_ids(0);
+            load_k(0);
+            load_v(0);
+            if (n > 1) fetch_ids(1);
+            for (int i = 0; i < n; i++) {
+                const int key0 = key_of(i);
+                if (!(ks <= FLT_TOP)) ks = __builtin_nanf("");
+                float s[MB][KG];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    u4v a[KC][2];
+#pragma unroll
+                    for (int x = 0; x < KC; x++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const u2v lo = widen4(kf[c][x][2 * h]), hi = widen4(kf[c][x][2 * h + 1]);
+                            a[x][h] = (u4v){lo[0], lo[1], hi[0], hi[1]};
+                        }
+#pragma unroll
+                    for (int m = 0; m < MB; m++) {
+                        f4 acc = {};
+#pragma unroll
+                        for (int x = 0; x < KC; x++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) acc = product16(a[x][h], qf[m][x][h], acc);
+                        const float f = by[m] * ks;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[m][4 * c + e] = acc[e] * f;
+                    }
+                }
+                if (i + 1 < n) load_k(i + 1);
+                // Whether every row sees every key of the tile.
+                const bool all = key0 + KT <= w.hi && !__any(bad) && (key0 + KT <= n0 + 1 || key0 + KT <= w.prefix) &&
+                                 (p.window <= 0 || n1 - key0 < p.window || key0 + KT <= w.prefix);
+                if constexpr (MOD) {
+                    const auto cap_all = [&](auto fine) __attribute__((always_inline)) {
+#pragma unroll
+                        for (int m = 0; m < MB; m++)
+#pragma unroll
+                            for (int e = 0; e < KG; e++) s[m][e] = capped<decltype(fine)::value>(s[m][e], p.cap);
+                    };
+                    if (p.cap >= HIGH_CAP) cap_all(std::true_type{});
+                    else if (p.cap > 0.f) cap_all(std::false_type{});
+#pragma unroll
+                    for (int m = 0; m < MB; m++)
+#pragma unroll
+                        for (int e = 0; e < KG; e++) s[m][e] = __builtin_fmaf(-slope[m], fabsf((float)(pos[m] - (key0 + KG * g + e))), s[m][e]);
+                }
+                u32 see[MB];
+#pragma unroll
+                for (int m = 0; m < MB; m++) see[m] = 0xffffu;
+                if (!all) {
+#pragma unroll
+                    for (int m = 0; m < MB; m++) {
+                        see[m] = 0;
+#pragma unroll
+                        for (int e = 0; e < KG; e++) {
+                            const int key = key0 + KG * g + e;
+                            const bool ok = key < w.hi && !bad && ((key <= pos[m] && (p.window <= 0 || pos[m] - key < p.window)) || key < pre[m]);
+                            if (!ok) s[m][e] = -__builtin_inff();
+                            see[m] |= ok ? 1u << e : 0;
+                        }
+                    }
+                }
+                // Softmax.
+                u4v pf[MB][2];
+                const bool finite = vs <= FLT_TOP;
+#pragma unroll
+                for (int m = 0; m < MB; m++) {
+                    float mx = s[m][0];
+#pragma unroll
+                    for (int e = 1; e < KG; e++) mx = fmaxf(mx, s[m][e]);
+                    mx = rows_max(mx);
+                    const float mine = see[m] && finite ? vs : 0.f, vx = rows_max(mine);
+                    const bool move = mx > m_[m] + 8.f || (m_[m] == -__builtin_inff() && mx > m_[m]), grow = vx > vm[m];
+                    if (__any(move || grow)) {
+                        const float a = move ? __builtin_amdgcn_exp2f(m_[m] - mx) : 1.f, b = grow ? vm[m] / vx : 1.f;
+                        m_[m] = move ? mx : m_[m];
+                        vm[m] = grow ? vx : vm[m];
+                        l_[m] *= a;
+#pragma unroll
+                        for (int j = 0; j < VC; j++) o[m][j] *= a * b;
+                    }
+                    if (see[m] && !finite) l_[m] = __builtin_nanf("");
+                    const float base = m_[m] == -__builtin_inff() ? 0.f : m_[m], f = mine * (128.f / vm[m]);
+                    float pw[KG];
+#pragma unroll
+                    for (int e = 0; e < KG; e++) pw[e] = __builtin_amdgcn_exp2f(s[m][e] - base);
+#pragma unroll
+                    for (int e = 0; e < KG; e++) l_[m] += pw[e];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        h8 x;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[e] = (half_t)(pw[8 * h + e] * f);
+                        pf[m][h] = __builtin_bit_cast(u4v, x);
+                    }
+                }
+                // O^T += V^T P^T.
+#pragma unroll
+                for (int j = 0; j < VC; j++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        u4v a;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            u32 v0, v1;
+                            if constexpr (VC == 8) v0 = vf[8 * h + 2 * e][j >> 2], v1 = vf[8 * h + 2 * e + 1][j >> 2];
+                            else v0 = vf[8 * h + 2 * e], v1 = vf[8 * h + 2 * e + 1];
+                            a[e] = widen_pair(v0, v1, j & 3);
+                        }
+#pragma unroll
+                        for (int m = 0; m < MB; m++) o[m][j] = product16(a, pf[m][h], o[m][j]);
+                    }
+                if (i + 1 < n) {
+                    load_v(i + 1);
+                    if (i + 2 < n) fetch_ids(i + 2);
+                }
+            }
+        }
+
+        // The four waves' results meet in LDS, 16 rows at a time: thread (row t / 16, dims from t % 16 on) adds them.
+#pragma unroll
+        for (int m = 0; m < MB; m++) {
+            const float l = rows_sum(l_[m]), unit = vm[m] * (1.f / 128.f);
+            __syncthreads();
+            if (g == 0) {
+                ml[0][wave][r] = m_[m];
+                ml[1][wave][r] = l;
+            }
+            float* dst = (float*)smem + (wave * 16 + r) * OP;
+#pragma unroll
+            for (int i = 0; i < 4; i++)  // dims VC (4 g + i) + j
+#pragma unroll
+                for (int j = 0; j < VC; j += 4)
+                    *(f4*)(dst + VC * (4 * g + i) + j) = (f4){o[m][j][i], o[m][j + 1][i], o[m][j + 2][i], o[m][j + 3][i]} * unit;
+            __syncthreads();
+            const int row = t >> 4, c = (t & 15) * (D / 16);
+            float top = ml[0][0][row];
+#pragma unroll
+            for (int x = 1; x < 4; x++) top = fmaxf(top, ml[0][x][row]);
+            float sum = 0.f, y[D / 16];
+#pragma unroll
+            for (int e = 0; e < D / 16; e++) y[e] = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const float a = ml[0][x][row] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ml[0][x][row] - top);
+                sum = __builtin_fmaf(ml[1][x][row], a, sum);
+                const float* src = (const float*)smem + (x * 16 + row) * OP + c;
+#pragma unroll
+                for (int e = 0; e < D / 16; e += 4) {
+                    const f4 z = *(const f4*)(src + e);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) y[e + k] = __builtin_fmaf(z[k], a, y[e + k]);
+                }
+            }
+            const int tr = 16 * m + row;
+            if (whole) {
+                if (w.r0 + tr <= w.r1) {
+                    const int token = div_by(w.r0 + tr, p.G), head = run.kvh * (int)p.G.d + w.r0 + tr - token * (int)p.G.d;
+                    T* out = (T*)p.o + (long)(w.first + token) * p.sot + head * p.soh + c;
+                    store_row<T, D>(out, y, sum);
+                }
+            } else {
+                float* part = partial<MT, D>(p, block, begins);
+#pragma unroll
+                for (int e = 0; e < D / 16; e += 4) *(f4*)(part + tr * D + c + e) = (f4){y[e], y[e + 1], y[e + 2], y[e + 3]};
+                if (c == 0) {
+                    part[MT * D + tr] = top;
+                    part[MT * D + MT + tr] = sum;
+                }
+            }
+        }
+        __syncthreads();
+        if (begins && !last_part) {
+            cut.more = (int)((w.units - run.count + run.quota - 1) / run.quota);
+            cut.kvh = run.kvh;
+            cut.first = w.first;
+            cut.rows = w.rows;
+            cut.r0 = w.r0;
+        }
+        run.count -= min(w.units - run.unit, run.count);
+        run.unit = 0;
+        if (run.count > 0) next_tile<MT>(p, run);
+    }
+    if (t == 0) ((Cut*)p.ws)[block] = cut;
+}
+
+template <class T, int D, int MT>
+__global__ __launch_bounds__(256) void merge8_kernel(Attn8Args p) { merge_parts<T, D, MT>(p); }
+
+// ------------------------------------------------------------------------------------------------ launches
+
+struct Plan8 {
+    int mt, grid;
+    size_t workspace;
+};
+static int make_plan8(long T, long B, long H, long Hkv, long D, int type, Plan8* plan) {
+    if (T <= 0 || B <= 0 || B > MAX_SEQUENCES || Hkv <= 0 || H <= 0 || H % Hkv || (D != 64 && D != 128) || type < RDA_FP16 || type > RDA_BF16) return RDA_ERR_INVALID;
+    if (T * (H / Hkv) >= 1L << 31) return RDA_ERR_INVALID;
+    const long rows = T * (H / Hkv) / B;
+    plan->mt = rows <= 16 ? 16 : 32;
+    plan->grid = 512;
+    if ((T * (H / Hkv) / plan->mt + 1) * B >= 1L << 31) return RDA_ERR_INVALID;
+    plan->workspace = (size_t)plan->grid * sizeof(Cut) + (size_t)plan->grid * 2 * plan->mt * (D + 2) * 4;
+    return 0;
+}
+
+template <class T, int D, int MB>
+static int launch_rows8(const Attn8Args& a, void* stream) {
+    constexpr int OP = D + 4;
+    const size_t o = 4 * 16 * OP * 4, sums = (size_t)(a.B + 1) * 4, lds = o > sums ? o : sums;
+    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.grid), dim3(256), lds, (hipStream_t)stream, a); };
+    a.cap > 0.f || a.slopes ? launch(rows8_kernel<T, D, MB, true>) : launch(rows8_kernel<T, D, MB, false>);
+    if (const hipError_t e = hipGetLastError()) return (int)e;
+    hipLaunchKernelGGL((merge8_kernel<T, D, 16 * MB>), dim3(a.grid, 4 * MB), dim3(256), 0, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+template <class X, class Q, int PS>
+static int launch_append8(const Append8Args& a, dim3 grid, size_t lds, void* stream) {
+    static std::atomic<size_t> done[RDA_MAX_DEVICES];
+    if (lds > 32768)  // angles of 64 tokens and more than 64 pairs, or of 32 and 128: up to 64 KB
+        if (const int e = ensure_dynamic_lds((const void*)append8_kernel<X, Q, PS>, lds, done)) return e;
+    hipLaunchKernelGGL((append8_kernel<X, Q, PS>), grid, dim3(256), lds, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+// Codes are read and written 8 and 16 at a time.
+static bool code_rows(const void* p, const long* strides) {
+    for (int i = 0; i < 3; i++)
+        if (strides[i] % 16) return false;
+    return ((uintptr_t)p & 15) == 0;
+}
+static bool cache8_ok(long P, long S, long N, long block) {
+    return N > 0 && P > 0 && P < 1L << 31 && S > 0 && (block == 16 || block == 32 || block == 64) && S % block == 0 && N <= MAX_KEYS8 / S;
+}
+
+extern "C" {
+
+int rda_paged_append_i8(const void* q, const void* k, const void* v, void* q_out, void* k_codes, void* v_codes, float* k_scales, float* v_scales, const int* table,
+                        const int* starts, const int* lengths, const double* turns, float factor, int interleaved, const void* q_weight, const void* k_weight,
+                        int weight_type, float eps, int type, int q_type, const long* dims, void* stream) {
+    const long T = dims[0], H = dims[1], Hkv = dims[2], D = dims[3], R = dims[4], B = dims[5], N = dims[6], P = dims[8], S = dims[9], block = dims[10];
+    if (T <= 0 || T > MAX_ROWS || H < 0 || Hkv <= 0 || H + 2 * Hkv > 65535 || !rotary_ok(turns, D, R) || B <= 0 || B > MAX_SEQUENCES || !cache8_ok(P, S, N, block))
+        return RDA_ERR_INVALID;
+    if (type < RDA_FP16 || type > RDA_FP32 || q_type < RDA_FP16 || q_type > RDA_BF16 || weight_type < RDA_FP16 || weight_type > RDA_FP32) return RDA_ERR_INVALID;
+    if (!vector_rows(k, dims + 13, 2, type) || !vector_rows(v, dims + 15, 2, type) || !code_rows(k_codes, dims + 19) || !code_rows(v_codes, dims + 22)) return RDA_ERR_INVALID;
+    if (H && (!vector_rows(q, dims + 11, 2, type) || !vector_rows(q_out, dims + 17, 2, q_type))) return RDA_ERR_INVALID;
+    if (!vector_rows(q_weight, dims, 0, type) || !vector_rows(k_weight, dims, 0, type) || (H && !q_weight != !k_weight)) return RDA_ERR_INVALID;
+    Append8Args a = {{turns, (int)D, (int)R, interleaved & 1, factor, 1.f}, q, k, v, q_out, (signed char*)k_codes, (signed char*)v_codes, k_scales, v_scales, table, starts,
+                     lengths, q_weight, k_weight, weight_type, eps, (int)T, (int)H, (int)Hkv, (int)B, (int)N, (int)P, (int)block, 0, make_div((int)S), dims[7],
+                     dims[11], dims[12], dims[13], dims[14], dims[15], dims[16], dims[17], dims[18], dims[19], dims[20], dims[21], dims[22], dims[23], dims[24],
+                     dims[25], dims[26], dims[27], dims[28], dims[29], dims[30]};
+    const long slots = T / block + 2 * B, heads = H + 2 * Hkv, together = 64 / block;
+    // Heads of a workgroup: as many as leave 2048 workgroups, so that angles are made for more than one head at a time.
+    long slice = (heads * slots / 2048 + together - 1) / together * together;
+    if (slice < together) slice = together;
+    if (slice > heads) slice = (heads + together - 1) / together * together;
+    a.slice = (int)slice;
+    const size_t lds = (size_t)block * (R / 2) * 8;
+    const dim3 grid((unsigned)slots, (unsigned)((heads + slice - 1) / slice));
+    const int rows = 64 / (int)(D / 16);  // of a pass of a wave
+    const auto from = [&](auto x) {
+        using X = decltype(x);
+        const auto to = [&](auto y) {
+            using Q = decltype(y);
+            return rows >= 16 ? launch_append8<X, Q, 1>(a, grid, lds, stream) : rows >= 8 ? launch_append8<X, Q, 2>(a, grid, lds, stream) : launch_append8<X, Q, 4>(a, grid, lds, stream);
+        };
+        return q_type == RDA_FP16 ? to(half_t{}) : to(bf16_t{});
+    };
+    return type == RDA_FP16 ? from(half_t{}) : type == RDA_BF16 ? from(bf16_t{}) : from(float{});
+}
+
+int rda_paged_read_i8(const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, const int* table, const int* starts, const int* lengths,
+                      void* k_out, void* v_out, int type, const long* dims, void* stream) {
+    const long T = dims[0], Hkv = dims[1], D = dims[2], B = dims[3], N = dims[4], P = dims[6], S = dims[7], block = dims[8];
+    if (T <= 0 || T > MAX_ROWS || Hkv <= 0 || Hkv > 65535 || D <= 0 || D % 16 || D > 2 * MAX_PAIRS || B <= 0 || B > MAX_SEQUENCES || !cache8_ok(P, S, N, block)) return RDA_ERR_INVALID;
+    if (type < RDA_FP16 || type > RDA_FP32 || !code_rows(k_codes, dims + 9) || !code_rows(v_codes, dims + 12) || !vector_rows(k_out, dims, 0, type) ||
+        !vector_rows(v_out, dims, 0, type))
+        return RDA_ERR_INVALID;
+    const Read8Args a = {(const signed char*)k_codes, (const signed char*)v_codes, k_scales, v_scales, table, starts, lengths, k_out, v_out,
+                         (int)T, (int)Hkv, (int)D, (int)B, (int)N, (int)P, block == 16 ? 4 : block == 32 ? 5 : 6, make_div((int)S), dims[5],
+                         dims[9], dims[10], dims[11], dims[12], dims[13], dims[14], dims[15], dims[16], dims[17], dims[18], dims[19], dims[20]};
+    const auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((T + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
+        return (int)hipGetLastError();
+    };
+    return type == RDA_FP16 ? launch(read8_kernel<half_t>) : type == RDA_BF16 ? launch(read8_kernel<bf16_t>) : launch(read8_kernel<float>);
+}
+
+size_t rda_paged_attn_i8_workspace(long T, long B, long H, long Hkv, long D, int type) {
+    Plan8 plan;
+    return make_plan8(T, B, H, Hkv, D, type, &plan) ? 0 : plan.workspace;
+}
+
+int rda_paged_attn_i8(const void* q, void* out, const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, const int* table,
+                      const int* starts, const int* lengths, const int* prefix, const float* slopes, void* workspace, float scale, float softcap, int window, int fill,
+                      int type, const long* dims, void* stream) {
+    const long T = dims[0], H = dims[1], Hkv = dims[2], D = dims[3], B = dims[4], N = dims[5], P = dims[7], S = dims[8], block = dims[9];
+    Plan8 plan;
+    if (const int e = make_plan8(T, B, H, Hkv, D, type, &plan)) return e;
+    if (!cache8_ok(P, S, N, block) || window < 0 || !(softcap >= 0.f) || ((uintptr_t)workspace & 15)) return RDA_ERR_INVALID;
+    if (!vector_rows(q, dims + 10, 2, type) || !vector_rows(out, dims + 12, 2, type) || !code_rows(k_codes, dims + 14) || !code_rows(v_codes, dims + 17)) return RDA_ERR_INVALID;
+    // Units of a KV head in 32 bits, whatever the lengths.
+    if ((T * (H / Hkv) / plan.mt + B) * (N * S / 32 + 1 + ahead(plan.mt, false)) >= 1L << 32) return RDA_ERR_INVALID;
+    for (int i : {14, 15, 17, 18, 20, 21, 23, 24})
+        if (dims[i] < 0 || dims[i] >= 1L << 32) return RDA_ERR_INVALID;
+    Attn8Args a;
+    a.q = q; a.o = out; a.k = k_codes; a.v = v_codes;
+    a.ks = k_scales; a.vs = v_scales;
+    a.table = table; a.starts = starts; a.lengths = lengths; a.prefix = prefix;
+    a.slopes = slopes;
+    a.ws = (char*)workspace;
+    a.T = (int)T; a.B = (int)B; a.H = (int)H; a.Hkv = (int)Hkv; a.P = (int)P; a.N = (int)N; a.capacity = (int)(N * S);
+    a.S = make_div((int)S); a.G = make_div((int)(H / Hkv));
+    a.shift = block == 16 ? 4 : block == 32 ? 5 : 6;
+    a.pitch = dims[6];
+    a.sqt = dims[10]; a.sqh = dims[11]; a.sot = dims[12]; a.soh = dims[13];
+    a.kpp = (u32)dims[14]; a.kpr = (u32)dims[15]; a.kph = dims[16]; a.vpp = (u32)dims[17]; a.vpr = (u32)dims[18]; a.vph = dims[19];
+    a.ksp = (u32)dims[20]; a.ksb = (u32)dims[21]; a.ksh = dims[22]; a.vsp = (u32)dims[23]; a.vsb = (u32)dims[24]; a.vsh = dims[25];
+    a.scale = softcap > 0.f ? scale / softcap * 2.f * LOG2E : scale * LOG2E;
+    a.cap = softcap * LOG2E;
+    // Normal, positive and finite: masked scores are -inf before they meet the scale.
+    if (!(a.scale >= 1.2e-38f && a.scale <= 3e38f && a.cap <= 3e38f)) return RDA_ERR_INVALID;
+    a.window = window;
+    // No more workgroups than units there can be: a short table of few sequences needs none that finds no work.
+    const long units = (T * (H / Hkv) / plan.mt + B) * ((N * S + 255) / 256 + ahead(plan.mt, false)) * Hkv;
+    a.grid = (int)(units < plan.grid ? units : plan.grid);
+    a.runs = make_div(a.grid);
+    a.fill = fill;
+    const auto heads = [&](auto x) {
+        using X = decltype(x);
+        if (plan.mt == 16) return D == 64 ? launch_rows8<X, 64, 1>(a, stream) : launch_rows8<X, 128, 1>(a, stream);
+        return D == 64 ? launch_rows8<X, 64, 2>(a, stream) : launch_rows8<X, 128, 2>(a, stream);
+    };
+    return type == RDA_FP16 ? heads(half_t{}) : heads(bf16_t{});
+}
+
+}  // extern "C"

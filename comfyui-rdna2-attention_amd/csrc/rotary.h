@@ -112,3 +112,36 @@ __device__ __forceinline__ int sequence_of(const int* starts, int B, int t, int 
 static bool rotary_ok(const double* turns, long D, long R) {
     return D > 0 && D % 16 == 0 && D <= 2 * MAX_PAIRS && R >= 0 && R % 16 == 0 && R <= D && (R == 0 || turns);
 }
+
+// ------------------------------------------------------------------------------------------------ norms of heads
+
+// Eight weights of a head's norm as fp32, from any of the three types.
+__device__ __forceinline__ f8 weights8(const void* w, int type, int at) {
+    return type == RDA_FP16 ? load8((const half_t*)w + at) : type == RDA_BF16 ? load8((const bf16_t*)w + at) : load8((const float*)w + at);
+}
+// The sum over the `per` lanes that hold a head (lane / per is the head's place): by lane swaps where per is a power of two.
+__device__ __forceinline__ float head_sum(float x, int per, int lane) {
+    if ((per & (per - 1)) == 0) {
+        if (per >= 2) x += dpp<0xB1>(x);
+        if (per >= 4) x += dpp<0x4E>(x);
+        if (per >= 8) x += dpp<0x141>(x);
+        if (per >= 16) x += dpp<0x140>(x);
+        return x;
+    }
+    const int base = lane - lane % per;
+    float s = 0.f;
+    for (int i = 0; i < per; i++) s += __shfl(x, base + i);
+    return s;
+}
+__device__ __forceinline__ float dot16(const f8& a, const f8& b, const f8& c, const f8& d) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) s = __builtin_fmaf(a[i], b[i], s);
+#pragma unroll
+    for (int i = 0; i < 8; i++) s = __builtin_fmaf(c[i], d[i], s);
+    return s;
+}
+// 1 / sqrt(mean of the head's squares + eps), in 32 bits.
+__device__ __forceinline__ float inverse_rms(const f8& lo, const f8& hi, int D, float eps, int per, int lane) {
+    return 1.f / sqrtf(head_sum(dot16(lo, lo, hi, hi), per, lane) * (1.f / (float)D) + eps);
+}

@@ -1,7 +1,7 @@
 """Rotary positions for text models on MI355X: pairs of a head's values turned by angles that grow with the token's position, in the
 half and the interleaved layout, over all or part of the head, with the frequency scalings of long contexts. The RoPE of a Krea 2
 block, whose matrices the model makes (rms_norm.rms_norm_rope), is another operator; paged_kv.append turns queries and keys on the
-way into the cache with the same arithmetic as `rotate`.
+way into the cache with the same arithmetic as `rotate`. `norm_rotate` norms queries and keys head by head first, in the same pass.
 """
 import math
 
@@ -21,7 +21,7 @@ kernels = None
 def get_kernels():
     global kernels
     if kernels is None:
-        kernels = Kernels("rotary", ("rotate_positions",))
+        kernels = Kernels("rotary", ("rotate_positions", "norm_rotate", "norm_rotate_back", "norm_rotate_back_workspace"))
     return kernels
 
 
@@ -209,3 +209,122 @@ def _check_rotate(x, positions, rotary, out, key):
     sx, so = x.stride(), out.stride()
     values = [B, L, x.shape[-2], x.shape[-1], rotary.dim, *(sx[:3] if x.dim() == 4 else (0, *sx[:2])), *(so[:3] if x.dim() == 4 else (0, *so[:2]))]
     return x, _rotate_sizes.keep(key, values) if ready else _lib.long_array(values)
+
+
+class HeadNorm:
+    """RMS norms of a layer's query and key heads: q and k are their weights, (D,) each, contiguous, of one type (fp16, bf16 or fp32), kept as they are -- a
+    training step's updates of them are seen --, eps what is added to a head's mean square."""
+
+    def __init__(self, q, k, eps=1e-6):
+        if q.dim() != 1 or q.shape != k.shape or q.dtype not in TYPES or k.dtype != q.dtype or q.device != k.device or q.numel() == 0 or q.numel() % 16:
+            raise ValueError("HeadNorm takes weights q and k as (D,) of one type (fp16, bf16 or fp32) on one device, D a multiple of 16")
+        if not (rows_ready(q) and rows_ready(k)):
+            raise ValueError("HeadNorm takes contiguous weights on 16-byte boundaries")
+        if not 0.0 <= eps < 1e30:
+            raise ValueError("HeadNorm takes an eps that is not negative")
+        self.q, self.k, self.eps = q, k, float(eps)
+
+
+_norm_sizes, _norm_back_sizes, _norm_workspaces = Sizes(), Sizes(), {}
+
+
+class _NormTurn(torch.autograd.Function):
+    """norm_rotate where gradients are recorded; the gradient has none itself."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, rotary, eps):
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions, rotary.turns)
+        ctx.rotary, ctx.eps = rotary, eps
+        return _norm_rotate(q, k, positions, rotary, q_weight, k_weight, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, q_grad, k_grad):
+        q, k, q_weight, k_weight, positions, _ = ctx.saved_tensors
+        return (*_norm_rotate_back(q, k, q_grad, k_grad, positions, ctx.rotary, q_weight, k_weight, ctx.eps), None, None, None)
+
+
+def norm_rotate(q, k, positions, rotary, norm):
+    """q (tokens, heads, D) and k (tokens, KV heads, D), or both with a batch dimension before them as rotate takes, normed head by head and turned by
+    `positions`, in one launch: (q, k), new contiguous tensors of their type. A head x becomes the turn of w x / sqrt(mean(x^2) + norm.eps), w norm.q or
+    norm.k, in 32 bits, rounded once. Any strides with a contiguous last dimension. Gradients of q, k and the weights are carried where they are
+    recorded, those of the weights summed in 32 bits and rounded once; the same inputs give the same bits."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or norm.q.requires_grad or norm.k.requires_grad):
+        return _NormTurn.apply(q, k, norm.q, norm.k, positions, rotary, norm.eps)
+    return _norm_rotate(q, k, positions, rotary, norm.q, norm.k, norm.eps)
+
+
+def _norm_rotate(q, k, positions, rotary, q_weight, k_weight, eps):
+    q, k, positions = _aligned(q), _aligned(k), positions.contiguous()
+    key = (q.dtype, q.shape, q.stride(), k.dtype, k.shape, k.stride(), positions.dtype, positions.shape, rotary.dim, q_weight.shape)
+    dims = _norm_sizes.get(key)
+    if dims is None:
+        q, k, dims = _check_norm_rotate(q, k, positions, rotary, q_weight, key)
+    same_device("norm_rotate", q, k, positions, q_weight, k_weight, rotary.turns)
+    q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(k, memory_format=torch.contiguous_format)
+    if positions.numel() == 0:
+        return q_out, k_out
+    _lib.check(get_kernels().norm_rotate(q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), positions.data_ptr(), positions.dtype is torch.int64,
+                                         q_weight.data_ptr(), k_weight.data_ptr(), TYPES[q_weight.dtype], eps, rotary.turns.data_ptr(), rotary.factor,
+                                         rotary.interleaved, TYPES[q.dtype], dims, _lib.raw_stream()))
+    return q_out, k_out
+
+
+def _norm_rotate_back(q, k, q_grad, k_grad, positions, rotary, q_weight, k_weight, eps):
+    """The gradients of q, k and the weights."""
+    q, k, positions = vector_rows(q), vector_rows(k), positions.contiguous()
+    q_grad, k_grad = vector_rows(q_grad), vector_rows(k_grad)
+    q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(k, memory_format=torch.contiguous_format)
+    if positions.numel() == 0:
+        return q_out, k_out, torch.zeros_like(q_weight), torch.zeros_like(k_weight)
+    q_weight_out, k_weight_out = torch.empty_like(q_weight), torch.empty_like(k_weight)
+    same_device("norm_rotate's gradient", q, k, q_grad, k_grad, positions, q_weight, k_weight, rotary.turns)
+    key = (q.shape, q.stride(), k.shape, k.stride(), q_grad.stride(), k_grad.stride(), rotary.dim)
+    dims = _norm_back_sizes.get(key)
+    if dims is None:
+        dims = _norm_back_sizes.keep(key, _norm_dims(q, k, rotary) + [s for t in (q_grad, k_grad) for s in _strides(t)])
+    sizes = (positions.numel(), q.shape[-2], k.shape[-2], q.shape[-1])
+    kernels = get_kernels()
+    size = _norm_workspaces.get(sizes)
+    if size is None:
+        if len(_norm_workspaces) >= 4096:
+            _norm_workspaces.clear()
+        size = _norm_workspaces[sizes] = kernels.norm_rotate_back_workspace(*sizes)
+    workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    _lib.check(kernels.norm_rotate_back(q.data_ptr(), k.data_ptr(), q_grad.data_ptr(), k_grad.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
+                                        q_weight_out.data_ptr(), k_weight_out.data_ptr(), positions.data_ptr(), positions.dtype is torch.int64,
+                                        q_weight.data_ptr(), k_weight.data_ptr(), TYPES[q_weight.dtype], eps, rotary.turns.data_ptr(), rotary.factor,
+                                        rotary.interleaved, workspace.data_ptr(), TYPES[q.dtype], dims, _lib.raw_stream()))
+    return q_out, k_out, q_weight_out, k_weight_out
+
+
+def _aligned(t):
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
+
+
+def _strides(t):
+    return t.stride()[:3] if t.dim() == 4 else (0, *t.stride()[:2])
+
+
+def _norm_dims(q, k, rotary):
+    B, L = (1, q.shape[0]) if q.dim() == 3 else q.shape[:2]
+    return [B, L, q.shape[-2], k.shape[-2], q.shape[-1], rotary.dim, *_strides(q), *_strides(k)]
+
+
+def _check_norm_rotate(q, k, positions, rotary, weight, key):
+    """(q and k, copied where the kernel cannot address them; the size arguments) of a norm_rotate call, or ValueError."""
+    D = weight.shape[0]
+    if q.dim() not in (3, 4) or q.dtype not in TYPES or q.shape[-1] != D or not 0 < q.shape[-2] <= 65535 or not rotary.dim <= D <= MAX_HEAD:
+        raise ValueError(f"norm_rotate takes q as (tokens, heads, D) or (batch, length, heads, D) in fp16, bf16 or fp32, D the weights' {D}, from {rotary.dim} "
+                         f"to {MAX_HEAD}, 1 to 65535 heads, not {tuple(q.shape)} {q.dtype}")
+    if k.dtype != q.dtype or k.shape[:-2] != q.shape[:-2] or k.dim() != q.dim() or k.shape[-1] != D or not 0 < k.shape[-2] <= 65535:
+        raise ValueError(f"norm_rotate takes k of q's type, tokens and D, not {tuple(k.shape)} {k.dtype}")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != q.shape[:-2]:
+        raise ValueError(f"norm_rotate takes int32 or int64 positions of shape {tuple(q.shape[:-2])}, not {tuple(positions.shape)} {positions.dtype}")
+    if positions.numel() > MAX_TOKENS:
+        raise ValueError(f"norm_rotate takes at most {MAX_TOKENS} tokens")
+    ready = q.numel() == 0 or (rows_ready(q) and rows_ready(k))
+    if not ready:
+        q, k = vector_rows(q), vector_rows(k)
+    values = _norm_dims(q, k, rotary)
+    return q, k, _norm_sizes.keep(key, values) if ready else _lib.long_array(values)

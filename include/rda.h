@@ -229,6 +229,48 @@ int rda_paged_attn(const void* q, void* out, const void* k_pages, const void* v_
                    const int* prefix, const float* slopes, void* workspace, float scale, float softcap, int window, int fill, int type,
                    const long* dims, void* stream);
 
+/* ------------------------------------------------------------------ norms of heads ----- */
+/* RMS norms of query and key heads with their turn by position: q, k (B, L, H or Hkv, D) of `type`, each head of values x to R(n) (w x r),
+ * r = (mean of x^2 + eps)^-1/2, w the tensor's D weights of weight_type, R(n) the turn of rda_rotate_positions (R > 0), rounded once.
+ * q_out, k_out are contiguous and overlap no input. dims: B, L, H, Hkv, D, R, strides (b, l, h) of q, of k. */
+int rda_norm_rotate(const void* q, const void* k, void* q_out, void* k_out, const void* positions, int wide, const void* q_weight, const void* k_weight,
+                    int weight_type, float eps, const double* turns, float factor, int interleaved, int type, const long* dims, void* stream);
+
+/* Its gradients: q_out, k_out (contiguous) those of q and k for the gradients q_grad, k_grad of its outputs, q_weight_out, k_weight_out (weight_type)
+ * those of the weights, summed over all tokens and heads in 32 bits in an order that depends on the sizes alone. dims: as above, then strides (b, l, h) of
+ * q_grad, of k_grad. workspace: rda_norm_rotate_back_workspace bytes of B x L tokens; calls that overlap take one each. */
+size_t rda_norm_rotate_back_workspace(long tokens, long H, long Hkv, long D);
+int rda_norm_rotate_back(const void* q, const void* k, const void* q_grad, const void* k_grad, void* q_out, void* k_out, void* q_weight_out,
+                         void* k_weight_out, const void* positions, int wide, const void* q_weight, const void* k_weight, int weight_type, float eps,
+                         const double* turns, float factor, int interleaved, void* workspace, int type, const long* dims, void* stream);
+
+/* ------------------------------------------------------------------ quantized paged cache */
+/* A paged cache of int8 codes (P, S, Hkv, D) with fp32 scales (P, S / block, Hkv): a value is code x scale, the scale one of `block` consecutive tokens
+ * (16, 32 or 64; S a multiple) of a KV head, for keys and values apart. Scales are not negative; one that is not finite stands for a block of NaN. Codes'
+ * strides are multiples of 16. Batches as of rda_paged_append, of at most 8192 sequences. */
+
+/* Appends as rda_paged_append, k and q normed before their turn where weights are given (as rda_norm_rotate; NULL: not), q_out of q_type (0 or 1). A
+ * block's scale is max(largest magnitude of its values here / 127, 1e-30), and at least the one that it has where its first token is not among the new
+ * ones; codes are the nearest whole numbers to value / scale, those of older tokens to code x old / new scale. Values that are not all finite make the scale
+ * NaN. Blocks that two sequences of a call write hold either's. dims: T, H, Hkv, D, R, B, N, table pitch, P, S, block, strides (t, h) of q, k, v, q_out,
+ * (page, row, head) of k_codes, v_codes, (page, block, head) of k_scales, v_scales. */
+int rda_paged_append_i8(const void* q, const void* k, const void* v, void* q_out, void* k_codes, void* v_codes, float* k_scales, float* v_scales,
+                        const int* table, const int* starts, const int* lengths, const double* turns, float factor, int interleaved,
+                        const void* q_weight, const void* k_weight, int weight_type, float eps, int type, int q_type, const long* dims, void* stream);
+
+/* Reads the rows of a batch back: k_out, v_out (T, Hkv, D) of `type`, contiguous; row t of sequence b is what rda_paged_append_i8 would write
+ * there. Rows of no sequence, and of positions or pages that do not exist, are 0. dims: T, Hkv, D, B, N, table pitch, P, S, block, strides of codes and scales as
+ * above. */
+int rda_paged_read_i8(const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, const int* table, const int* starts,
+                      const int* lengths, void* k_out, void* v_out, int type, const long* dims, void* stream);
+
+/* Attention as rda_paged_attn over a quantized cache, q and out of `type` (0 or 1). dims: T, H, Hkv, D, B, N, table pitch, P, S, block, strides (t, h) of q, of out,
+ * and of codes and scales as above. */
+size_t rda_paged_attn_i8_workspace(long T, long B, long H, long Hkv, long D, int type);
+int rda_paged_attn_i8(const void* q, void* out, const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, const int* table,
+                      const int* starts, const int* lengths, const int* prefix, const float* slopes, void* workspace, float scale, float softcap, int window,
+                      int fill, int type, const long* dims, void* stream);
+
 /* ------------------------------------------------------------------ calibration -------- */
 /* Measurement only, no counterpart in the reference: `blocks` workgroups of four waves each issue `iters` rounds of
  * 8 independent MFMAs (int8 = 1: v_mfma_i32_32x32x32_i8, 65536 ops each; int8 = 0: v_mfma_f32_32x32x16_f16, 32768
