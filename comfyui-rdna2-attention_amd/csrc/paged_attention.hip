@@ -453,47 +453,6 @@ __global__ __launch_bounds__(256, MB == 1 && D == 64 ? 3 : 2) void rows_kernel(P
 // Capped scores take three transcendentals each where plain ones take one: 2 x 4096 tokens of 16 heads of 128 in a window of 2048, 103 GFLOP, 190 us:
 // at two workgroups a CU vector work and products fill ~80% of the cycles (217 us with the whole capped score made before the softmax's product).
 // With D = 64 a score's exponential stands beside half the products. Tiles that are masked cost ~2.4 full ones, a tile's start ~7 us of latency.
-template <int D>
-struct TilesLds {
-    static constexpr int ROW = 2 * D, TILE = 32 * ROW, V = 3 * TILE;  // K stages, V stages
-    // find_run's tile sums before them and the rows turned around after them (32 x 256 bytes a wave) lie in the same place; then find_run's words.
-    static constexpr int SHARED = 6 * TILE > 33024 ? 6 * TILE : 33024;
-    static_assert(SHARED >= 4 * (MAX_SEQUENCES + 1) && SHARED >= 4 * 32 * 256 && SHARED % 256 == 0);
-    static constexpr int BYTES = SHARED + (256 + 16) * 4;
-};
-typedef __fp16 tr_t __attribute__((__vector_size__(4 * sizeof(__fp16))));
-typedef __attribute__((address_space(3))) tr_t lds_tr_t;
-typedef __attribute__((address_space(3))) u4v lds_u4v_t;
-__device__ __forceinline__ u4v lds_u4(u32 addr) { return *(const lds_u4v_t*)(size_t)addr; }
-__device__ __forceinline__ u2v lds_tr(u32 addr) { return __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr_t*)(size_t)addr)); }
-__device__ __forceinline__ f2 both_halves(float x) {  // x of the lane's row from lanes 0-31, and from lanes 32-63
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return (f2){__uint_as_float(r[0]), __uint_as_float(r[1])};
-}
-template <class T>
-__device__ __forceinline__ f16v product32(const u4v& a, const u4v& b, const f16v& c) {
-    if constexpr (std::is_same<T, half_t>::value) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
-}
-// Two values rounded to T as one word, and the sum of a word's two values added to l.
-template <class T>
-__device__ __forceinline__ u32 pair_of(float a, float b) {
-    if constexpr (std::is_same<T, half_t>::value) return __builtin_bit_cast(u32, __builtin_convertvector((f2){a, b}, h2));
-    else return __builtin_bit_cast(u32, __builtin_convertvector((f2){a, b}, b2));
-}
-template <class T>
-__device__ __forceinline__ float add_pair(u32 w, float l) {
-    if constexpr (std::is_same<T, half_t>::value) return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), (h2){(_Float16)1.f, (_Float16)1.f}, l, false);
-    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), (b2){(bf16_t)1.f, (bf16_t)1.f}, l, false);
-}
-
-// The lane's number, read again where a rare branch needs it, so that the tile loop holds no registers for it.
-__device__ __forceinline__ int lane_again() {
-    int x;
-    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
-    return x;
-}
-
 template <class T, int D, bool MOD, bool RUNS>
 __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(PagedArgs p) {
     constexpr int MT = 128, UK = 32, AHEAD = ahead(MT, MOD), ROW = 2 * D, KS = D / 16, DT = D / 32;  // KS: products of a score block; DT: of a 16-key step with V

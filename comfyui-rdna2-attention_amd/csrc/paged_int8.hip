@@ -580,6 +580,533 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
     if (t == 0) ((Cut*)p.ws)[block] = cut;
 }
 
+// Tiles of 128 rows, as tiles_kernel of 16-bit caches (paged_attention.hip), whose tile layouts, step order and masks these are: 32 rows to each of four waves
+// that share 32-key tiles of K and V in LDS, there as fp16 codes. What differs:
+//
+// * A tile's codes come through registers: 16 (D = 64: 8) a thread of K and of V, loaded a step ahead, widened once for all four waves and written to the
+//   stage two tiles ahead. A wave's eight rows of a tile lie in one page.
+// * Keys 0-15 and 16-31 of a tile have a scale each, and are the two halves in which P is made: the scale of K (times the row's factor) is the factor of the
+//   exponent's product anyway, and the scale of V, relative to the row's vm, goes into the exponent as its logarithm. l then gets a half's sum of
+//   rounded P times what takes that out again. So full steps do nothing more per score than those of a 16-bit cache.
+// * Where a scale of V is above the row's vm, or below it by more than 2^8, or is not finite, the step is not a full one: the plain steps sum P before it
+//   is scaled, and move vm (to twice the scale: O is then seldom rescaled).
+#define TILES8_WGS(D, MOD) 2
+#define LIFT_TILES 9.f        // P stands 2^9 vs / vm above 2^(x - m), of which at most 2^2 are in a plain step
+#define MOST_TILES 32768.f    // of a full step's sum of P in a lane, so that no P is above it
+#define LEAST_RATIO -8.f      // log2 of vs / vm
+
+template <int D>
+struct Tiles8Lds {
+    using L = TilesLds<D>;
+    static constexpr int SCALES = L::BYTES, BYTES = SCALES + 3 * 2 * 16;  // {K's scale, V's, log2 of V's, 1 / V's} of each stage's two groups
+};
+
+template <class T, int D, bool MOD>
+__global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Args p) {
+    constexpr int MT = 128, UK = 32, AHEAD = ahead(MT, MOD), ROW = 2 * D, KS = D / 16, DT = D / 32;
+    constexpr int CB = D / 8;  // codes of a thread
+    constexpr int CR = 1024 / ROW;  // rows of a store of the output
+    using L = TilesLds<D>;
+    typedef typename std::conditional<D == 128, u4v, u2v>::type raw_t;
+    typedef __attribute__((address_space(3))) f4 lds_f4_t;
+    extern __shared__ __attribute__((aligned(256))) char smem[];
+    const int lane = threadIdx.x & 63, g = lane >> 5, lq = lane & 31;
+    const int wave = uniform((int)(threadIdx.x >> 6));
+    const int block = work_block(p.grid);
+    Run run = find_run<MT, UK, AHEAD, 256>(p, (int*)smem, (u32*)(smem + L::SHARED), block);
+    int* flags = (int*)(smem + L::SHARED) + 256 + 8;  // a wave's: whether the cache lacks a page that it looked up
+    Cut cut = {};
+    const u32 smem_u = lds_addr(smem);
+
+    while (run.count > 0) {
+        const WorkTile w = uniform(make_tile<MT, UK, AHEAD>(p, run.b, run.j));
+        if (run.unit + run.count <= AHEAD) break;  // the next run's
+        const bool begins = run.unit == 0, last_part = run.unit + run.count >= w.units, whole = begins && last_part;
+        const int u0 = begins ? 0 : run.unit - AHEAD, u1 = min(w.units, run.unit + run.count) - AHEAD, n = w.hi > w.lo ? u1 - u0 : 0;
+        const int* table = p.table + run.b * p.pitch;
+        const signed char* kbase = uniform((const signed char*)p.k + run.kvh * p.kph);
+        const signed char* vbase = uniform((const signed char*)p.v + run.kvh * p.vph);
+        const float *ksbase = uniform(p.ks + run.kvh * p.ksh), *vsbase = uniform(p.vs + run.kvh * p.vsh);
+        const int key_first = w.lo + u0 * UK, last16 = (w.hi - 1) & ~15;
+        auto key_of = [&](int i) __attribute__((always_inline)) { return key_first + i * UK; };
+        const int wr0 = w.r0 + 32 * wave;  // the wave's first row
+        const bool active = wr0 <= w.r1;
+        const int n0 = uniform(w.p0 + div_by(min(wr0, w.r1), p.G)), n1 = uniform(w.p0 + div_by(min(wr0 + 31, w.r1), p.G));
+
+        // Copies: the wave's rows 8 wave .. + 7 of a tile, eight lanes to a row. Rows behind the sequence's end in its last 16 keys are read as they are, later
+        // ones as those 16.
+        raw_t raw_k, raw_v;
+        float raw_ks, raw_vs;
+        int id = 0;  // the wave's table entry of the tile to be loaded next
+        const unsigned long long k_lane = (unsigned long long)(lane >> 3) * p.kpr + (lane & 7) * CB, v_lane = (unsigned long long)(lane >> 3) * p.vpr + (lane & 7) * CB;
+        auto group_of = [&](int i) __attribute__((always_inline)) { return min(key_of(i) + 16 * (wave >> 1), last16); };
+        auto fetch = [&](int i) __attribute__((always_inline)) { id = table[div_by(group_of(i), p.S)]; };
+        auto load = [&](int i) __attribute__((always_inline)) {
+            const int key = group_of(i), row = key - div_by(key, p.S) * (int)p.S.d;
+            const u32 at = (u32)uniform(id), page = at < (u32)p.P ? at : 0;
+            raw_k = *(const raw_t*)(kbase + row_at(page, p.kpp, (u32)row + 8 * (wave & 1), p.kpr) + k_lane);
+            raw_v = *(const raw_t*)(vbase + row_at(page, p.vpp, (u32)row + 8 * (wave & 1), p.vpr) + v_lane);
+            raw_ks = ksbase[row_at(page, p.ksp, (u32)row >> p.shift, p.ksb)];
+            raw_vs = vsbase[row_at(page, p.vsp, (u32)row >> p.shift, p.vsb)];
+        };
+        const int my_row = 8 * wave + (lane >> 3);
+        auto put = [&](u32 st) __attribute__((always_inline)) {
+            const int k_swizzle = D == 128 ? my_row & 15 : my_row >> 1 & 7, v_swizzle = D == 128 ? (my_row & 3) << 2 : (my_row >> 1 & 1) << 2;
+            char *kd = smem + st + my_row * ROW, *vd = kd + L::V;
+#pragma unroll
+            for (int c = 0; c < CB / 8; c++) {
+                const int chunk = (lane & 7) * (CB / 8) + c;
+                const u2v k0 = widen4(raw_k[2 * c]), k1 = widen4(raw_k[2 * c + 1]), v0 = widen4(raw_v[2 * c]), v1 = widen4(raw_v[2 * c + 1]);
+                *(u4v*)(kd + ((chunk ^ k_swizzle) << 4)) = (u4v){k0[0], k0[1], k1[0], k1[1]};
+                *(u4v*)(vd + ((chunk ^ v_swizzle) << 4)) = (u4v){v0[0], v0[1], v1[0], v1[1]};
+            }
+            const float ks = raw_ks <= FLT_TOP ? raw_ks : __builtin_nanf("");
+            *(f4*)(smem + Tiles8Lds<D>::SCALES + st / L::TILE * 32 + (wave >> 1) * 16) = (f4){ks, raw_vs, __builtin_amdgcn_logf(raw_vs), __builtin_amdgcn_rcpf(raw_vs)};
+        };
+        // Step i's part: tile i + 2 to its stage, tile i + 3's loads, tile i + 4's table entry.
+        auto advance = [&](int i, u32 st2) __attribute__((always_inline)) {
+            if (i + 2 < n) put(st2);
+            if (i + 3 < n) load(i + 3);
+            if (i + 4 < n) fetch(i + 4);
+        };
+        bool holes = false;  // whether the cache lacks any page of the run's part
+        if (n > 0) {
+            fetch(0);
+            const int first = id;
+            fetch(min(1, n - 1));
+            const int second = id;
+            fetch(min(2, n - 1));
+            const int third = id;
+            id = first;
+            load(0);
+            const raw_t k0 = raw_k, v0 = raw_v;
+            const float ks0 = raw_ks, vs0 = raw_vs;
+            id = second;
+            load(min(1, n - 1));
+            const raw_t k1 = raw_k, v1 = raw_v;
+            const float ks1 = raw_ks, vs1 = raw_vs;
+            raw_k = k0, raw_v = v0, raw_ks = ks0, raw_vs = vs0;
+            put(0);
+            raw_k = k1, raw_v = v1, raw_ks = ks1, raw_vs = vs1;
+            put(L::TILE);
+            id = third;
+            load(min(2, n - 1));
+            fetch(min(3, n - 1));
+            const int e1 = div_by(min(key_first + n * UK, w.hi) - 1, p.S);
+            bool hole = false;
+            for (int e = div_by(key_first, p.S) + (int)threadIdx.x; e <= e1; e += 256) hole |= (u32)table[e] >= (u32)p.P;
+            hole = __any(hole);
+            if (lane_again() == 0) flags[wave] = hole;
+        }
+
+        f16v o[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] = (f16v){};
+        float m = LEAST, l = 0.f, l_old = 0.f, vm = 1e-35f, lvm = -116.26748f;  // lvm: log2 of vm; 512 / vm stays finite
+
+        if (!active) {  // no rows: the wave copies its part
+            if (n > 0) __syncthreads();
+            u32 st2 = 2 * L::TILE;
+            for (int i = 0; i < n; i++) {
+                advance(i, st2);
+                st2 = st2 == 2 * L::TILE ? 0 : st2 + L::TILE;
+                __syncthreads();
+            }
+        } else {
+            // Q as the B operand of S^T = K Q^T: fp16, its row's largest brought to 2^14 to 2^15, which `by` takes back.
+            u4v qf[KS];
+            float slope = 0.f, by;
+            int pos = 0;
+            {
+                const int row = min(wr0 + lq, w.r1), token = div_by(row, p.G), head = run.kvh * (int)p.G.d + row - token * (int)p.G.d;
+                const T* src = (const T*)p.q + (long)(w.first + token) * p.sqt + head * p.sqh;
+                float top = 0.f;
+#pragma unroll
+                for (int x = 0; x < KS; x++) qf[x] = *(const u4v*)(src + (2 * x + g) * 8);
+                auto values = [&](int x) __attribute__((always_inline)) {
+                    typedef T t8 __attribute__((ext_vector_type(8)));
+                    return __builtin_convertvector(__builtin_bit_cast(t8, qf[x]), f8);
+                };
+#pragma unroll
+                for (int x = 0; x < KS; x++) {
+                    const f8 v = values(x);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(v[e]));
+                }
+                const f2 h = both_halves(top);
+                top = fmaxf(h[0], h[1]);
+                const int up = top > 0.f && top <= FLT_TOP ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+                by = ldexpf(p.scale, -up);
+#pragma unroll
+                for (int x = 0; x < KS; x++) {
+                    f8 v = values(x);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = ldexpf(v[e], up);
+                    qf[x] = __builtin_bit_cast(u4v, __builtin_convertvector(v, h8));
+                }
+#pragma unroll
+                for (int x = 0; x < KS; x++) asm volatile("" : "+v"(qf[x]));  // made here, not inside the tile loop
+                if constexpr (MOD) {
+                    if (p.slopes) slope = p.slopes[head] * LOG2E;
+                    pos = w.p0 + token;
+                }
+            }
+            // The lane's K reads: row lq, chunk 2 x + g, at k_base ^ 32 x. Its V^T reads: lane i of 16 reads 8 bytes of row 4 g + i / 4 and gets the
+            // transposed values; chunk 4 d on of the row at v_base ^ 64 d.
+            u32 k_base = smem_u + (u32)(lq * ROW + ((g ^ (D == 128 ? lq & 15 : lq >> 1 & 7)) << 4));
+            u32 v_base;
+            {
+                const int sg = lane & 15, vr = 4 * g + (sg >> 2), c = 2 * (lane >> 4 & 1) + (sg >> 1 & 1);
+                v_base = smem_u + (u32)(L::V + vr * ROW + (sg & 1) * 8 + ((c ^ (D == 128 ? (vr & 3) << 2 : (vr >> 1 & 1) << 2)) << 4));
+            }
+            asm volatile("" : "+v"(k_base), "+v"(v_base));
+
+            // `st`: the offset of the tile's stage (the xors above leave a stage's bits alone).
+            auto qk = [&](u32 st, float (&out)[16], auto&& hook) __attribute__((always_inline)) {
+                u32 kb = k_base + st;
+                asm volatile("" : "+v"(kb));
+                f16v acc = {};
+                u4v ka[KS / 2];
+#pragma unroll
+                for (int x = 0; x < KS / 2; x++) ka[x] = lds_u4(kb ^ (u32)(32 * x));
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 0; x < KS; x++) {
+                    acc = product32<half_t>(ka[x % (KS / 2)], qf[x], acc);
+                    if (x < KS / 2) ka[x] = lds_u4(kb ^ (u32)(32 * (KS / 2 + x)));
+                    hook(x);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int r = 0; r < 16; r++) out[r] = acc[r];
+            };
+            // The keys of a tile that the lane's row sees, a bit each.
+            auto seen_keys = [&](int key0) __attribute__((always_inline)) {
+                auto below = [&](int key) __attribute__((always_inline)) { return (u32)((1ull << min(max(key - key0, 0), 32)) - 1); };
+                const int ln = lane_again(), at = w.p0 + div_by(min(wr0 + (ln & 31), w.r1), p.G);
+                u32 seen = below(min(at + 1, w.hi));
+                if (p.window > 0) seen &= ~below(at - p.window + 1);
+                seen |= below(w.prefix);  // at most hi
+                if (holes) {
+                    const int key = min(key0 + (ln & 31), w.hi - 1);
+                    seen &= (u32)__ballot((u32)table[div_by(key, p.S)] < (u32)p.P);
+                }
+                return seen;
+            };
+            auto scales_of = [&](u32 st, int half) __attribute__((always_inline)) {
+                return *(const lds_f4_t*)(size_t)(smem_u + (u32)(Tiles8Lds<D>::SCALES + half * 16) + st / L::TILE * 32);
+            };
+            // What x is times in the softmax's exponent, besides the scales: capped scores without a bias stay the -1 / (1 + 2^e) of their tanh (see capped), times
+            // 2 cap. (From HIGH_CAP on, 2 cap passes 4096 and they are made whole first, as large scores are, below.)
+            const float scale = MOD && p.cap > 0.f && !p.slopes && p.cap < HIGH_CAP ? 2.f * p.cap : 1.f;
+            // Changed scores: c0, c1 the factors of the two halves' products.
+            auto bias = [&](float (&x)[16], int key0, float c0, float c1) __attribute__((always_inline)) {
+                if constexpr (MOD) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++) x[r] *= r < 8 ? c0 : c1;
+                    if (__builtin_expect(p.cap >= HIGH_CAP, 0)) {
+#pragma unroll
+                        for (int r = 0; r < 16; r++) x[r] = capped<true>(x[r], p.cap);
+                    } else if (p.cap > 0.f) {
+#pragma unroll
+                        for (int r = 0; r < 16; r++) x[r] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x[r]));
+                        if (scale != 1.f) return;
+#pragma unroll
+                        for (int r = 0; r < 16; r++) x[r] = __builtin_fmaf(2.f * p.cap, x[r], p.cap);
+                    }
+                    if (p.slopes) {
+                        const float d0 = (float)(pos - key0 - 4 * g);
+#pragma unroll
+                        for (int r = 0; r < 16; r++) x[r] = __builtin_fmaf(-slope, fabsf(d0 - (float)(8 * (r >> 2) + (r & 3))), x[r]);
+                    }
+                }
+            };
+            u4v pf[2];  // P of the two 16-key halves
+            // The tile at hand in full steps: of half h, 2^(fma(x, factor, add)) is P; sum of P so far; what takes P's scale out of a sum.
+            float factor1 = 1.f, add1 = 0.f, sum0 = 0.f, sum1 = 0.f, back0 = 0.f, back1 = 0.f;
+            // Part k (of four) of a half's P.
+            auto exps = [&](const float* x, int k, u4v& d, float factor, float add, float& sum) __attribute__((always_inline)) {
+                const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * k], factor, add)), b = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * k + 1], factor, add));
+                const u32 word = pair_of<half_t>(a, b);
+                sum = add_pair<half_t>(word, sum);
+                d[k] = word;
+            };
+            // A half's P of a plain step: scores are whole, P is summed first, then times f.
+            auto exps_plain = [&](const float* x, u4v& d, float f) __attribute__((always_inline)) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float a = __builtin_amdgcn_exp2f(x[2 * k] - m), b = __builtin_amdgcn_exp2f(x[2 * k + 1] - m);
+                    l += a;
+                    l += b;
+                    d[k] = pair_of<half_t>(a * f, b * f);
+                }
+            };
+            auto no_hook = [](int) {};
+            auto read_v = [&](u32 vb, int j, int d) __attribute__((always_inline)) {
+                const u32 at = (vb ^ (u32)(64 * d)) + 16 * j * ROW;
+                return __builtin_shufflevector(lds_tr(at), lds_tr(at + 8 * ROW), 0, 1, 2, 3);
+            };
+            auto pv = [&](u32 st, auto&& hook) __attribute__((always_inline)) {
+                u32 vb = v_base + st;
+                asm volatile("" : "+v"(vb));
+                u4v va[DT];
+#pragma unroll
+                for (int d = 0; d < DT; d++) va[d] = read_v(vb, 0, d);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    o[d] = product32<half_t>(va[d], pf[0], o[d]);
+                    va[d] = read_v(vb, 1, d);
+                    hook(d);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    o[d] = product32<half_t>(va[d], pf[1], o[d]);
+                    hook(DT + d);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+
+            // Tiles all of whose keys all of the wave's rows see: full0 .. full1 - 1.
+            int full0 = 0, full1 = 0;
+            float sa[16], sb[16];
+            bool large = false;
+            // A tile's first part, wherever it lies: its scores, whole (x factor - m in one rounding would leave fp32's range where scores pass 2^24: a wave that
+            // meets one of 4096 or more takes no full steps from then on), masked where not every row sees every key, the maximum, vm, and the first half of P.
+            // Returns whether full steps may follow; half1: what the second half's P is times.
+            auto begin_tile = [&](int i, u32 st, u32 seen, bool masked, float& half1) __attribute__((always_inline)) {
+                qk(st, sa, no_hook);
+                const f4 t0 = scales_of(st, 0), t1 = scales_of(st, 1);
+                const float c0 = by * t0[0], c1 = by * t1[0];
+                if constexpr (MOD) bias(sa, key_of(i), c0, c1);
+#pragma unroll
+                for (int r = 0; r < 16; r++) sa[r] *= MOD ? scale : r < 8 ? c0 : c1;
+                if constexpr (!MOD) {
+                    if (!large) {
+                        float a = 0.f;
+#pragma unroll
+                        for (int r = 0; r < 16; r++) a = fmaxf(a, fabsf(sa[r]));
+                        large = __any(a >= 4096.f);
+                    }
+                }
+                if (masked) {
+                    const u32 mine = seen >> (4 * (lane_again() >> 5));  // register r: key 8 (r / 4) + 4 g + r % 4
+#pragma unroll
+                    for (int r = 0; r < 16; r++) sa[r] = mine >> (8 * (r >> 2) + (r & 3)) & 1 ? sa[r] : -__builtin_inff();
+                }
+                float mx = sa[0];
+#pragma unroll
+                for (int r = 1; r < 16; r++) mx = fmaxf(mx, sa[r]);
+                const f2 h = both_halves(mx);
+                mx = fmaxf(h[0], h[1]);
+                const bool see0 = seen & 0xffffu, see1 = seen >> 16;
+                const float v0 = see0 && t0[1] <= FLT_TOP ? t0[1] : 0.f, v1 = see1 && t1[1] <= FLT_TOP ? t1[1] : 0.f, vx = fmaxf(v0, v1);
+                if (__any(mx > m + 2.f || vx > vm)) {
+                    const float mn = mx > m + 2.f ? mx : m, vn = vx > vm ? fminf(2.f * vx, FLT_TOP) : vm, a = __builtin_amdgcn_exp2f(m - mn);
+                    const float b = a * (vm / vn);
+                    m = mn;
+                    vm = vn;
+                    lvm = __builtin_amdgcn_logf(vn);
+                    l *= a;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) o[d] *= b;
+                }
+                l_old = l;
+                if ((see0 && !(t0[1] <= FLT_TOP)) || (see1 && !(t1[1] <= FLT_TOP))) l = l_old = __builtin_nanf("");
+                const float unit = 512.f / vm;
+                half1 = v1 * unit;
+                exps_plain(sa, pf[0], v0 * unit);
+                // For a full step that follows: the scores are whole, P's first half is in l.
+                sum0 = 0.f;
+                back0 = 0.f;
+                factor1 = 1.f;
+                const float d1 = t1[2] - lvm + LIFT_TILES;
+                add1 = d1 - m;
+                back1 = vm * (1.f / 512.f) * t1[3];
+                return !large && !__any(!(d1 <= LIFT_TILES && d1 >= LIFT_TILES + LEAST_RATIO));
+            };
+            // A step of the full tiles: tile i's scores are in s, its P's first half in pf[0] and sum0 (or in l); tile i + 1 is full
+            // too, and its scores go to nxt. Steps of KS (or 2 DT = KS) products: the four parts of half a tile's exponentials beside every
+            // (KS / 4)-th. P is made with the m and vm at hand: a lane's sum of no more than MOST_TILES proves that no P was above it; else, or where tile i + 1's
+            // scales of V do not suit vm, the step ends before the product (false), and the tile is taken again by a plain step.
+            auto beside = [](int x) __attribute__((always_inline)) { return x % (KS / 4) == KS / 4 - 1; };
+            auto full_step = [&](int i, u32 st, u32 st1, u32 st2, const float (&s)[16], float (&nxt)[16]) __attribute__((always_inline)) {
+                advance(i, st2);
+                const f4 t0 = scales_of(st1, 0), t1 = scales_of(st1, 1);
+                sum1 = 0.f;
+                qk(st1, nxt, [&](int x) { if (beside(x)) exps(s + 8, x / (KS / 4), pf[1], factor1, add1, sum1); });
+                const float d0 = t0[2] - lvm, d1 = t1[2] - lvm;
+                if (__builtin_expect(__any(!(sum0 + sum1 <= MOST_TILES && fmaxf(d0, d1) <= 0.f && d0 >= LEAST_RATIO && d1 >= LEAST_RATIO)), 0)) return false;
+                const float c0 = by * t0[0], c1 = by * t1[0];
+                bias(nxt, key_of(i + 1), c0, c1);
+                l = __builtin_fmaf(sum0, back0, __builtin_fmaf(sum1, back1, l));
+                l_old = l;
+                const float factor0 = MOD ? scale : c0, add0 = d0 + LIFT_TILES - m, unit = vm * (1.f / 512.f);
+                factor1 = MOD ? scale : c1;
+                add1 = d1 + LIFT_TILES - m;
+                back0 = unit * t0[3];
+                back1 = unit * t1[3];
+                sum0 = 0.f;
+                u4v pn;
+                pv(st, [&](int x) {
+                    if (beside(x)) {
+                        exps(nxt, x / (KS / 4), pn, factor0, add0, sum0);
+                        asm volatile("" : "+v"(pn), "+v"(sum0));
+                    }
+                });
+                pf[0] = pn;
+                __syncthreads();
+                return true;
+            };
+
+            if (n > 0) {
+                __syncthreads();
+                holes = uniform(flags[0] | flags[1] | flags[2] | flags[3]) != 0;
+                if (!holes) {
+                    const int upto = min(w.hi, p.window > 0 ? n0 + 1 : max(n0 + 1, w.prefix));
+                    full0 = p.window > 0 ? max(n1 - p.window + UK - key_first, 0) / UK : 0;  // the first tile with key0 > n1 - window
+                    full1 = min(max((upto - key_first) / UK, 0), n);
+                }
+            }
+            const int last = full1 - 3;  // pairs of full steps i, i + 1 up to it: tiles .. i + 2 are full
+            u32 st = 0, st1 = L::TILE, st2 = 2 * L::TILE;  // the stages of tiles i, i + 1, i + 2
+            auto turn_stages = [&]() __attribute__((always_inline)) {
+                const u32 x = st;
+                st = st1;
+                st1 = st2;
+                st2 = x;
+            };
+            for (int i = 0; i < n;) {
+                const bool masked = i < full0 || i >= full1;
+                u32 seen = ~0u;
+                if (masked) seen = seen_keys(key_of(i));
+                bool full = i >= full0 && i <= last, copied = false;  // whether step i's part of the copies is done
+                if (!full) {
+                    advance(i, st2);
+                    copied = true;
+                }
+                if (__any(seen != 0)) {
+                    float half1;
+                    while (true) {
+                        const bool may = begin_tile(i, st, seen, masked, half1);
+                        full = full && may;
+                        bool done = true, taken = true;  // taken: the tile's maximum is
+                        while (full) {
+                            taken = false;
+                            done = full_step(i, st, st1, st2, sa, sb);
+                            if (!done) break;
+                            i++;
+                            turn_stages();
+                            done = full_step(i, st, st1, st2, sb, sa);
+                            if (!done) break;
+                            i++;
+                            turn_stages();
+                            full = i <= last;
+                        }
+                        if (done) {
+                            if (!copied) advance(i, st2);
+                            copied = true;
+                            if (taken) {
+                                exps_plain(sa + 8, pf[1], half1);
+                                break;
+                            }
+                            sum1 = 0.f;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) exps(sa + 8, k, pf[1], factor1, add1, sum1);
+                            if (!__any(!(sum0 + sum1 <= MOST_TILES))) {
+                                l = __builtin_fmaf(sum0, back0, __builtin_fmaf(sum1, back1, l));
+                                break;
+                            }
+                        }
+                        // P above the maximum at hand, or a scale of V that does not suit: the tile again by a plain step, its copies made.
+                        l = l_old;
+                        copied = true;
+                        full = false;
+                    }
+                    pv(st, no_hook);
+                }
+                i++;
+                turn_stages();
+                __syncthreads();
+            }
+        }
+
+        // The rows turn around in LDS (chunk c of row r at c ^ (r & 15) or, of 8, c ^ (r & 7)) so that a store covers whole rows.
+        if (active) {
+            const int ln = lane_again(), lg = ln >> 5, lr = ln & 31;
+            const f2 lh = both_halves(l);
+            const float sum = lh[0] + lh[1], unit = vm * (1.f / 512.f);
+            char* turn = smem + wave * (32 * 256);
+            auto settle_lds = []() __attribute__((always_inline)) {
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            };
+            if (whole) {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that saw nothing: O is 0
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; r4++) {
+                        const f4 y = (f4){o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]} * unit * inv;
+                        const u2v word = {pair_of<T>(y[0], y[1]), pair_of<T>(y[2], y[3])};
+                        *(u2v*)(turn + lr * ROW + (((4 * d + r4) ^ (lr & (D / 8 - 1))) << 4) + 8 * lg) = word;
+                    }
+                settle_lds();
+#pragma unroll
+                for (int i = 0; i < 32 / CR; i++) {
+                    const int r = CR * i + ln / (D / 8), c = ln % (D / 8), out_row = wr0 + r;
+                    const u4v x = *(const u4v*)(turn + r * ROW + ((c ^ (r & (D / 8 - 1))) << 4));
+                    if (out_row <= w.r1) {
+                        const int token = div_by(out_row, p.G), head = run.kvh * (int)p.G.d + out_row - token * (int)p.G.d;
+                        *(u4v*)((T*)p.o + (long)(w.first + token) * p.sot + head * p.soh + c * 8) = x;
+                    }
+                }
+            } else {
+                float* part = partial<MT, D>(p, block, begins);
+#pragma unroll
+                for (int half = 0; half < D / 64; half++) {  // 64 values of fp32 at a time
+#pragma unroll
+                    for (int d = 0; d < 2; d++)
+#pragma unroll
+                        for (int r4 = 0; r4 < 4; r4++) {
+                            const f16v& z = o[2 * half + d];
+                            *(f4*)(turn + lr * 256 + (((8 * d + 2 * r4 + lg) ^ (lr & 15)) << 4)) = (f4){z[4 * r4], z[4 * r4 + 1], z[4 * r4 + 2], z[4 * r4 + 3]} * unit;
+                        }
+                    settle_lds();
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int r = 4 * i + (ln >> 4), c = ln & 15;
+                        *(f4*)(part + (32 * wave + r) * D + 64 * half + 4 * c) = *(const f4*)(turn + r * 256 + ((c ^ (r & 15)) << 4));
+                    }
+                    settle_lds();
+                }
+                if (lg == 0) {
+                    part[MT * D + 32 * wave + lr] = m;
+                    part[MT * D + MT + 32 * wave + lr] = sum;
+                }
+            }
+        }
+        __syncthreads();
+        if (begins && !last_part) {
+            cut.more = (int)((w.units - run.count + run.quota - 1) / run.quota);
+            cut.kvh = run.kvh;
+            cut.first = w.first;
+            cut.rows = w.rows;
+            cut.r0 = w.r0;
+        }
+        run.count -= min(w.units - run.unit, run.count);
+        run.unit = 0;
+        if (run.count > 0) next_tile<MT>(p, run);
+    }
+    if (threadIdx.x == 0) ((Cut*)p.ws)[block] = cut;
+}
+
 template <class T, int D, int MT>
 __global__ __launch_bounds__(256) void merge8_kernel(Attn8Args p) { merge_parts<T, D, MT>(p); }
 
@@ -593,7 +1120,7 @@ static int make_plan8(long T, long B, long H, long Hkv, long D, int type, Plan8*
     if (T <= 0 || B <= 0 || B > MAX_SEQUENCES || Hkv <= 0 || H <= 0 || H % Hkv || (D != 64 && D != 128) || type < RDA_FP16 || type > RDA_BF16) return RDA_ERR_INVALID;
     if (T * (H / Hkv) >= 1L << 31) return RDA_ERR_INVALID;
     const long rows = T * (H / Hkv) / B;
-    plan->mt = rows <= 16 ? 16 : 32;
+    plan->mt = rows <= 16 ? 16 : rows <= 64 || B * ((rows + 127) / 128) * Hkv <= 40 ? 32 : 128;
     plan->grid = 512;
     if ((T * (H / Hkv) / plan->mt + 1) * B >= 1L << 31) return RDA_ERR_INVALID;
     plan->workspace = (size_t)plan->grid * sizeof(Cut) + (size_t)plan->grid * 2 * plan->mt * (D + 2) * 4;
@@ -617,6 +1144,15 @@ static int launch_append8(const Append8Args& a, dim3 grid, size_t lds, void* str
     if (lds > 32768)  // angles of 64 tokens and more than 64 pairs, or of 32 and 128: up to 64 KB
         if (const int e = ensure_dynamic_lds((const void*)append8_kernel<X, Q, PS>, lds, done)) return e;
     hipLaunchKernelGGL((append8_kernel<X, Q, PS>), grid, dim3(256), lds, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+template <class T, int D>
+static int launch_tiles8(const Attn8Args& a, void* stream) {
+    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.grid), dim3(256), Tiles8Lds<D>::BYTES, (hipStream_t)stream, a); };
+    a.cap > 0.f || a.slopes ? launch(tiles8_kernel<T, D, true>) : launch(tiles8_kernel<T, D, false>);
+    if (const hipError_t e = hipGetLastError()) return (int)e;
+    hipLaunchKernelGGL((merge8_kernel<T, D, 128>), dim3(a.grid, 8), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 
@@ -719,12 +1255,13 @@ int rda_paged_attn_i8(const void* q, void* out, const void* k_codes, const void*
     if (!(a.scale >= 1.2e-38f && a.scale <= 3e38f && a.cap <= 3e38f)) return RDA_ERR_INVALID;
     a.window = window;
     // No more workgroups than units there can be: a short table of few sequences needs none that finds no work.
-    const long units = (T * (H / Hkv) / plan.mt + B) * ((N * S + 255) / 256 + ahead(plan.mt, false)) * Hkv;
+    const long least = plan.mt == 128 ? 32 : 256, units = (T * (H / Hkv) / plan.mt + B) * ((N * S + least - 1) / least + ahead(plan.mt, false)) * Hkv;
     a.grid = (int)(units < plan.grid ? units : plan.grid);
     a.runs = make_div(a.grid);
     a.fill = fill;
     const auto heads = [&](auto x) {
         using X = decltype(x);
+        if (plan.mt == 128) return D == 64 ? launch_tiles8<X, 64>(a, stream) : launch_tiles8<X, 128>(a, stream);
         if (plan.mt == 16) return D == 64 ? launch_rows8<X, 64, 1>(a, stream) : launch_rows8<X, 128, 1>(a, stream);
         return D == 64 ? launch_rows8<X, 64, 2>(a, stream) : launch_rows8<X, 128, 2>(a, stream);
     };
