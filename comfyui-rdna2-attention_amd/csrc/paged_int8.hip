@@ -275,9 +275,11 @@ __device__ __forceinline__ u2v widen4(u32 w) {
     w ^= 0x80808080u;
     return (u2v){less_bias(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)), less_bias(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u))};
 }
-// Byte j of a and of b as two fp16 codes (j a constant).
+// Byte j (a constant) of a and of b, their sign bits flipped before, as two fp16 codes x 2^-9: a byte in the low half of a word is the fp16 byte x 2^-24; that
+// times 2^15, less 128 x 2^-9 in the same operation, is exact.
 __device__ __forceinline__ u32 widen_pair(u32 a, u32 b, int j) {
-    return less_bias(__builtin_amdgcn_perm(b, a, 0x0c000c00u | (u32)j | (u32)(4 + j) << 16) ^ 0x64806480u);
+    const h2 x = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, a, 0x0c000c00u | (u32)j | (u32)(4 + j) << 16));
+    return __builtin_bit_cast(u32, __builtin_elementwise_fma(x, (h2){(half_t)32768.f, (half_t)32768.f}, (h2){(half_t)-0.25f, (half_t)-0.25f}));
 }
 __device__ __forceinline__ f4 product16(const u4v& a, const u4v& b, const f4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
@@ -364,7 +366,9 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
         if (w.hi > w.lo) {
             const int last = (w.hi - 1) / KG * KG;
             auto key_of = [&](int i) __attribute__((always_inline)) { return w.lo + (u0 + i) * UK + wave * KT; };
-            int kid, vid;  // table entries of the lane's K rows and of its keys of V
+            // Table entries of the lane's K rows and of its keys of V: of tile i + 1 until its loads of K, then of tile i + 2. What is waited for first is
+            // loaded first: scales and table entries ahead of V, whose loads end a step.
+            int kid, vid;
             auto fetch_ids = [&](int i) __attribute__((always_inline)) {
                 const int key0 = key_of(i);
                 kid = table[div_by(min(key0 + KG * (r >> 2), last), p.S)];
@@ -372,31 +376,35 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
             };
             u4v kf[4][KC];
             vvec vf[KG];
-            float ks = 0.f, vs = 0.f;
-            bool bad = false;  // the lane's keys are on a page that the cache does not have
+            float ks, vs, ks2, vs2;  // the scales of the lane's keys, of tile i and of tile i + 1
+            u32 vrow, vpage;         // where V of tile i + 1 lies
+            bool bad = false, bad2;  // the lane's keys are on a page that the cache does not have
             auto load_k = [&](int i) __attribute__((always_inline)) {
-                const int key = min(key_of(i) + KG * (r >> 2), last), row = key - div_by(key, p.S) * (int)p.S.d + (r & 3);
+                const int vkey = min(key_of(i) + KG * g, last), key = min(key_of(i) + KG * (r >> 2), last), row = key - div_by(key, p.S) * (int)p.S.d + (r & 3);
+                vrow = (u32)(vkey - div_by(vkey, p.S) * (int)p.S.d);
+                bad2 = (u32)vid >= (u32)p.P;
+                vpage = bad2 ? 0 : (u32)vid;
+                ks2 = ksbase[row_at(vpage, p.ksp, vrow >> p.shift, p.ksb)];
+                vs2 = vsbase[row_at(vpage, p.vsp, vrow >> p.shift, p.vsb)];
                 const signed char* src = kbase + row_at((u32)kid < (u32)p.P ? (u32)kid : 0, p.kpp, (u32)row, p.kpr) + 16 * g;
 #pragma unroll
                 for (int c = 0; c < 4; c++)
 #pragma unroll
                     for (int x = 0; x < KC; x++) kf[c][x] = *(const u4v*)(src + (unsigned long long)(4 * c) * p.kpr + 64 * x);
             };
-            auto load_v = [&](int i) __attribute__((always_inline)) {
-                const int key = min(key_of(i) + KG * g, last), row = key - div_by(key, p.S) * (int)p.S.d;
-                const u32 page = (u32)vid < (u32)p.P ? (u32)vid : 0;
-                bad = (u32)vid >= (u32)p.P;
-                const signed char* src = vbase + row_at(page, p.vpp, (u32)row, p.vpr) + r * VC;
+            auto load_v = [&]() __attribute__((always_inline)) {
+                const signed char* src = vbase + row_at(vpage, p.vpp, vrow, p.vpr) + r * VC;
 #pragma unroll
                 for (int e = 0; e < KG; e++) vf[e] = *(const vvec*)(src + (unsigned long long)e * p.vpr);
-                ks = ksbase[row_at(page, p.ksp, (u32)row >> p.shift, p.ksb)];
-                vs = vsbase[row_at(page, p.vsp, (u32)row >> p.shift, p.vsb)];
+                ks = ks2;
+                vs = vs2;
+                bad = bad2;
             };
             fetch_ids(0);
             load_k(0);
-            load_v(0);
-            if (n > 1) fetch_ids(1);
-            for (int i = 0; i < n; i++) {
+            fetch_ids(min(1, n - 1));
+            load_v();
+            for (int i = 0;; i++) {
                 const int key0 = key_of(i);
                 if (!(ks <= FLT_TOP)) ks = __builtin_nanf("");
                 float s[MB][KG];
@@ -422,9 +430,12 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
                         for (int e = 0; e < 4; e++) s[m][4 * c + e] = acc[e] * f;
                     }
                 }
-                if (i + 1 < n) load_k(i + 1);
+                const bool hole = bad;
+                // (The last tile's K again behind it, from L2: under a branch the waits for V would be for these loads too.)
+                load_k(min(i + 1, n - 1));
+                fetch_ids(min(i + 2, n - 1));
                 // Whether every row sees every key of the tile.
-                const bool all = key0 + KT <= w.hi && !__any(bad) && (key0 + KT <= n0 + 1 || key0 + KT <= w.prefix) &&
+                const bool all = key0 + KT <= w.hi && !__any(hole) && (key0 + KT <= n0 + 1 || key0 + KT <= w.prefix) &&
                                  (p.window <= 0 || n1 - key0 < p.window || key0 + KT <= w.prefix);
                 if constexpr (MOD) {
                     const auto cap_all = [&](auto fine) __attribute__((always_inline)) {
@@ -450,7 +461,7 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
 #pragma unroll
                         for (int e = 0; e < KG; e++) {
                             const int key = key0 + KG * g + e;
-                            const bool ok = key < w.hi && !bad && ((key <= pos[m] && (p.window <= 0 || pos[m] - key < p.window)) || key < pre[m]);
+                            const bool ok = key < w.hi && !hole && ((key <= pos[m] && (p.window <= 0 || pos[m] - key < p.window)) || key < pre[m]);
                             if (!ok) s[m][e] = -__builtin_inff();
                             see[m] |= ok ? 1u << e : 0;
                         }
@@ -492,6 +503,8 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
                 }
                 // O^T += V^T P^T.
 #pragma unroll
+                for (int e = 0; e < KG; e++) vf[e] ^= 0x80808080u;
+#pragma unroll
                 for (int j = 0; j < VC; j++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
@@ -506,17 +519,15 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
 #pragma unroll
                         for (int m = 0; m < MB; m++) o[m][j] = product16(a, pf[m][h], o[m][j]);
                     }
-                if (i + 1 < n) {
-                    load_v(i + 1);
-                    if (i + 2 < n) fetch_ids(i + 2);
-                }
+                if (i + 1 >= n) break;
+                load_v();
             }
         }
 
         // The four waves' results meet in LDS, 16 rows at a time: thread (row t / 16, dims from t % 16 on) adds them.
 #pragma unroll
         for (int m = 0; m < MB; m++) {
-            const float l = rows_sum(l_[m]), unit = vm[m] * (1.f / 128.f);
+            const float l = rows_sum(l_[m]), unit = vm[m] * 4.f;  // P's 2^7, codes' 2^-9
             __syncthreads();
             if (g == 0) {
                 ml[0][wave][r] = m_[m];
@@ -590,7 +601,7 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
 //   rounded P times what takes that out again. So full steps do nothing more per score than those of a 16-bit cache.
 // * Where a scale of V is above the row's vm, or below it by more than 2^8, or is not finite, the step is not a full one: the plain steps sum P before it
 //   is scaled, and move vm (to twice the scale: O is then seldom rescaled).
-#define TILES8_WGS(D, MOD) 2
+#define TILES8_WGS(D, MOD) ((D) == 64 && !(MOD) ? 3 : 2)
 #define LIFT_TILES 9.f        // P stands 2^9 vs / vm above 2^(x - m), of which at most 2^2 are in a plain step
 #define MOST_TILES 32768.f    // of a full step's sum of P in a lane, so that no P is above it
 #define LEAST_RATIO -8.f      // log2 of vs / vm
@@ -609,6 +620,9 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
     using L = TilesLds<D>;
     typedef typename std::conditional<D == 128, u4v, u2v>::type raw_t;
     typedef __attribute__((address_space(3))) f4 lds_f4_t;
+    // Loads in flight over LDS reads are of the global address space: flat ones would count as LDS accesses, which the reads wait for.
+    typedef __attribute__((address_space(1))) raw_t global_raw_t;
+    typedef __attribute__((address_space(1))) float global_float_t;
     extern __shared__ __attribute__((aligned(256))) char smem[];
     const int lane = threadIdx.x & 63, g = lane >> 5, lq = lane & 31;
     const int wave = uniform((int)(threadIdx.x >> 6));
@@ -644,10 +658,10 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
         auto load = [&](int i) __attribute__((always_inline)) {
             const int key = group_of(i), row = key - div_by(key, p.S) * (int)p.S.d;
             const u32 at = (u32)uniform(id), page = at < (u32)p.P ? at : 0;
-            raw_k = *(const raw_t*)(kbase + row_at(page, p.kpp, (u32)row + 8 * (wave & 1), p.kpr) + k_lane);
-            raw_v = *(const raw_t*)(vbase + row_at(page, p.vpp, (u32)row + 8 * (wave & 1), p.vpr) + v_lane);
-            raw_ks = ksbase[row_at(page, p.ksp, (u32)row >> p.shift, p.ksb)];
-            raw_vs = vsbase[row_at(page, p.vsp, (u32)row >> p.shift, p.vsb)];
+            raw_k = *(const global_raw_t*)(kbase + row_at(page, p.kpp, (u32)row + 8 * (wave & 1), p.kpr) + k_lane);
+            raw_v = *(const global_raw_t*)(vbase + row_at(page, p.vpp, (u32)row + 8 * (wave & 1), p.vpr) + v_lane);
+            raw_ks = *(const global_float_t*)(ksbase + row_at(page, p.ksp, (u32)row >> p.shift, p.ksb));
+            raw_vs = *(const global_float_t*)(vsbase + row_at(page, p.vsp, (u32)row >> p.shift, p.vsb));
         };
         const int my_row = 8 * wave + (lane >> 3);
         auto put = [&](u32 st) __attribute__((always_inline)) {
@@ -1121,7 +1135,7 @@ static int make_plan8(long T, long B, long H, long Hkv, long D, int type, Plan8*
     if (T * (H / Hkv) >= 1L << 31) return RDA_ERR_INVALID;
     const long rows = T * (H / Hkv) / B;
     plan->mt = rows <= 16 ? 16 : rows <= 64 || B * ((rows + 127) / 128) * Hkv <= 40 ? 32 : 128;
-    plan->grid = 512;
+    plan->grid = plan->mt == 128 && D == 64 ? 768 : 512;
     if ((T * (H / Hkv) / plan->mt + 1) * B >= 1L << 31) return RDA_ERR_INVALID;
     plan->workspace = (size_t)plan->grid * sizeof(Cut) + (size_t)plan->grid * 2 * plan->mt * (D + 2) * 4;
     return 0;
@@ -1256,7 +1270,8 @@ int rda_paged_attn_i8(const void* q, void* out, const void* k_codes, const void*
     a.window = window;
     // No more workgroups than units there can be: a short table of few sequences needs none that finds no work.
     const long least = plan.mt == 128 ? 32 : 256, units = (T * (H / Hkv) / plan.mt + B) * ((N * S + least - 1) / least + ahead(plan.mt, false)) * Hkv;
-    a.grid = (int)(units < plan.grid ? units : plan.grid);
+    const int most = softcap > 0.f || slopes ? 512 : plan.grid;
+    a.grid = (int)(units < most ? units : most);
     a.runs = make_div(a.grid);
     a.fill = fill;
     const auto heads = [&](auto x) {
