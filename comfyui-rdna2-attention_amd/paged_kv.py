@@ -91,10 +91,10 @@ class QuantizedCache:
 
     @classmethod
     def empty(cls, pages, page_size, kv_heads, dim, block=32, device="cuda"):
-        """A cache of `pages` pages of nothing yet, contiguous."""
+        """A cache of `pages` pages of nothing yet, each head's tokens of a page together in memory, which attention reads fastest."""
         if block not in BLOCKS or page_size <= 0 or page_size % block:
             raise ValueError(f"QuantizedCache takes blocks of 16, 32 or 64 tokens, pages of whole blocks, not {block} and {page_size}")
-        codes = torch.zeros(2, pages, page_size, kv_heads, dim, dtype=torch.int8, device=device)
+        codes = torch.zeros(2, pages, kv_heads, page_size, dim, dtype=torch.int8, device=device).transpose(2, 3)
         scales = torch.zeros(2, pages, page_size // block, kv_heads, dtype=torch.float32, device=device)
         return cls(codes[0], codes[1], scales[0], scales[1])
 
