@@ -25,21 +25,57 @@ struct Append8Args {
     long pitch, sqt, sqh, skt, skh, svt, svh, sot, soh, kpp, kpr, kph, vpp, vpr, vph, ksp, ksb, ksh, vsp, vsb, vsh;
 };
 
-// Workgroups (x, *) take a block of one sequence's new tokens each. Sequence b's are the x from first_slot(b) on: with its n new tokens it touches at most
-// (n - 2) / block + 2 blocks, and has n / block rounded down + 2 slots at least, whatever its position, so that no sums over the sequences are needed.
-__device__ __forceinline__ int first_slot(const Append8Args& p, int b) { return min(max(p.starts[b], 0), p.T) / p.block + 2 * b; }
-__device__ __forceinline__ int sequence_of_slot(const Append8Args& p, int slot, int lane) {
-    int at = 0, n = p.B;  // as sequence_of: the number of first slots of 1 .. B at or below slot
+// The last of B sequences that begins at or below `target` (B: behind them), its first row and the next one's, and its length; a sequence begins at
+// key(starts[b], b). 64 are looked at in a step, one per lane, and the last step's lanes hold what is asked for of theirs, so that it costs one access to
+// memory where there are at most 64.
+struct Sequence {
+    int b, first, end, length;
+};
+template <class Key>
+__device__ __forceinline__ Sequence find_sequence(const int* starts, const int* lengths, int B, int target, int lane, Key&& key) {
+    int at = 0, n = B;  // the answer is at .. at + n
     while (n > 64) {
         const int step = (n + 63) >> 6, i = (lane + 1) * step;
-        const bool below = i <= n && first_slot(p, at + i) <= slot;
+        const bool below = i <= n && key(starts[at + i], at + i) <= target;
         const int c = __popcll(__ballot(below));
         at += c * step;
         n = min(step - 1, n - c * step);
     }
-    const bool below = lane < n && first_slot(p, at + 1 + lane) <= slot;
-    return at + __popcll(__ballot(below));
+    const int from = starts[min(at + lane, B)], to = starts[min(at + lane + 1, B)], length = lengths[min(at + lane, B - 1)];
+    const bool below = lane < n && key(to, at + lane + 1) <= target;
+    const int c = __builtin_amdgcn_readfirstlane(__popcll(__ballot(below)));
+    Sequence s = {__builtin_amdgcn_readfirstlane(at) + c, 0, 0, 0};
+    if (c < 64) {
+        s.first = __builtin_amdgcn_readlane(from, c);
+        s.end = __builtin_amdgcn_readlane(to, c);
+        s.length = __builtin_amdgcn_readlane(length, c);
+    } else if (s.b < B) {
+        s.first = starts[s.b];
+        s.end = starts[s.b + 1];
+        s.length = lengths[s.b];
+    }
+    return s;
 }
+
+// Eight values or weights as they lie in memory, so that loads are not waited for where they are issued.
+template <class X>
+struct Raw8 {
+    u4v v[sizeof(X) / 2];
+    __device__ __forceinline__ void load(const X* p) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(X) / 2); i++) v[i] = ((const u4v*)p)[i];
+    }
+    __device__ __forceinline__ f8 values() const { return load8((const X*)v); }
+};
+struct RawWeights {
+    u4v v[2];  // of 16-bit types the first alone
+    __device__ __forceinline__ void load(const void* w, int type, int at) {
+        const char* p = (const char*)w + at * (type == RDA_FP32 ? 4 : 2);
+        v[0] = *(const u4v*)p;
+        v[1] = *(const u4v*)(p + (type == RDA_FP32 ? 16 : 0));
+    }
+    __device__ __forceinline__ f8 values(int type) const { return weights8(v, type, 0); }
+};
 
 // The largest over the wave's lanes.
 __device__ __forceinline__ u32 wave_max(u32 x) {
@@ -73,6 +109,37 @@ __device__ __forceinline__ f8 load_codes(const signed char* p) {
 }
 #define FLT_TOP 3.402823466e38f
 #define LEAST_SCALE 1e-30f
+// The largest magnitude of 16 values, as bits: magnitudes order as their bits do, infinities and NaN above the finite ones.
+__device__ __forceinline__ u32 largest(const f8& a, const f8& b) {
+    u32 top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) top = max(top, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(b[e]) & 0x7fffffffu));
+    return top;
+}
+// The scale of a block whose new values' largest magnitude is `top` and whose older ones' scale is `had` (0: it has none): NaN, and codes of 0, where not all are finite.
+struct NewScale {
+    float now, by;
+    bool finite;
+};
+__device__ __forceinline__ NewScale new_scale(u32 top, float had) {
+    const bool finite = top < 0x7f800000u && had <= FLT_TOP;
+    const float now = finite ? fmaxf(fmaxf(__uint_as_float(top) / 127.f, LEAST_SCALE), had) : __builtin_nanf("");
+    return {now, finite ? 1.f / now : 0.f, finite};
+}
+// The largest over the `per` lanes that hold a head.
+__device__ __forceinline__ u32 head_max(u32 x, int per, int lane) {
+    if ((per & (per - 1)) == 0) {
+        if (per >= 2) x = max(x, (u32)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, true));
+        if (per >= 4) x = max(x, (u32)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true));
+        if (per >= 8) x = max(x, (u32)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xF, 0xF, true));
+        if (per >= 16) x = max(x, (u32)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xF, 0xF, true));
+        return x;
+    }
+    const int base = lane - lane % per;
+    u32 top = 0;
+    for (int i = 0; i < per; i++) top = max(top, (u32)__shfl((int)x, base + i));
+    return top;
+}
 
 // One step's keys and values as codes into their blocks, keys normed and turned on the way, and queries normed and turned. A workgroup takes a block
 // and `slice` heads (queries, keys, values in this order): it makes the angles of the block's new tokens once, and takes 16 tokens of a head to a wave, block / 16
@@ -84,31 +151,25 @@ __global__ __launch_bounds__(256) void append8_kernel(Append8Args p) {
     __shared__ u32 most[2][4];
     f2* cs = (f2*)smem;  // [row of the block][pair]
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int slot = blockIdx.x, b = __builtin_amdgcn_readfirstlane(sequence_of_slot(p, slot, lane));
-    if (b >= p.B) return;
-    const int first = min(max(p.starts[b], 0), p.T), tokens = min(max(p.starts[b + 1], first), p.T) - first;
+    const int pairs = p.r.R / 2, rows_at_once = pairs ? 256 / pairs : 0, my_pair = pairs ? t % pairs : 0;  // of the angles: a thread's pair stays
+    const double turns = pairs ? p.r.turns[my_pair] : 0.;
+    const int slot = blockIdx.x, shift = p.block == 16 ? 4 : p.block == 32 ? 5 : 6;
+    // Sequence b's slots are those from here on: with its n new tokens it touches at most (n - 2) / block + 2 blocks, and has n / block rounded down
+    // + 2 slots at least, whatever its position, so that no sums over the sequences are needed.
+    auto first_slot = [&](int start, int b) __attribute__((always_inline)) { return (min(max(start, 0), p.T) >> shift) + 2 * b; };
+    const Sequence q = find_sequence(p.starts, p.lengths, p.B, slot, lane, first_slot);
+    if (q.b >= p.B) return;
+    const int first = min(max(q.first, 0), p.T), tokens = min(max(q.end, first), p.T) - first;
     if (tokens == 0) return;
-    const int p0 = max(p.lengths[b], -(1 << 30)) - tokens;             // position of the first new token; negative: no place for it
-    const int shift = p.block == 16 ? 4 : p.block == 32 ? 5 : 6;
-    const int b0 = ((p0 >> shift) + (slot - first_slot(p, b))) << shift;  // the block's first position
+    const int p0 = max(q.length, -(1 << 30)) - tokens;  // position of the first new token; negative: no place for it
+    const int b0 = ((p0 >> shift) + (slot - first_slot(q.first, q.b))) << shift;  // the block's first position
     const int o0 = max(p0 - b0, 0), o1 = min(p0 + tokens - b0, p.block);  // its new rows
     if (o0 >= o1) return;
     const int head0 = blockIdx.y * p.slice, head1 = min(head0 + p.slice, p.H + 2 * p.Hkv);
     const int entry = b0 >= 0 ? div_by(b0, p.S) : p.N;
     int page = -1;
-    if (entry < p.N) page = p.table[b * p.pitch + entry];
-    const bool there = page >= 0 && page < p.P;
-    const int row0 = there ? b0 - entry * (int)p.S.d : 0, part0 = row0 >> shift;  // the block's first row of the page; its number there
+    if (entry < p.N) page = p.table[q.b * p.pitch + entry];
 
-    const int pairs = p.r.R / 2;
-    if (pairs && head0 < p.H + p.Hkv) {
-        for (int i = t; i < (o1 - o0) * pairs; i += 256) {
-            const int row = o0 + i / pairs, pair = i % pairs;
-            const f2 v = cos_sin((double)(b0 + row), p.r.turns[pair]);
-            cs[row * pairs + pair] = (f2){v[0] * p.r.factor, v[1] * p.r.factor};
-        }
-        __syncthreads();
-    }
     const Place pl = place(p.r, lane);
     const int per = p.r.D / 16, waves = p.block >> 4, sub = wave & (waves - 1), together = 4 / waves;  // waves of a head; the wave's 16 rows; heads at once
     int row[PS];
@@ -119,23 +180,57 @@ __global__ __launch_bounds__(256) void append8_kernel(Append8Args p) {
         row[i] = 16 * sub + x;
         mine[i] = pl.head < pl.heads && x < 16 && row[i] >= o0 && row[i] < o1;
     }
+    // The values and weights of the wave's head of the heads h0 on, and the scale that its block has.
+    Raw8<X> raw_lo[PS], raw_hi[PS];
+    RawWeights raw_wl, raw_wh;
+    float *raw_scale = nullptr, raw_had = 0.f;
+    auto load = [&](int h0) __attribute__((always_inline)) {
+        const int h = min(h0 + wave / waves, head1 - 1), hk = h - p.H, hv = hk - p.Hkv;
+        const X* src = hk < 0 ? (const X*)p.q + h * p.sqh : hv < 0 ? (const X*)p.k + hk * p.skh : (const X*)p.v + hv * p.svh;
+        const long st = hk < 0 ? p.sqt : hv < 0 ? p.skt : p.svt;
+#pragma unroll
+        for (int i = 0; i < PS; i++) {
+            const X* at = src + (first + b0 - p0 + (mine[i] ? row[i] : o0)) * st;
+            raw_lo[i].load(at + pl.at);
+            raw_hi[i].load(at + pl.to);
+        }
+        if (p.kw && hv < 0) {
+            raw_wl.load(hk < 0 ? p.qw : p.kw, p.wtype, pl.at);
+            raw_wh.load(hk < 0 ? p.qw : p.kw, p.wtype, pl.to);
+        }
+        if (page >= 0 && page < p.P && hk >= 0) {
+            const int part = (b0 - entry * (int)p.S.d) >> shift;  // the block's number in its page
+            raw_scale = hv < 0 ? p.ks + page * p.ksp + part * p.ksb + hk * p.ksh : p.vs + page * p.vsp + part * p.vsb + hv * p.vsh;
+            if (o0 > 0) raw_had = *raw_scale;
+        }
+    };
+    load(head0);
+    const bool there = page >= 0 && page < p.P;
+    const int row0 = there ? b0 - entry * (int)p.S.d : 0;  // the block's first row of the page
+
+    if (pairs && head0 < p.H + p.Hkv) {
+        if (t < rows_at_once * pairs)
+            for (int row = o0 + t / pairs; row < o1; row += rows_at_once) {
+                const f2 v = cos_sin((double)(b0 + row), turns);
+                cs[row * pairs + my_pair] = (f2){v[0] * p.r.factor, v[1] * p.r.factor};
+            }
+        __syncthreads();
+    }
     int turn_of = 0;
     for (int h0 = head0; h0 < head1; h0 += together, turn_of ^= 1) {
         const int h = h0 + wave / waves, hk = h - p.H, hv = hk - p.Hkv;
-        const bool active = h < head1;
+        const bool active = h < head1, writes = active && hk >= 0 && there;
+        float* const scale = raw_scale;
+        const float had = raw_had;
         f8 lo[PS], hi[PS];
         if (active) {
-            const X* src = hk < 0 ? (const X*)p.q + h * p.sqh : hv < 0 ? (const X*)p.k + hk * p.skh : (const X*)p.v + hv * p.svh;
-            const long st = hk < 0 ? p.sqt : hv < 0 ? p.skt : p.svt;
 #pragma unroll
             for (int i = 0; i < PS; i++) {
-                const X* at = src + (first + b0 - p0 + (mine[i] ? row[i] : o0)) * st;
-                lo[i] = load8(at + pl.at);
-                hi[i] = load8(at + pl.to);
+                lo[i] = raw_lo[i].values();
+                hi[i] = raw_hi[i].values();
             }
-            const void* w = hk < 0 ? p.qw : hv < 0 ? p.kw : nullptr;
-            if (w) {
-                const f8 wl = weights8(w, p.wtype, pl.at), wh = weights8(w, p.wtype, pl.to);
+            if (p.kw && hv < 0) {
+                const f8 wl = raw_wl.values(p.wtype), wh = raw_wh.values(p.wtype);
 #pragma unroll
                 for (int i = 0; i < PS; i++) {
                     const float inv = inverse_rms(lo[i], hi[i], p.r.D, p.eps, per, lane);
@@ -151,6 +246,7 @@ __global__ __launch_bounds__(256) void append8_kernel(Append8Args p) {
                     turn(lo[i], hi[i], c, s, p.r.interleaved);
                 }
             }
+            if (h0 + together < head1) load(h0 + together);
             if (hk < 0) {
 #pragma unroll
                 for (int i = 0; i < PS; i++)
@@ -166,17 +262,8 @@ __global__ __launch_bounds__(256) void append8_kernel(Append8Args p) {
         if (active && hk >= 0) {
 #pragma unroll
             for (int i = 0; i < PS; i++)
-                if (mine[i])
-#pragma unroll
-                    for (int e = 0; e < 8; e++) top = max(top, max(__float_as_uint(lo[i][e]) & 0x7fffffffu, __float_as_uint(hi[i][e]) & 0x7fffffffu));
+                if (mine[i]) top = max(top, largest(lo[i], hi[i]));
             top = wave_max(top);
-        }
-        const bool writes = active && hk >= 0 && there;
-        float* scale = nullptr;
-        float had = 0.f;
-        if (writes) {
-            scale = hv < 0 ? p.ks + page * p.ksp + part0 * p.ksb + hk * p.ksh : p.vs + page * p.vsp + part0 * p.vsb + hv * p.vsh;
-            if (o0 > 0) had = *scale;
         }
         if (waves > 1) {  // also: every wave has read the scale before one writes it
             if (lane == 0) most[turn_of][wave] = top;
@@ -186,18 +273,16 @@ __global__ __launch_bounds__(256) void append8_kernel(Append8Args p) {
         if (!writes) continue;
         signed char* codes = hv < 0 ? p.kc + page * p.kpp + row0 * p.kpr + hk * p.kph : p.vc + page * p.vpp + row0 * p.vpr + hv * p.vph;
         const long cr = hv < 0 ? p.kpr : p.vpr;
-        const float need = fmaxf(__uint_as_float(top) / 127.f, LEAST_SCALE);
-        const bool finite = top < 0x7f800000u && had <= FLT_TOP;
-        const float now = finite ? fmaxf(need, had) : __builtin_nanf(""), by = finite ? 1.f / now : 0.f;
+        const NewScale s = new_scale(top, had);
 #pragma unroll
         for (int i = 0; i < PS; i++) {
             if (mine[i]) {
-                store_codes(codes + row[i] * cr + pl.at, finite ? over(lo[i], now, by) : (f8){});
-                store_codes(codes + row[i] * cr + pl.to, finite ? over(hi[i], now, by) : (f8){});
+                store_codes(codes + row[i] * cr + pl.at, s.finite ? over(lo[i], s.now, s.by) : (f8){});
+                store_codes(codes + row[i] * cr + pl.to, s.finite ? over(hi[i], s.now, s.by) : (f8){});
             }
         }
-        if (o0 > 0 && finite && now != had) {
-            const float shrink = had * by;
+        if (o0 > 0 && s.finite && s.now != had) {
+            const float shrink = had * s.by;
 #pragma unroll
             for (int i = 0; i < PS; i++) {
                 const int x = i * pl.heads + pl.head;
@@ -209,7 +294,126 @@ __global__ __launch_bounds__(256) void append8_kernel(Append8Args p) {
                 }
             }
         }
-        if (sub == 0 && lane == 0) *scale = now;
+        if (sub == 0 && lane == 0) *scale = s.now;
+    }
+}
+
+// The same for steps of few tokens a sequence, whose blocks have one new row, seldom more: a wave takes a token and as many heads of one tensor as its lanes
+// hold, 16 values each. A block's new keys and values are written by the wave of its first new token, which goes over the others once for the
+// largest value and once to write them. (The kernel above runs a wave for each head of a block here: 14.4 us for 64 single
+// tokens of 32 + 2 x 8 heads, this one 4.5; 11.1 where the keys of every block, 31 rows, are rounded anew.)
+template <class X, class Q>
+__global__ __launch_bounds__(256) void append8_few_kernel(Append8Args p) {
+    __shared__ __attribute__((aligned(16))) f2 cs_all[4][MAX_PAIRS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    f2* cs = cs_all[wave];
+    const int pairs = p.r.R / 2, shift = p.block == 16 ? 4 : p.block == 32 ? 5 : 6;
+    double f0 = 0, f1 = 0;
+    if (pairs) {
+        f0 = p.r.turns[min(lane, pairs - 1)];
+        f1 = p.r.turns[min(lane + 64, pairs - 1)];
+    }
+    const Place pl = place(p.r, lane);
+    const int per = p.r.D / 16;
+    // Workgroup y: slices of the query heads, of the key heads, of the value heads, four of them to its waves.
+    const int qs = (p.H + pl.heads - 1) / pl.heads, ks = (p.Hkv + pl.heads - 1) / pl.heads, slice = blockIdx.y * 4 + wave;
+    if (slice >= qs + 2 * ks) return;
+    const int kind = slice < qs ? 0 : slice < qs + ks ? 1 : 2, heads = kind ? p.Hkv : p.H;
+    const int h = (slice - (kind == 0 ? 0 : kind == 1 ? qs : qs + ks)) * pl.heads + pl.head;
+    const bool mine = pl.head < pl.heads && h < heads;
+    const int hc = mine ? h : 0;
+    const X* src = kind == 0 ? (const X*)p.q + hc * p.sqh : kind == 1 ? (const X*)p.k + hc * p.skh : (const X*)p.v + hc * p.svh;
+    const long st = kind == 0 ? p.sqt : kind == 1 ? p.skt : p.svt;
+    const void* w = kind == 0 ? p.qw : kind == 1 ? p.kw : nullptr;
+    const int token = blockIdx.x;
+    Raw8<X> raw_lo, raw_hi;
+    RawWeights raw_wl, raw_wh;
+    raw_lo.load(src + token * st + pl.at);
+    raw_hi.load(src + token * st + pl.to);
+    if (w) {
+        raw_wl.load(w, p.wtype, pl.at);
+        raw_wh.load(w, p.wtype, pl.to);
+    }
+    const Sequence q = find_sequence(p.starts, p.lengths, p.B, token, lane, [](int start, int) { return start; });
+    if (q.b >= p.B || token < q.first) return;
+    const int first = max(q.first, 0), end = min(max(q.end, first), p.T);
+    const int n = max(q.length, -(1 << 30)) - (end - token);  // the token's position
+    const int b0 = (n >> shift) << shift, entry = b0 >= 0 ? div_by(b0, p.S) : p.N;
+    int rows = 1;  // of the block's new ones, from this one on
+    if (kind) {
+        if (token > first && n > b0) return;  // not the block's first new token
+        rows = min(end - token, b0 + p.block - n);
+    }
+    int page = -1;
+    if (kind && entry < p.N) page = p.table[q.b * p.pitch + entry];
+    if (kind && (page < 0 || page >= p.P)) return;
+    const int o0 = n - b0;
+    signed char* codes = nullptr;
+    float *scale = nullptr, had = 0.f;
+    long cr = 0;
+    if (kind) {
+        const int row0 = b0 - entry * (int)p.S.d, part = row0 >> shift;
+        codes = kind == 1 ? p.kc + page * p.kpp + row0 * p.kpr + hc * p.kph : p.vc + page * p.vpp + row0 * p.vpr + hc * p.vph;
+        scale = kind == 1 ? p.ks + page * p.ksp + part * p.ksb + hc * p.ksh : p.vs + page * p.vsp + part * p.vsb + hc * p.vsh;
+        cr = kind == 1 ? p.kpr : p.vpr;
+        if (o0 > 0) had = *scale;
+    }
+    u32 top = 0;
+    NewScale s = {};
+    for (int it = 0, all = rows == 1 ? 1 : 2 * rows; it < all; it++) {
+        const int i = it < rows ? it : it - rows;
+        if (it > 0) {
+            raw_lo.load(src + (token + i) * st + pl.at);
+            raw_hi.load(src + (token + i) * st + pl.to);
+        }
+        f8 lo = raw_lo.values(), hi = raw_hi.values();
+        if (w) {
+            const float inv = inverse_rms(lo, hi, p.r.D, p.eps, per, lane);
+            lo = lo * inv * raw_wl.values(p.wtype);
+            hi = hi * inv * raw_wh.values(p.wtype);
+        }
+        if (pairs && kind < 2) {
+            __builtin_amdgcn_wave_barrier();  // the last token's angles have been read
+            make_angles(p.r, f0, f1, (double)(n + i), cs, lane);
+            f8 c, sn;
+            angles_of(pl, cs, c, sn);
+            if (pl.pair >= 0) turn(lo, hi, c, sn, p.r.interleaved);
+        }
+        if (kind == 0) {
+            if (mine) {
+                Q* dst = (Q*)p.qo + token * p.sot + h * p.soh;
+                store8(dst + pl.at, lo);
+                store8(dst + pl.to, hi);
+            }
+            return;
+        }
+        if (it < rows) top = max(top, largest(lo, hi));
+        if (it == rows - 1) {
+            s = new_scale(head_max(top, per, lane), had);
+            if (mine && o0 > 0 && s.finite && s.now != had) {
+                const float shrink = had * s.by;
+                for (int r = 0; r < o0; r += 8) {  // eight rows' loads ahead of their stores
+                    f8 a[8], z[8];
+#pragma unroll
+                    for (int x = 0; x < 8; x++) {
+                        const signed char* at = codes + min(r + x, o0 - 1) * cr;
+                        a[x] = load_codes(at + pl.at);
+                        z[x] = load_codes(at + pl.to);
+                    }
+#pragma unroll
+                    for (int x = 0; x < 8; x++)
+                        if (r + x < o0) {
+                            store_codes(codes + (r + x) * cr + pl.at, a[x] * shrink);
+                            store_codes(codes + (r + x) * cr + pl.to, z[x] * shrink);
+                        }
+                }
+            }
+            if (mine && lane % per == 0) *scale = s.now;
+        }
+        if (mine && it >= all - rows) {
+            store_codes(codes + (o0 + i) * cr + pl.at, s.finite ? over(lo, s.now, s.by) : (f8){});
+            store_codes(codes + (o0 + i) * cr + pl.to, s.finite ? over(hi, s.now, s.by) : (f8){});
+        }
     }
 }
 
@@ -231,12 +435,12 @@ template <class X>
 __global__ __launch_bounds__(256) void read8_kernel(Read8Args p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), token = blockIdx.x * 4 + wave;
     if (token >= p.T) return;
-    const int b = __builtin_amdgcn_readfirstlane(sequence_of(p.starts, p.B, token, lane));
+    const Sequence q = find_sequence(p.starts, p.lengths, p.B, token, lane, [](int start, int) { return start; });
     int page = -1, row = 0;
-    if (b < p.B && token >= p.starts[b]) {
-        const long n = (long)p.lengths[b] - p.starts[b + 1] + token;
+    if (q.b < p.B && token >= q.first) {
+        const long n = (long)q.length - q.end + token;
         const int entry = n >= 0 && n < 1L << 31 ? div_by((int)n, p.S) : p.N;
-        if (entry < p.N) page = p.table[b * p.pitch + entry], row = (int)n - entry * (int)p.S.d;
+        if (entry < p.N) page = p.table[q.b * p.pitch + entry], row = (int)n - entry * (int)p.S.d;
     }
     const bool there = page >= 0 && page < p.P;
     const int per = p.D / 16, chunks = p.Hkv * per;
@@ -1204,8 +1408,9 @@ int rda_paged_append_i8(const void* q, const void* k, const void* v, void* q_out
                      dims[11], dims[12], dims[13], dims[14], dims[15], dims[16], dims[17], dims[18], dims[19], dims[20], dims[21], dims[22], dims[23], dims[24],
                      dims[25], dims[26], dims[27], dims[28], dims[29], dims[30]};
     const long slots = T / block + 2 * B, heads = H + 2 * Hkv, together = 64 / block;
-    // Heads of a workgroup: as many as leave 2048 workgroups, so that angles are made for more than one head at a time.
-    long slice = (heads * slots / 2048 + together - 1) / together * together;
+    // Heads of a workgroup: as many as leave 1024 workgroups, so that angles are made for more than one head at a time (16384 tokens at 512 / 1024 / 2048 / 4096:
+    // 103 / 100 / 101 / 112 us).
+    long slice = (heads * slots / 1024 + together - 1) / together * together;
     if (slice < together) slice = together;
     if (slice > heads) slice = (heads + together - 1) / together * together;
     a.slice = (int)slice;
@@ -1216,6 +1421,12 @@ int rda_paged_append_i8(const void* q, const void* k, const void* v, void* q_out
         using X = decltype(x);
         const auto to = [&](auto y) {
             using Q = decltype(y);
+            // 64 sequences of 1 / 2 / 3 / 5 / 8 tokens: 4.5 / 7.3 / 10.0 / 15.1 / 25.1 us by tokens, 14.4 / 14.2 / 12.5 / 12.7 / 11.7 by blocks; 256 of one 5.3 and 38.6.
+            if (T < 4 * B) {
+                const int held = rows, slices = (int)((H + held - 1) / held + 2 * ((Hkv + held - 1) / held));
+                hipLaunchKernelGGL((append8_few_kernel<X, Q>), dim3((unsigned)T, (unsigned)((slices + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
+                return (int)hipGetLastError();
+            }
             return rows >= 16 ? launch_append8<X, Q, 1>(a, grid, lds, stream) : rows >= 8 ? launch_append8<X, Q, 2>(a, grid, lds, stream) : launch_append8<X, Q, 4>(a, grid, lds, stream);
         };
         return q_type == RDA_FP16 ? to(half_t{}) : to(bf16_t{});
