@@ -509,11 +509,11 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
     const int t = threadIdx.x, lane = t & 63, g = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int block = p.spread ? (int)blockIdx.x : work_block(p.grid);
-    Run run = find_run<MT, UK, AHEAD, 256>(p, (int*)smem, shared, block);
+    Run run = find_run<MT, UK, AHEAD, 256, true>(p, (int*)smem, shared, block);
     Cut cut = {};
 
     while (run.count > 0) {
-        const WorkTile w = uniform(make_tile<MT, UK, AHEAD>(p, run.b, run.j));
+        const WorkTile w = uniform(make_tile<MT, UK, AHEAD, true>(p, run.b, run.j));
         if (run.unit + run.count <= AHEAD) break;  // the next run's
         const bool begins = run.unit == 0, last_part = run.unit + run.count >= w.units, whole = begins && last_part;
         const int u0 = begins ? 0 : run.unit - AHEAD, u1 = min(w.units, run.unit + run.count) - AHEAD, n = u1 - u0;
@@ -570,7 +570,7 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
 
         if (w.hi > w.lo) {
             const int last = (w.hi - 1) / KG * KG;
-            auto key_of = [&](int i) __attribute__((always_inline)) { return w.lo + (u0 + i) * UK + wave * KT; };
+            auto key_of = [&](int i) __attribute__((always_inline)) { return w.lo + (u0 + i) * UK + (u0 + i >= w.head ? w.skip : 0) + wave * KT; };
             // Table entries of the lane's K rows and of its keys of V: of tile i + 1 until its loads of K, then of tile i + 2. What is waited for first is
             // loaded first: scales and table entries ahead of V, whose loads end a step.
             int kid, vid;
@@ -832,13 +832,13 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
     const int lane = threadIdx.x & 63, g = lane >> 5, lq = lane & 31;
     const int wave = uniform((int)(threadIdx.x >> 6));
     const int block = work_block(p.grid);
-    Run run = find_run<MT, UK, AHEAD, 256>(p, (int*)smem, (u32*)(smem + L::SHARED), block);
+    Run run = find_run<MT, UK, AHEAD, 256, true>(p, (int*)smem, (u32*)(smem + L::SHARED), block);
     int* flags = (int*)(smem + L::SHARED) + 256 + 8;  // a wave's: whether the cache lacks a page that it looked up
     Cut cut = {};
     const u32 smem_u = lds_addr(smem);
 
     while (run.count > 0) {
-        const WorkTile w = uniform(make_tile<MT, UK, AHEAD>(p, run.b, run.j));
+        const WorkTile w = uniform(make_tile<MT, UK, AHEAD, true>(p, run.b, run.j));
         if (run.unit + run.count <= AHEAD) break;  // the next run's
         const bool begins = run.unit == 0, last_part = run.unit + run.count >= w.units, whole = begins && last_part;
         const int u0 = begins ? 0 : run.unit - AHEAD, u1 = min(w.units, run.unit + run.count) - AHEAD, n = w.hi > w.lo ? u1 - u0 : 0;
@@ -846,8 +846,8 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
         const signed char* kbase = uniform((const signed char*)p.k + run.kvh * p.kph);
         const signed char* vbase = uniform((const signed char*)p.v + run.kvh * p.vph);
         const float *ksbase = uniform(p.ks + run.kvh * p.ksh), *vsbase = uniform(p.vs + run.kvh * p.vsh);
-        const int key_first = w.lo + u0 * UK, last16 = (w.hi - 1) & ~15;
-        auto key_of = [&](int i) __attribute__((always_inline)) { return key_first + i * UK; };
+        const int key_first = w.lo + u0 * UK, last16 = (w.hi - 1) & ~15, head = w.head - u0;  // key_first: were no keys skipped
+        auto key_of = [&](int i) __attribute__((always_inline)) { return key_first + i * UK + (i >= head ? w.skip : 0); };
         const int wr0 = w.r0 + 32 * wave;  // the wave's first row
         const bool active = wr0 <= w.r1;
         const int n0 = uniform(w.p0 + div_by(min(wr0, w.r1), p.G)), n1 = uniform(w.p0 + div_by(min(wr0 + 31, w.r1), p.G));
@@ -911,9 +911,9 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
             id = third;
             load(min(2, n - 1));
             fetch(min(3, n - 1));
-            const int e1 = div_by(min(key_first + n * UK, w.hi) - 1, p.S);
+            const int e1 = div_by(min(key_of(n - 1) + UK, w.hi) - 1, p.S);  // (with what is skipped)
             bool hole = false;
-            for (int e = div_by(key_first, p.S) + (int)threadIdx.x; e <= e1; e += 256) hole |= (u32)table[e] >= (u32)p.P;
+            for (int e = div_by(key_of(0), p.S) + (int)threadIdx.x; e <= e1; e += 256) hole |= (u32)table[e] >= (u32)p.P;
             hole = __any(hole);
             if (lane_again() == 0) flags[wave] = hole;
         }
@@ -1188,8 +1188,10 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
                 holes = uniform(flags[0] | flags[1] | flags[2] | flags[3]) != 0;
                 if (!holes) {
                     const int upto = min(w.hi, p.window > 0 ? n0 + 1 : max(n0 + 1, w.prefix));
-                    full0 = p.window > 0 ? max(n1 - p.window + UK - key_first, 0) / UK : 0;  // the first tile with key0 > n1 - window
-                    full1 = min(max((upto - key_first) / UK, 0), n);
+                    const int window_first = key_first + w.skip;
+                    full0 = p.window > 0 ? max(n1 - p.window + UK - window_first, 0) / UK : 0;  // the first tile with key0 > n1 - window
+                    if (w.skip) full0 = max(full0, head);
+                    full1 = min(max((upto - window_first) / UK, 0), n);
                 }
             }
             const int last = full1 - 3;  // pairs of full steps i, i + 1 up to it: tiles .. i + 2 are full

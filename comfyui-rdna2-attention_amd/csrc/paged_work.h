@@ -38,6 +38,7 @@ struct WorkTile {
     int p0;           // position of its token 0 (negative: the length is below the new tokens')
     int keys, prefix; // the sequence's cached keys; those every row sees
     int lo, hi, units;
+    int head, skip;   // SKIP: keys left out behind the first `head` units (a multiple of UK)
 };
 
 __device__ __forceinline__ int seq_rows(const PagedArgs& p, int b, int& first) {
@@ -51,7 +52,7 @@ __device__ __forceinline__ int seq_rows(const PagedArgs& p, int b, int& first) {
 // 16 rows at 0 / 1 / 2: 61 single tokens of ragged lengths 144.7 / 140.3 / 142.0, 32 sequences of 5 tokens 130 / 123 / 130. (Times of the code that
 // the choice was made on; the 24 heads take 190 now.)
 __host__ __device__ constexpr int ahead(int mt, bool mod) { return mt == 128 ? (mod ? 4 : 8) : 1; }
-template <int MT, int UK, int AHEAD>
+template <int MT, int UK, int AHEAD, bool SKIP = false>
 __device__ __forceinline__ WorkTile make_tile(const PagedArgs& p, int b, int j) {
     WorkTile t;
     t.rows = seq_rows(p, b, t.first);
@@ -66,7 +67,15 @@ __device__ __forceinline__ WorkTile make_tile(const PagedArgs& p, int b, int j) 
     // With a prefix a tile's keys begin at 0, and those between the prefix and the window are walked too, though no row sees them: over 65536 keys
     // with a window of 4096 a single token takes 14 us, with a prefix of 4 keys as well 59, a chunk of 512 tokens 78 and 513.
     t.lo = p.window > 0 && t.prefix == 0 && n0 >= p.window ? (n0 - p.window + 1) / UK * UK : 0;
-    t.units = AHEAD + max((t.hi - t.lo + UK - 1) / UK, 1);  // a tile without keys is one unit: its rows are written too
+    t.head = t.skip = 0;
+    if constexpr (SKIP) {
+        // SKIP leaves them out: the first `head` units are the prefix's, the others begin where the tile's first row's window does.
+        if (p.window > 0 && t.prefix > 0 && n0 >= p.window) {
+            t.head = (t.prefix + UK - 1) / UK;
+            t.skip = max((n0 - p.window + 1) / UK * UK - t.head * UK, 0);
+        }
+    }
+    t.units = AHEAD + max((t.hi - t.lo - t.skip + UK - 1) / UK, 1);  // a tile without keys is one unit: its rows are written too
     return t;
 }
 
@@ -78,7 +87,7 @@ __device__ __forceinline__ const X* uniform(const X* p) {
     return (const X*)((unsigned long long)(u32)uniform((int)(u >> 32)) << 32 | (u32)uniform((int)u));
 }
 __device__ __forceinline__ WorkTile uniform(WorkTile t) {
-    return {uniform(t.first), uniform(t.rows), uniform(t.r0), uniform(t.r1), uniform(t.p0), uniform(t.keys), uniform(t.prefix), uniform(t.lo), uniform(t.hi), uniform(t.units)};
+    return {uniform(t.first), uniform(t.rows), uniform(t.r0), uniform(t.r1), uniform(t.p0), uniform(t.keys), uniform(t.prefix), uniform(t.lo), uniform(t.hi), uniform(t.units), uniform(t.head), uniform(t.skip)};
 }
 
 // Inclusive sums over a wave's lanes, and over the workgroup's NT values (red holds NT / 64 sums).
@@ -137,7 +146,7 @@ __device__ __forceinline__ void begin_at_tile(Run& run) {
     }
 }
 // smem: B + 1 tile sums; shared: NT + 8 words.
-template <int MT, int UK, int AHEAD, int NT>
+template <int MT, int UK, int AHEAD, int NT, bool SKIP = false>
 __device__ __forceinline__ Run find_run(const PagedArgs& p, int* smem, u32* shared, int block) {
     const int t = threadIdx.x;
     u32* red = shared + NT;
@@ -156,7 +165,7 @@ __device__ __forceinline__ Run find_run(const PagedArgs& p, int* smem, u32* shar
                     if ((int)__shfl(end, b + o - 1) <= lane) b += o;
             }
             const int before = (int)__shfl(end - tiles, min(b, 63)), all = __builtin_amdgcn_readlane((int)end, 63);
-            const u32 units = lane < all ? make_tile<MT, UK, AHEAD>(p, b, lane - before).units : 0, upto = scan_wave(units);
+            const u32 units = lane < all ? make_tile<MT, UK, AHEAD, SKIP>(p, b, lane - before).units : 0, upto = scan_wave(units);
             const u32 s = cut_run(p, (u32)__builtin_amdgcn_readlane((int)upto, 63), block, run);
             if (run.count == 0) return run;
             const int at = uniform((int)__builtin_ctzll(__ballot(upto > s)));
@@ -201,7 +210,7 @@ __device__ __forceinline__ Run find_run(const PagedArgs& p, int* smem, u32* shar
     u32 units = 0;
     for (int i = t0; i < t1; i++) {
         while (smem[b + 1] <= i) b++;
-        units += make_tile<MT, UK, AHEAD>(p, b, i - smem[b]).units;
+        units += make_tile<MT, UK, AHEAD, SKIP>(p, b, i - smem[b]).units;
     }
     const u32 upto = scan_block<NT>(units, red), from = upto - units;
     if (t == NT - 1) red[4] = upto;
@@ -214,7 +223,7 @@ __device__ __forceinline__ Run find_run(const PagedArgs& p, int* smem, u32* shar
         int bb = bt;
         for (int i = t0; i < t1; i++) {
             while (smem[bb + 1] <= i) bb++;
-            const u32 n = make_tile<MT, UK, AHEAD>(p, bb, i - smem[bb]).units;
+            const u32 n = make_tile<MT, UK, AHEAD, SKIP>(p, bb, i - smem[bb]).units;
             if (s < at + n) {
                 shared[0] = bb;
                 shared[1] = i - smem[bb];

@@ -286,6 +286,20 @@ def test_scores(dev, type_, heads, kv, D, page, block, options):
     attend(dev, type_, D, heads, kv, page, block, seqs, seed=7, **o)
 
 
+@pytest.mark.parametrize("new,kv", [(1, 2), (5, 2), (40, 2), (150, 24)])
+@pytest.mark.parametrize("window,prefix", [(100, 4), (513, 40), (1, 1), (700, 300), (2000, 260)])
+def test_first_keys_and_a_window(dev, new, kv, window, prefix):
+    """A prefix of a few keys, a window, and none of the many keys between: single tokens and chunks at the end of long caches, in their midst, beside short ones
+    whose window reaches the prefix, and with pages missing in the prefix, between, and in the window."""
+    def edit(table):
+        table[1, 0], table[1, 10], table[1, 41] = -1, 1 << 20, -5
+
+    prefixes = torch.tensor([prefix, prefix, prefix, 0, prefix], dtype=torch.int32)
+    seqs = [(new, 3000), (new, 2700), (new, max(new, 350)), (new, 1500), (new, 1024)]
+    attend(dev, "fp16", 64, 2 * kv, kv, 64, 32, seqs, seed=21, table_edit=edit, window=window, prefix=prefixes)
+    attend(dev, "bf16", 128, kv, kv, 48, 16, seqs[:2], seed=22, window=window, prefix=prefixes[:2], softcap=20.0)
+
+
 @pytest.mark.parametrize("type_,kv", [("fp16", 2), ("bf16", 2), ("fp16", 24), ("bf16", 24)])
 def test_rows_that_see_nothing(dev, type_, kv):
     """Lengths below the new tokens (negative positions), lengths of zero, pages that the cache does not have, rows behind the last sequence."""
