@@ -799,8 +799,8 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
 // Tiles of 128 rows, as tiles_kernel of 16-bit caches (paged_attention.hip), whose tile layouts, step order and masks these are: 32 rows to each of four waves
 // that share 32-key tiles of K and V in LDS, there as fp16 codes. What differs:
 //
-// * A tile's codes come through registers: 16 (D = 64: 8) a thread of K and of V, loaded a step ahead, widened once for all four waves and written to the
-//   stage two tiles ahead. A wave's eight rows of a tile lie in one page.
+// * A tile's codes are copied to LDS as they are, widened once for all four waves, 16 (D = 64: 8) a thread of K and of V, and written to the stage two tiles ahead. A
+//   wave's eight rows of a tile lie in one page.
 // * Keys 0-15 and 16-31 of a tile have a scale each, and are the two halves in which P is made: the scale of K (times the row's factor) is the factor of the
 //   exponent's product anyway, and the scale of V, relative to the row's vm, goes into the exponent as its logarithm. l then gets a half's sum of
 //   rounded P times what takes that out again. So full steps do nothing more per score than those of a 16-bit cache.
@@ -814,7 +814,7 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
 template <int D>
 struct Tiles8Lds {
     using L = TilesLds<D>;
-    static constexpr int SCALES = L::BYTES, BYTES = SCALES + 3 * 2 * 16;  // {K's scale, V's, log2 of V's, 1 / V's} of each stage's two groups
+    static constexpr int RAW = (L::BYTES + 255) / 256 * 256, HALF = 32 * D, BYTES = RAW + 4 * HALF;  // codes of two tiles, K and V of each
 };
 
 template <class T, int D, bool MOD>
@@ -824,10 +824,7 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
     constexpr int CR = 1024 / ROW;  // rows of a store of the output
     using L = TilesLds<D>;
     typedef typename std::conditional<D == 128, u4v, u2v>::type raw_t;
-    typedef __attribute__((address_space(3))) f4 lds_f4_t;
-    // Loads in flight over LDS reads are of the global address space: flat ones would count as LDS accesses, which the reads wait for.
-    typedef __attribute__((address_space(1))) raw_t global_raw_t;
-    typedef __attribute__((address_space(1))) float global_float_t;
+    typedef __attribute__((address_space(1))) float global_float_t;  // (flat loads would count as LDS accesses too)
     extern __shared__ __attribute__((aligned(256))) char smem[];
     const int lane = threadIdx.x & 63, g = lane >> 5, lq = lane & 31;
     const int wave = uniform((int)(threadIdx.x >> 6));
@@ -852,65 +849,88 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
         const bool active = wr0 <= w.r1;
         const int n0 = uniform(w.p0 + div_by(min(wr0, w.r1), p.G)), n1 = uniform(w.p0 + div_by(min(wr0 + 31, w.r1), p.G));
 
-        // Copies: the wave's rows 8 wave .. + 7 of a tile, eight lanes to a row. Rows behind the sequence's end in its last 16 keys are read as they are, later
-        // ones as those 16.
-        raw_t raw_k, raw_v;
-        float raw_ks, raw_vs;
-        int id = 0;  // the wave's table entry of the tile to be loaded next
-        const unsigned long long k_lane = (unsigned long long)(lane >> 3) * p.kpr + (lane & 7) * CB, v_lane = (unsigned long long)(lane >> 3) * p.vpr + (lane & 7) * CB;
-        auto group_of = [&](int i) __attribute__((always_inline)) { return min(key_of(i) + 16 * (wave >> 1), last16); };
-        auto fetch = [&](int i) __attribute__((always_inline)) { id = table[div_by(group_of(i), p.S)]; };
-        auto load = [&](int i) __attribute__((always_inline)) {
-            const int key = group_of(i), row = key - div_by(key, p.S) * (int)p.S.d;
-            const u32 at = (u32)uniform(id), page = at < (u32)p.P ? at : 0;
-            raw_k = *(const global_raw_t*)(kbase + row_at(page, p.kpp, (u32)row + 8 * (wave & 1), p.kpr) + k_lane);
-            raw_v = *(const global_raw_t*)(vbase + row_at(page, p.vpp, (u32)row + 8 * (wave & 1), p.vpr) + v_lane);
-            raw_ks = *(const global_float_t*)(ksbase + row_at(page, p.ksp, (u32)row >> p.shift, p.ksb));
-            raw_vs = *(const global_float_t*)(vsbase + row_at(page, p.vsp, (u32)row >> p.shift, p.vsb));
+        // What the tiles from `base` on need, tile base + lane in a lane, read anew every ~58 of them: the page of the wave's rows, and of keys 0-15 and 16-31 the
+        // scale of K (NaN if it is not finite), log2 of that of V, and its reciprocal.
+        int base = 0, ids = 0;
+        float ks0 = 0.f, ks1 = 0.f, lv0 = 0.f, lv1 = 0.f, iv0 = 0.f, iv1 = 0.f;
+        auto refresh = [&](int from) __attribute__((always_inline)) {
+            base = from;
+            const int key = key_of(min(from + lane_again(), n - 1)), k0 = min(key, last16), k1 = min(key + 16, last16), e0 = div_by(k0, p.S), e1 = div_by(k1, p.S);
+            const u32 t0 = (u32)table[e0], t1 = (u32)table[e1], p0 = t0 < (u32)p.P ? t0 : 0, p1 = t1 < (u32)p.P ? t1 : 0;
+            const u32 r0 = (u32)(k0 - e0 * (int)p.S.d) >> p.shift, r1 = (u32)(k1 - e1 * (int)p.S.d) >> p.shift;
+            ids = (int)(wave >> 1 ? p1 : p0);
+            ks0 = *(const global_float_t*)(ksbase + row_at(p0, p.ksp, r0, p.ksb));
+            ks1 = *(const global_float_t*)(ksbase + row_at(p1, p.ksp, r1, p.ksb));
+            const float v0 = *(const global_float_t*)(vsbase + row_at(p0, p.vsp, r0, p.vsb)), v1 = *(const global_float_t*)(vsbase + row_at(p1, p.vsp, r1, p.vsb));
+            ks0 = ks0 <= FLT_TOP ? ks0 : __builtin_nanf("");
+            ks1 = ks1 <= FLT_TOP ? ks1 : __builtin_nanf("");
+            lv0 = __builtin_amdgcn_logf(v0);
+            lv1 = __builtin_amdgcn_logf(v1);
+            iv0 = __builtin_amdgcn_rcpf(v0);
+            iv1 = __builtin_amdgcn_rcpf(v1);
+        };
+        auto of_tile = [&](float x, int i) __attribute__((always_inline)) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i - base)); };
+
+        // Codes come by direct copies, two tiles ahead of where they are widened: the wave's rows 8 wave .. + 7 of tile t to the half t % 2 of RAW, 16 bytes a lane
+        // (D = 64: of half the lanes), and each thread widens 16 (8) of its own wave's codes for the stages that all four read. Rows behind the sequence's end in
+        // its last 16 keys are read as they are, later ones as those 16. Past the run's last tile that one is copied again, so that there are always two copies
+        // behind those that are waited for.
+        using LDS = Tiles8Lds<D>;
+        constexpr int LANES = D / 16;  // of a row
+        const u32 k_off = (u32)(lane / LANES) * p.kpr + (lane % LANES) * 16, v_off = (u32)(lane / LANES) * p.vpr + (lane % LANES) * 16;
+        auto issue = [&](int t) __attribute__((always_inline)) {
+            const int tile = min(t, n - 1), key = min(key_of(tile) + 16 * (wave >> 1), last16), row = key - div_by(key, p.S) * (int)p.S.d + 8 * (wave & 1);
+            const u32 page = (u32)__builtin_amdgcn_readlane(ids, tile - base);
+            const signed char *k = uniform(kbase + row_at(page, p.kpp, (u32)row, p.kpr)), *v = uniform(vbase + row_at(page, p.vpp, (u32)row, p.vpr));
+            const char* to = smem + LDS::RAW + (t & 1) * 2 * LDS::HALF + wave * (8 * D);
+            if (D == 128 || lane_again() < 32) {
+                dma16(k, k_off, to);
+                dma16(v, v_off, to + LDS::HALF);
+            }
         };
         const int my_row = 8 * wave + (lane >> 3);
-        auto put = [&](u32 st) __attribute__((always_inline)) {
-            const int k_swizzle = D == 128 ? my_row & 15 : my_row >> 1 & 7, v_swizzle = D == 128 ? (my_row & 3) << 2 | (my_row & 1) : (my_row >> 1 & 1) << 2;
-            char *kd = smem + st + my_row * ROW, *vd = kd + L::V;
-#pragma unroll
-            for (int c = 0; c < CB / 8; c++) {
-                const int chunk = (lane & 7) * (CB / 8) + c;
-                const u2v k0 = widen4(raw_k[2 * c]), k1 = widen4(raw_k[2 * c + 1]), v0 = widen4(raw_v[2 * c]), v1 = widen4(raw_v[2 * c + 1]);
-                *(u4v*)(kd + ((chunk ^ k_swizzle) << 4)) = (u4v){k0[0], k0[1], k1[0], k1[1]};
-                *(u4v*)(vd + ((chunk ^ v_swizzle) << 4)) = (u4v){v0[0], v0[1], v1[0], v1[1]};
-            }
-            const float ks = raw_ks <= FLT_TOP ? raw_ks : __builtin_nanf("");
-            *(f4*)(smem + Tiles8Lds<D>::SCALES + st / L::TILE * 32 + (wave >> 1) * 16) = (f4){ks, raw_vs, __builtin_amdgcn_logf(raw_vs), __builtin_amdgcn_rcpf(raw_vs)};
+        u32 k_to = (u32)(my_row * ROW + (((lane & 7) * (CB / 8) ^ (D == 128 ? my_row & 15 : my_row >> 1 & 7)) << 4));
+        u32 v_to = (u32)(L::V + my_row * ROW + (((lane & 7) * (CB / 8) ^ (D == 128 ? (my_row & 3) << 2 | (my_row & 1) : (my_row >> 1 & 1) << 2)) << 4));
+        auto raw_of = [&](int t, int half) __attribute__((always_inline)) {
+            return *(const raw_t*)(smem + LDS::RAW + (t & 1) * 2 * LDS::HALF + half * LDS::HALF + wave * (8 * D) + lane_again() * CB);
         };
-        // Step i's part: tile i + 2 to its stage, tile i + 3's loads, tile i + 4's table entry.
+        // Chunk c of 16 bytes in the stages: half h of it, the second one with the store of both. The two chunks of a thread differ by the last bit of their place.
+        u2v wide;
+        auto put_half = [&](const raw_t& raw, int c, int h, u32 to) __attribute__((always_inline)) {
+            const u2v x = widen4(raw[2 * c + h]);
+            if (h == 0) wide = x;
+            else *(u4v*)(smem + (to ^ (u32)(c << 4))) = (u4v){wide[0], wide[1], x[0], x[1]};
+        };
+        // Step i's part: tile i + 2 to its stage, tile i + 4's copies.
         auto advance = [&](int i, u32 st2) __attribute__((always_inline)) {
-            if (i + 2 < n) put(st2);
-            if (i + 3 < n) load(i + 3);
-            if (i + 4 < n) fetch(i + 4);
+            if (i + 5 - base > 63) refresh(i);
+            wait_copies_but<2>();
+            if (i + 2 < n) {
+                const raw_t k = raw_of(i + 2, 0), v = raw_of(i + 2, 1);
+#pragma unroll
+                for (int x = 0; x < CB / 4; x++) put_half(k, x / 2, x % 2, st2 + k_to);
+#pragma unroll
+                for (int x = 0; x < CB / 4; x++) put_half(v, x / 2, x % 2, st2 + v_to);
+            }
+            issue(i + 4);
         };
         bool holes = false;  // whether the cache lacks any page of the run's part
         if (n > 0) {
-            fetch(0);
-            const int first = id;
-            fetch(min(1, n - 1));
-            const int second = id;
-            fetch(min(2, n - 1));
-            const int third = id;
-            id = first;
-            load(0);
-            const raw_t k0 = raw_k, v0 = raw_v;
-            const float ks0 = raw_ks, vs0 = raw_vs;
-            id = second;
-            load(min(1, n - 1));
-            const raw_t k1 = raw_k, v1 = raw_v;
-            const float ks1 = raw_ks, vs1 = raw_vs;
-            raw_k = k0, raw_v = v0, raw_ks = ks0, raw_vs = vs0;
-            put(0);
-            raw_k = k1, raw_v = v1, raw_ks = ks1, raw_vs = vs1;
-            put(L::TILE);
-            id = third;
-            load(min(2, n - 1));
-            fetch(min(3, n - 1));
+            refresh(0);
+            wait_copies();
+            issue(0);
+            issue(1);
+            wait_copies();
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const raw_t k = raw_of(t, 0), v = raw_of(t, 1);
+#pragma unroll
+                for (int x = 0; x < CB / 4; x++) put_half(k, x / 2, x % 2, t * L::TILE + k_to);
+#pragma unroll
+                for (int x = 0; x < CB / 4; x++) put_half(v, x / 2, x % 2, t * L::TILE + v_to);
+            }
+            issue(2);
+            issue(3);
             const int e1 = div_by(min(key_of(n - 1) + UK, w.hi) - 1, p.S);  // (with what is skipped)
             bool hole = false;
             for (int e = div_by(key_of(0), p.S) + (int)threadIdx.x; e <= e1; e += 256) hole |= (u32)table[e] >= (u32)p.P;
@@ -1016,9 +1036,6 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
                 }
                 return seen;
             };
-            auto scales_of = [&](u32 st, int half) __attribute__((always_inline)) {
-                return *(const lds_f4_t*)(size_t)(smem_u + (u32)(Tiles8Lds<D>::SCALES + half * 16) + st / L::TILE * 32);
-            };
             // What x is times in the softmax's exponent, besides the scales: capped scores without a bias stay the -1 / (1 + 2^e) of their tanh (see capped), times
             // 2 cap. (From HIGH_CAP on, 2 cap passes 4096 and they are made whole first, as large scores are, below.)
             const float scale = MOD && p.cap > 0.f && !p.slopes && p.cap < HIGH_CAP ? 2.f * p.cap : 1.f;
@@ -1100,8 +1117,7 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
             // Returns whether full steps may follow; half1: what the second half's P is times.
             auto begin_tile = [&](int i, u32 st, u32 seen, bool masked, float& half1) __attribute__((always_inline)) {
                 qk(st, sa, no_hook);
-                const f4 t0 = scales_of(st, 0), t1 = scales_of(st, 1);
-                const float c0 = by * t0[0], c1 = by * t1[0];
+                const float c0 = by * of_tile(ks0, i), c1 = by * of_tile(ks1, i), vs0 = __builtin_amdgcn_rcpf(of_tile(iv0, i)), vs1 = __builtin_amdgcn_rcpf(of_tile(iv1, i));
                 if constexpr (MOD) bias(sa, key_of(i), c0, c1);
 #pragma unroll
                 for (int r = 0; r < 16; r++) sa[r] *= MOD ? scale : r < 8 ? c0 : c1;
@@ -1124,7 +1140,7 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
                 const f2 h = both_halves(mx);
                 mx = fmaxf(h[0], h[1]);
                 const bool see0 = seen & 0xffffu, see1 = seen >> 16;
-                const float v0 = see0 && t0[1] <= FLT_TOP ? t0[1] : 0.f, v1 = see1 && t1[1] <= FLT_TOP ? t1[1] : 0.f, vx = fmaxf(v0, v1);
+                const float v0 = see0 && vs0 <= FLT_TOP ? vs0 : 0.f, v1 = see1 && vs1 <= FLT_TOP ? vs1 : 0.f, vx = fmaxf(v0, v1);
                 if (__any(mx > m + 2.f || vx > vm)) {
                     const float mn = mx > m + 2.f ? mx : m, vn = vx > vm ? fminf(2.f * vx, FLT_TOP) : vm, a = __builtin_amdgcn_exp2f(m - mn);
                     const float b = a * (vm / vn);
@@ -1136,7 +1152,7 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
                     for (int d = 0; d < DT; d++) o[d] *= b;
                 }
                 l_old = l;
-                if ((see0 && !(t0[1] <= FLT_TOP)) || (see1 && !(t1[1] <= FLT_TOP))) l = l_old = __builtin_nanf("");
+                if ((see0 && !(vs0 <= FLT_TOP)) || (see1 && !(vs1 <= FLT_TOP))) l = l_old = __builtin_nanf("");
                 const float unit = 512.f / vm;
                 half1 = v1 * unit;
                 exps_plain(sa, pf[0], v0 * unit);
@@ -1144,9 +1160,9 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
                 sum0 = 0.f;
                 back0 = 0.f;
                 factor1 = 1.f;
-                const float d1 = t1[2] - lvm + LIFT_TILES;
+                const float d1 = of_tile(lv1, i) - lvm + LIFT_TILES;
                 add1 = d1 - m;
-                back1 = vm * (1.f / 512.f) * t1[3];
+                back1 = vm * (1.f / 512.f) * of_tile(iv1, i);
                 return !large && !__any(!(d1 <= LIFT_TILES && d1 >= LIFT_TILES + LEAST_RATIO));
             };
             // A step of the full tiles: tile i's scores are in s, its P's first half in pf[0] and sum0 (or in l); tile i + 1 is full
@@ -1155,21 +1171,34 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
             // scales of V do not suit vm, the step ends before the product (false), and the tile is taken again by a plain step.
             auto beside = [](int x) __attribute__((always_inline)) { return x % (KS / 4) == KS / 4 - 1; };
             auto full_step = [&](int i, u32 st, u32 st1, u32 st2, const float (&s)[16], float (&nxt)[16]) __attribute__((always_inline)) {
-                advance(i, st2);
-                const f4 t0 = scales_of(st1, 0), t1 = scales_of(st1, 1);
+                // Tile i + 2 (there is one) goes to its stage beside the products, half a chunk beside every second one: their vector work and the products overlap.
+                wait_copies_but<2>();
+                const raw_t now_k = raw_of(i + 2, 0);
+                auto put_beside = [&](const raw_t& raw, int x, u32 to) __attribute__((always_inline)) {
+                    if (x % 2 == 0 && x / 2 < CB / 4) put_half(raw, x / 4, x / 2 & 1, to);
+                };
                 sum1 = 0.f;
-                qk(st1, nxt, [&](int x) { if (beside(x)) exps(s + 8, x / (KS / 4), pf[1], factor1, add1, sum1); });
-                const float d0 = t0[2] - lvm, d1 = t1[2] - lvm;
-                if (__builtin_expect(__any(!(sum0 + sum1 <= MOST_TILES && fmaxf(d0, d1) <= 0.f && d0 >= LEAST_RATIO && d1 >= LEAST_RATIO)), 0)) return false;
-                const float c0 = by * t0[0], c1 = by * t1[0];
+                qk(st1, nxt, [&](int x) {
+                    if (beside(x)) exps(s + 8, x / (KS / 4), pf[1], factor1, add1, sum1);
+                    put_beside(now_k, x, st2 + k_to);
+                });
+                const raw_t now_v = raw_of(i + 2, 1);
+                const float d0 = of_tile(lv0, i + 1) - lvm, d1 = of_tile(lv1, i + 1) - lvm;
+                if (__builtin_expect(__any(!(sum0 + sum1 <= MOST_TILES && fmaxf(d0, d1) <= 0.f && d0 >= LEAST_RATIO && d1 >= LEAST_RATIO)), 0)) {
+#pragma unroll
+                    for (int x = 0; x < CB / 4; x++) put_half(now_v, x / 2, x % 2, st2 + v_to);
+                    issue(i + 4);
+                    return false;
+                }
+                const float c0 = by * of_tile(ks0, i + 1), c1 = by * of_tile(ks1, i + 1);
                 bias(nxt, key_of(i + 1), c0, c1);
                 l = __builtin_fmaf(sum0, back0, __builtin_fmaf(sum1, back1, l));
                 l_old = l;
                 const float factor0 = MOD ? scale : c0, add0 = d0 + LIFT_TILES - m, unit = vm * (1.f / 512.f);
                 factor1 = MOD ? scale : c1;
                 add1 = d1 + LIFT_TILES - m;
-                back0 = unit * t0[3];
-                back1 = unit * t1[3];
+                back0 = unit * of_tile(iv0, i + 1);
+                back1 = unit * of_tile(iv1, i + 1);
                 sum0 = 0.f;
                 u4v pn;
                 pv(st, [&](int x) {
@@ -1177,8 +1206,10 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
                         exps(nxt, x / (KS / 4), pn, factor0, add0, sum0);
                         asm volatile("" : "+v"(pn), "+v"(sum0));
                     }
+                    put_beside(now_v, x, st2 + v_to);
                 });
                 pf[0] = pn;
+                issue(i + 4);
                 __syncthreads();
                 return true;
             };
@@ -1218,6 +1249,7 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
                         full = full && may;
                         bool done = true, taken = true;  // taken: the tile's maximum is
                         while (full) {
+                            if (i + 6 - base > 63) refresh(i);
                             taken = false;
                             done = full_step(i, st, st1, st2, sa, sb);
                             if (!done) break;
@@ -1257,6 +1289,7 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
             }
         }
 
+        wait_copies();  // those behind the last tile
         // The rows turn around in LDS (chunk c of row r at c ^ (r & 15) or, of 8, c ^ (r & 7)) so that a store covers whole rows.
         if (active) {
             const int ln = lane_again(), lg = ln >> 5, lr = ln & 31;
@@ -1376,8 +1409,11 @@ static int launch_append8(const Append8Args& a, dim3 grid, size_t lds, void* str
 
 template <class T, int D>
 static int launch_tiles8(const Attn8Args& a, void* stream) {
+    static std::atomic<size_t> done[2][RDA_MAX_DEVICES];
+    const bool mod = a.cap > 0.f || a.slopes;
+    if (const int e = ensure_dynamic_lds(mod ? (const void*)tiles8_kernel<T, D, true> : (const void*)tiles8_kernel<T, D, false>, Tiles8Lds<D>::BYTES, done[mod])) return e;
     const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.grid), dim3(256), Tiles8Lds<D>::BYTES, (hipStream_t)stream, a); };
-    a.cap > 0.f || a.slopes ? launch(tiles8_kernel<T, D, true>) : launch(tiles8_kernel<T, D, false>);
+    mod ? launch(tiles8_kernel<T, D, true>) : launch(tiles8_kernel<T, D, false>);
     if (const hipError_t e = hipGetLastError()) return (int)e;
     hipLaunchKernelGGL((merge8_kernel<T, D, 128>), dim3(a.grid, 8), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
