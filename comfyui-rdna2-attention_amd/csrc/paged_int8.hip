@@ -496,9 +496,12 @@ __device__ __forceinline__ f4 product16(const u4v& a, const u4v& b, const f4& c)
 // of two that its scores' factor takes back (a bf16 value less than 2^-28 of its row's largest may lose bits). P is what the scale of V leaves of
 // it relative to the largest scale that the row has met, vm: O is in units of vm, and rescaled when that grows, as when the maximum moves. l sums P
 // before both.
+//
+// (Tiles of 32 rows take 32 keys a wave: with 64 their registers do not suffice.)
+__host__ __device__ constexpr int rows8_steps(int mb) { return mb == 1 ? 2 : 1; }  // 32 keys each
 template <class T, int D, int MB, bool MOD>
 __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
-    constexpr int KT = 64, KG = 16, UK = 4 * KT, MT = 16 * MB, AHEAD = ahead(MT, MOD);
+    constexpr int NS = rows8_steps(MB), KT = 32 * NS, KG = 8 * NS, UK = 4 * KT, MT = 16 * MB, AHEAD = ahead(MT, MOD);
     constexpr int KC = D / 64;  // 16-byte vectors of a lane's part of a K row
     constexpr int VC = D / 16;  // consecutive dims of a lane's part of a V row
     constexpr int OP = D + 4;   // pitch of a row of O in LDS
@@ -579,7 +582,7 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
                 kid = table[div_by(min(key0 + KG * (r >> 2), last), p.S)];
                 vid = table[div_by(min(key0 + KG * g, last), p.S)];
             };
-            u4v kf[4][KC];
+            u4v kf[KG / 4][KC];
             vvec vf[KG];
             float ks, vs, ks2, vs2;  // the scales of the lane's keys, of tile i and of tile i + 1
             u32 vrow, vpage;         // where V of tile i + 1 lies
@@ -593,7 +596,7 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
                 vs2 = vsbase[row_at(vpage, p.vsp, vrow >> p.shift, p.vsb)];
                 const signed char* src = kbase + row_at((u32)kid < (u32)p.P ? (u32)kid : 0, p.kpp, (u32)row, p.kpr) + 16 * g;
 #pragma unroll
-                for (int c = 0; c < 4; c++)
+                for (int c = 0; c < KG / 4; c++)
 #pragma unroll
                     for (int x = 0; x < KC; x++) kf[c][x] = *(const u4v*)(src + (unsigned long long)(4 * c) * p.kpr + 64 * x);
             };
@@ -614,7 +617,7 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
                 if (!(ks <= FLT_TOP)) ks = __builtin_nanf("");
                 float s[MB][KG];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < KG / 4; c++) {
                     u4v a[KC][2];
 #pragma unroll
                     for (int x = 0; x < KC; x++)
@@ -658,7 +661,7 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
                 }
                 u32 see[MB];
 #pragma unroll
-                for (int m = 0; m < MB; m++) see[m] = 0xffffu;
+                for (int m = 0; m < MB; m++) see[m] = (1u << KG) - 1;
                 if (!all) {
 #pragma unroll
                     for (int m = 0; m < MB; m++) {
@@ -673,7 +676,7 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
                     }
                 }
                 // Softmax.
-                u4v pf[MB][2];
+                u4v pf[MB][NS];
                 const bool finite = vs <= FLT_TOP;
 #pragma unroll
                 for (int m = 0; m < MB; m++) {
@@ -699,7 +702,7 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
 #pragma unroll
                     for (int e = 0; e < KG; e++) l_[m] += pw[e];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
+                    for (int h = 0; h < NS; h++) {
                         h8 x;
 #pragma unroll
                         for (int e = 0; e < 8; e++) x[e] = (half_t)(pw[8 * h + e] * f);
@@ -712,7 +715,7 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
 #pragma unroll
                 for (int j = 0; j < VC; j++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
+                    for (int h = 0; h < NS; h++) {
                         u4v a;
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
@@ -1525,7 +1528,7 @@ int rda_paged_attn_i8(const void* q, void* out, const void* k_codes, const void*
     if (!(a.scale >= 1.2e-38f && a.scale <= 3e38f && a.cap <= 3e38f)) return RDA_ERR_INVALID;
     a.window = window;
     // No more workgroups than units there can be: a short table of few sequences needs none that finds no work.
-    const long least = plan.mt == 128 ? 32 : 256, units = (T * (H / Hkv) / plan.mt + B) * ((N * S + least - 1) / least + ahead(plan.mt, false)) * Hkv;
+    const long least = plan.mt == 128 ? 32 : 128 * rows8_steps(plan.mt / 16), units = (T * (H / Hkv) / plan.mt + B) * ((N * S + least - 1) / least + ahead(plan.mt, false)) * Hkv;
     const int most = softcap > 0.f || slopes ? 512 : plan.grid;
     a.grid = (int)(units < most ? units : most);
     a.runs = make_div(a.grid);
