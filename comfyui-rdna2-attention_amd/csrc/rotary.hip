@@ -105,8 +105,8 @@ __global__ __launch_bounds__(ROW_WAVES * 64) void append_kernel(AppendArgs p) {
     }
     const int b = __builtin_amdgcn_readfirstlane(sequence_of(p.starts, p.B, token, lane));
     if (b >= p.B || token < p.starts[b]) return;
-    const long n = (long)p.lengths[b] - p.starts[b + 1] + token;  // below 2^31 in size
-    const int block = n >= 0 ? div_by((int)n, p.S) : p.N, row = (int)n - block * (int)p.S.d;
+    const long n = (long)p.lengths[b] - p.starts[b + 1] + token;  // 2^31 and more where starts fall below 0 and lengths are large
+    const int block = n >= 0 && n < 1L << 31 ? div_by((int)n, p.S) : p.N, row = (int)n - block * (int)p.S.d;
     int page = -1;
     if (block < p.N) page = p.table[b * p.pitch + block];
     make_angles(p.r, f0, f1, (double)n, cs, lane);
