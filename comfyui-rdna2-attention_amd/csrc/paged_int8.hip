@@ -342,7 +342,7 @@ __global__ __launch_bounds__(256) void append8_few_kernel(Append8Args p) {
     int rows = 1;  // of the block's new ones, from this one on
     if (kind) {
         if (token > first && n > b0) return;  // not the block's first new token
-        rows = min(end - token, b0 + p.block - n);
+        rows = min(end - token, p.block - (n - b0));
     }
     int page = -1;
     if (kind && entry < p.N) page = p.table[q.b * p.pitch + entry];
@@ -1508,7 +1508,7 @@ int rda_paged_attn_i8(const void* q, void* out, const void* k_codes, const void*
     // Units of a KV head in 32 bits, whatever the lengths.
     if ((T * (H / Hkv) / plan.mt + B) * (N * S / 32 + 1 + ahead(plan.mt, false)) >= 1L << 32) return RDA_ERR_INVALID;
     for (int i : {14, 15, 17, 18, 20, 21, 23, 24})
-        if (dims[i] < 0 || dims[i] >= 1L << 32) return RDA_ERR_INVALID;
+        if (dims[i] < 0 || dims[i] >= (i == 15 || i == 18 ? 1L << 28 : 1L << 32)) return RDA_ERR_INVALID;  // eight rows of codes: 32-bit offsets
     Attn8Args a;
     a.q = q; a.o = out; a.k = k_codes; a.v = v_codes;
     a.ks = k_scales; a.vs = v_scales;

@@ -247,11 +247,11 @@ def _append_quantized(cache, batch, k, v, rotary, q, q_out, norm):
         k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
     qw, kw = (None, None) if norm is None else (norm.q, norm.k)
     _no_gradient("append", qw, kw)
-    key = (cache.sizes, batch.sizes, k.dtype, k.shape, k.stride(), v.dtype, v.shape, v.stride(), 0 if rotary is None else rotary.dim, None if kw is None else kw.shape,
+    key = (cache.sizes, batch.sizes, k.dtype, k.shape, k.stride(), v.dtype, v.shape, v.stride(), 0 if rotary is None else rotary.dim, None if kw is None else (qw.dtype, qw.shape, kw.dtype, kw.shape),
            None if q is None else (q.dtype, q.shape, q.stride()), None if q_out is None else (q_out.dtype, q_out.shape, q_out.stride()))
     dims = _append_quantized_sizes.get(key)
     if dims is None:
-        k, v, q, dims = _check_append_quantized(cache, batch, k, v, rotary, q, q_out, kw, key)
+        k, v, q, dims = _check_append_quantized(cache, batch, k, v, rotary, q, q_out, norm, key)
     same_device("append", kc, ks, batch._table, k, v, q, q_out, qw, kw, None if rotary is None else rotary.turns)
     if q_out is not None and q_out.data_ptr() % 16:
         raise ValueError(QUANTIZED_Q_OUT_ERROR)
@@ -273,7 +273,7 @@ def _append_quantized(cache, batch, k, v, rotary, q, q_out, norm):
 QUANTIZED_Q_OUT_ERROR = "append's q_out has q's shape, is fp16 or bf16 over a QuantizedCache, with a contiguous last dimension and rows on 16-byte boundaries, each its own"
 
 
-def _check_append_quantized(cache, batch, k, v, rotary, q, q_out, weight, key):
+def _check_append_quantized(cache, batch, k, v, rotary, q, q_out, norm, key):
     """(k, v and q, copied where the kernel cannot address them; the size arguments) of an append to a QuantizedCache, or ValueError."""
     kc, vc, ks, vs = cache.k, cache.v, cache.k_scales, cache.v_scales
     _, _, Hkv, D = kc.shape
@@ -281,8 +281,8 @@ def _check_append_quantized(cache, batch, k, v, rotary, q, q_out, weight, key):
         raise ValueError(f"append takes k and v as (tokens, {Hkv}, {D}) of one type: fp16, bf16 or fp32")
     if D > MAX_HEAD or (rotary is not None and rotary.dim > D):
         raise ValueError(f"append takes heads of at most {MAX_HEAD} values, and no more rotated ones than these")
-    if weight is not None and weight.shape != (D,):
-        raise ValueError(f"append takes a norm of {D} weights")
+    if norm is not None and not (norm.q.shape == norm.k.shape == (D,) and norm.q.dtype == norm.k.dtype and norm.k.dtype in TYPES):
+        raise ValueError(f"append takes a norm of {D} weights, of one type: fp16, bf16 or fp32")
     T, H = k.shape[0], 0
     if q is not None:
         H = q.shape[1] if q.dim() == 3 else 0
@@ -338,8 +338,8 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     softcap > 0, softcap tanh(scale q.k / softcap), to 7e-7 of softcap, or, in fp32 and from a softcap of 1420 on, to 2e-6 of the score (so a cap
     far above the scores changes nothing); with slopes (fp32, one per head, finite), less slopes[h] |n - j|. heads is a multiple of the
     cache's KV heads, which they share in order. A token that sees nothing gets 0. Returns out (q's shape, not overlapping q; rows of no
-    sequence left as they were), or a new tensor, with those rows 0. Keys between a prefix and the window cost time as if they were seen. A call takes
-    up to 102 MB of workspace from torch's allocator."""
+    sequence left as they were), or a new tensor, with those rows 0. Keys between a prefix and the window cost time as if they were seen (over a
+    QuantizedCache none). A call takes up to 102 MB of workspace from torch's allocator."""
     kc, vc = cache._k, cache._v
     _no_gradient("attention", q, slopes, out)
     fill = out is None
@@ -409,8 +409,8 @@ def _check_attention(cache, batch, q, out, slopes, prefix, key):
     if prefix is not None and (prefix.dtype != torch.int32 or prefix.numel() != B or not prefix.is_contiguous()):
         raise ValueError(f"attention takes prefix as {B} contiguous int32 values")
     scales = (*cache.k_scales.stride(), *cache.v_scales.stride()) if quantized else ()
-    if max(*kc.stride()[:2], *vc.stride()[:2], *scales) >= 2 ** 32:
-        raise ValueError("attention takes a cache whose pages and rows are less than 2^32 values apart")
+    if max(*kc.stride()[:2], *vc.stride()[:2], *scales) >= 2 ** 32 or (quantized and max(kc.stride(1), vc.stride(1)) >= 2 ** 28):
+        raise ValueError("attention takes a cache whose pages and rows (of a QuantizedCache: rows 2^28) are less than 2^32 values apart")
     if T * (H // Hkv) >= 2 ** 31:
         raise ValueError("attention takes fewer than 2^31 rows of tokens and heads per KV head")
     ready = T == 0 or rows_ready(q)

@@ -222,7 +222,10 @@ class HeadNorm:
             raise ValueError("HeadNorm takes contiguous weights on 16-byte boundaries")
         if not 0.0 <= eps < 1e30:
             raise ValueError("HeadNorm takes an eps that is not negative")
-        self.q, self.k, self.eps = q, k, float(eps)
+        self._q, self._k, self.eps = q, k, float(eps)
+
+    q = property(lambda self: self._q, doc="The weights of the query heads.")
+    k = property(lambda self: self._k, doc="The weights of the key heads.")
 
 
 _norm_sizes, _norm_back_sizes, _norm_workspaces = Sizes(), Sizes(), {}
@@ -248,7 +251,8 @@ def norm_rotate(q, k, positions, rotary, norm):
     """q (tokens, heads, D) and k (tokens, KV heads, D), or both with a batch dimension before them as rotate takes, normed head by head and turned by
     `positions`, in one launch: (q, k), new contiguous tensors of their type. A head x becomes the turn of w x / sqrt(mean(x^2) + norm.eps), w norm.q or
     norm.k, in 32 bits, rounded once. Any strides with a contiguous last dimension. Gradients of q, k and the weights are carried where they are
-    recorded, those of the weights summed in 32 bits and rounded once; the same inputs give the same bits."""
+    recorded, those of the weights summed in 32 bits and rounded once; the same inputs give the same bits. (A backward pass is captured as torch's own are: with
+    no graph of the same leaves alive that was recorded outside of the capture.)"""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or norm.q.requires_grad or norm.k.requires_grad):
         return _NormTurn.apply(q, k, norm.q, norm.k, positions, rotary, norm.eps)
     return _norm_rotate(q, k, positions, rotary, norm.q, norm.k, norm.eps)
@@ -256,10 +260,10 @@ def norm_rotate(q, k, positions, rotary, norm):
 
 def _norm_rotate(q, k, positions, rotary, q_weight, k_weight, eps):
     q, k, positions = _aligned(q), _aligned(k), positions.contiguous()
-    key = (q.dtype, q.shape, q.stride(), k.dtype, k.shape, k.stride(), positions.dtype, positions.shape, rotary.dim, q_weight.shape)
+    key = (q.dtype, q.shape, q.stride(), k.dtype, k.shape, k.stride(), positions.dtype, positions.shape, rotary.dim, q_weight.dtype, q_weight.shape, k_weight.dtype, k_weight.shape)
     dims = _norm_sizes.get(key)
     if dims is None:
-        q, k, dims = _check_norm_rotate(q, k, positions, rotary, q_weight, key)
+        q, k, dims = _check_norm_rotate(q, k, positions, rotary, q_weight, k_weight, key)
     same_device("norm_rotate", q, k, positions, q_weight, k_weight, rotary.turns)
     q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(k, memory_format=torch.contiguous_format)
     if positions.numel() == 0:
@@ -311,8 +315,10 @@ def _norm_dims(q, k, rotary):
     return [B, L, q.shape[-2], k.shape[-2], q.shape[-1], rotary.dim, *_strides(q), *_strides(k)]
 
 
-def _check_norm_rotate(q, k, positions, rotary, weight, key):
+def _check_norm_rotate(q, k, positions, rotary, weight, k_weight, key):
     """(q and k, copied where the kernel cannot address them; the size arguments) of a norm_rotate call, or ValueError."""
+    if weight.dtype not in TYPES or k_weight.dtype != weight.dtype or k_weight.shape != weight.shape:
+        raise ValueError("norm_rotate takes weights of one type (fp16, bf16 or fp32) and size")
     D = weight.shape[0]
     if q.dim() not in (3, 4) or q.dtype not in TYPES or q.shape[-1] != D or not 0 < q.shape[-2] <= 65535 or not rotary.dim <= D <= MAX_HEAD:
         raise ValueError(f"norm_rotate takes q as (tokens, heads, D) or (batch, length, heads, D) in fp16, bf16 or fp32, D the weights' {D}, from {rotary.dim} "

@@ -135,7 +135,7 @@ def test_entry_points_reject_before_any_launch():
 
     for bad in (dict(T=0), dict(H=7), dict(H=0), dict(Hkv=0), dict(D=96), dict(B=0), dict(B=8193), dict(N=0), dict(P=0), dict(S=0), dict(S=40), dict(block=48), dict(N=1 << 26),
                 dict(sqt=1028), dict(soh=132), dict(kr=248), dict(vh=8), dict(q=a + 8), dict(ws=a + 8), dict(type_=2), dict(type_=-1), dict(window=-1), dict(softcap=-1.0),
-                dict(softcap=float("nan")), dict(T=1 << 30), dict(scale=0.0), dict(scale=float("nan")), dict(scale=1e-39), dict(kp=1 << 32), dict(ksb=1 << 32), dict(vsp=-4)):
+                dict(softcap=float("nan")), dict(T=1 << 30), dict(scale=0.0), dict(scale=float("nan")), dict(scale=1e-39), dict(kp=1 << 32), dict(kr=1 << 28), dict(vr=1 << 28), dict(ksb=1 << 32), dict(vsp=-4)):
         assert attn(**bad) == 1, bad
     assert lib.rda_paged_attn_i8_workspace(4, 2, 8, 2, 128, 1) > 0 and lib.rda_paged_attn_i8_workspace(4, 2, 8, 2, 128, 2) == 0
 
