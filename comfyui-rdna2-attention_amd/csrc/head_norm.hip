@@ -9,6 +9,9 @@
 // Both passes move each value once, as rotate does, and are laid out like it (rotary.hip): a wave takes a token and a slice of one tensor's heads, its lanes
 // make the token's angles once, a head's sum crosses the D / 16 lanes that hold it. The weights' gradient stays in a lane's registers over all of the
 // tokens that its wave takes; workgroups leave their sums of it in a workspace, which a second launch adds up in a fixed order.
+//
+// 8192 tokens of 32 + 8 heads of 128 bf16: forward 36 us (168 MB, 4.7 TB/s), backward 45 (252 MB, 5.6 TB/s) and 4 for the weights' sums. One token: 4.3 us, a launch's and three
+// accesses' latency.
 #include "rotary.h"
 
 #define BACK_PASSES 2  // heads per lane and token of the backward pass: two hold a head's values and its gradient's

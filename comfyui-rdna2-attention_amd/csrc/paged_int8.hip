@@ -145,6 +145,9 @@ __device__ __forceinline__ u32 head_max(u32 x, int per, int lane) {
 // and `slice` heads (queries, keys, values in this order): it makes the angles of the block's new tokens once, and takes 16 tokens of a head to a wave, block / 16
 // waves to a head. A block whose first tokens are older keeps a scale at least as large as it had; where the scale grows the older codes are
 // rounded anew to it by the same workgroup, which alone writes the block of that head.
+//
+// The loads of the next heads go out ahead of the arithmetic on these. 16384 tokens of 32 + 2 x 8 heads of 128 fp16 with norms, 369 MB: 90 us, 4.1 TB/s, vector work
+// 44% of the cycles; 3 ragged chunks of fp32, 43 MB: 13.7 us.
 template <class X, class Q, int PS>
 __global__ __launch_bounds__(256) void append8_kernel(Append8Args p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -430,7 +433,8 @@ struct Read8Args {
 };
 
 // Keys and values of a batch's rows as the values that their codes stand for: a wave takes a row, its lanes 16 values each. Rows of no
-// sequence, and of positions that the cache does not have, are 0.
+// sequence, and of positions that the cache does not have, are 0. Bound by memory: 24 sequences, 160 MB, 32 us, 4.9 TB/s; 257 rows 4 us, three accesses to memory one
+// after the other.
 template <class X>
 __global__ __launch_bounds__(256) void read8_kernel(Read8Args p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), token = blockIdx.x * 4 + wave;
@@ -495,9 +499,15 @@ __device__ __forceinline__ f4 product16(const u4v& a, const u4v& b, const f4& c)
 // scale of K and of V. All products are of fp16: codes are exact there, and a row of q is brought to a largest magnitude of 2^14 to 2^15 by a power
 // of two that its scores' factor takes back (a bf16 value less than 2^-28 of its row's largest may lose bits). P is what the scale of V leaves of
 // it relative to the largest scale that the row has met, vm: O is in units of vm, and rescaled when that grows, as when the maximum moves. l sums P
-// before both.
+// before both: P and its sum are then off by roundings of P to fp16 that do not cancel, up to 1.3 times the rms error of a plain form that keeps P in 32 bits (fp16
+// outputs; with bf16 ones the output's rounding hides it).
 //
-// (Tiles of 32 rows take 32 keys a wave: with 64 their registers do not suffice.)
+// Bound by the keys and values read: 64 single tokens over 8192 keys (8 KV heads of 128), 1.08 GB, 206 us, 5.2 TB/s, in pages of whole heads 188, 5.7, where a large sum
+// reads at 6.0; vector work, half of it widening codes, takes 33% of the cycles. Loads are issued in the order in which they are waited for: each wait is then for
+// its own loads alone, with the next tile's 16 KiB (of K, then of V) behind them.
+//
+// Tiles of 32 rows take 32 keys a wave (64 spill registers: 32 sequences of 5 tokens over 4096 keys 85 us, 75 so); tiles of 16 rows 64 (with 32: 213 us for 64 x 8192, and
+// at three workgroups a CU 219, where 61 ragged sequences gain 5%).
 __host__ __device__ constexpr int rows8_steps(int mb) { return mb == 1 ? 2 : 1; }  // 32 keys each
 template <class T, int D, int MB, bool MOD>
 __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
@@ -809,6 +819,11 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
 //   rounded P times what takes that out again. So full steps do nothing more per score than those of a 16-bit cache.
 // * Where a scale of V is above the row's vm, or below it by more than 2^8, or is not finite, the step is not a full one: the plain steps sum P before it
 //   is scaled, and move vm (to twice the scale: O is then seldom rescaled).
+//
+// A chunk of 2048 tokens over 14336 keys, 32 heads over 8 of 128: 618 to 627 us, 0.82 to 0.83 PFLOP/s, 64% of a library product of 8192^3; the 16-bit cache's kernel takes 568. Products take 37% of the
+// cycles and vector work 56% (ten instructions a product, where the 16-bit kernel has five: widening, scales), which add up on a SIMD. Two workgroups a CU: at three the registers
+// spill (1920 us). Widening at the start of a step 655, beside the products and two tiles ahead 619; V read ahead of the look at P no faster. With D = 64, half the
+// products beside the same vector work, 414 (16-bit: 312).
 #define TILES8_WGS(D, MOD) ((D) == 64 && !(MOD) ? 3 : 2)
 #define LIFT_TILES 9.f        // P stands 2^9 vs / vm above 2^(x - m), of which at most 2^2 are in a plain step
 #define MOST_TILES 32768.f    // of a full step's sum of P in a lane, so that no P is above it
@@ -893,7 +908,7 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
         };
         const int my_row = 8 * wave + (lane >> 3);
         u32 k_to = (u32)(my_row * ROW + (((lane & 7) * (CB / 8) ^ (D == 128 ? my_row & 15 : my_row >> 1 & 7)) << 4));
-        u32 v_to = (u32)(L::V + my_row * ROW + (((lane & 7) * (CB / 8) ^ (D == 128 ? (my_row & 3) << 2 | (my_row & 1) : (my_row >> 1 & 1) << 2)) << 4));
+        u32 v_to = (u32)(L::V + my_row * ROW + (((lane & 7) * (CB / 8) ^ (D == 128 ? (my_row & 3) << 2 : (my_row >> 1 & 1) << 2)) << 4));
         auto raw_of = [&](int t, int half) __attribute__((always_inline)) {
             return *(const raw_t*)(smem + LDS::RAW + (t & 1) * 2 * LDS::HALF + half * LDS::HALF + wave * (8 * D) + lane_again() * CB);
         };
@@ -999,7 +1014,7 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
             u32 v_base;
             {
                 const int sg = lane & 15, vr = 4 * g + (sg >> 2), c = 2 * (lane >> 4 & 1) + (sg >> 1 & 1);
-                v_base = smem_u + (u32)(L::V + vr * ROW + (sg & 1) * 8 + ((c ^ (D == 128 ? (vr & 3) << 2 | (vr & 1) : (vr >> 1 & 1) << 2)) << 4));
+                v_base = smem_u + (u32)(L::V + vr * ROW + (sg & 1) * 8 + ((c ^ (D == 128 ? (vr & 3) << 2 : (vr >> 1 & 1) << 2)) << 4));
             }
             asm volatile("" : "+v"(k_base), "+v"(v_base));
 
