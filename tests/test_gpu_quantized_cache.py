@@ -6,7 +6,7 @@ import torch
 from comfyui_rdna2_attention_amd import paged_kv, rotary
 from helpers import gen
 from paged_reference import rounding, sequences, turned
-from quantized_reference import attended_quantized, check_appended, norm_turned, values
+from quantized_reference import attended_quantized, check_appended, norm_turned, normed, values
 from test_gpu_paged import BATCHES, batch_of, check
 
 pytestmark = pytest.mark.gpu
@@ -70,6 +70,51 @@ def test_append(dev, type_, out, normed, page, block, D, heads, kv):
     check(q_out[:T], rq, qoff, ot)
     check_appended(kd.cpu(), ksd.cpu(), rk, koff, k0, ks0, table, starts, lengths, block)
     check_appended(vd.cpu(), vsd.cpu(), rv, voff, v0, vs0, table, starts, lengths, block)
+
+
+def test_append_many_sequences_of_chunks(dev):
+    """More sequences than a wave has lanes, each of several tokens; norms without a turn; then the same tokens again, which changes nothing."""
+    g = gen(51)
+    B, page, kv, D = 300, 32, 1, 64
+    new = torch.randint(0, 24, (B,), generator=g)
+    seqs = [(int(n), int(n) + int(c)) for n, c in zip(new, torch.randint(0, 70, (B,), generator=g))]
+    table, starts, lengths, pages = batch_of(seqs, page, g)
+    T = int(starts[-1])
+    assert T >= 4 * B
+    q, k, v = (torch.randn(T, h, D, generator=g).bfloat16() for h in (2, kv, kv))
+    norm = rotary.HeadNorm(*((1 + 0.3 * torch.randn(D, generator=g)).to(dev) for _ in range(2)), eps=1e-5)
+    k0, v0, ks0, vs0 = codes_of(pages, page, kv, D, 16, g)
+    kd, vd, ksd, vsd = on(dev, k0, v0, ks0, vs0)
+    cache, batch = paged_kv.QuantizedCache(kd, vd, ksd, vsd), paged_kv.Batch(*on(dev, table, starts, lengths))
+    out = paged_kv.append(cache, batch, k.to(dev), v.to(dev), q=q.to(dev), q_out=torch.empty(T, 2, D, dtype=torch.float16, device=dev), norm=norm)
+    (rk, krel), (rq, qrel) = normed(k, norm.k.cpu(), 1e-5), normed(q, norm.q.cpu(), 1e-5)
+    check(out, rq, rq.abs() * qrel, torch.float16)
+    check_appended(kd.cpu(), ksd.cpu(), rk, rk.abs() * krel, k0, ks0, table, starts, lengths, 16)
+    check_appended(vd.cpu(), vsd.cpu(), v.double(), v.double() * 0, v0, vs0, table, starts, lengths, 16)
+    before = [t.clone() for t in (kd, vd, ksd, vsd)]
+    paged_kv.append(cache, batch, k.to(dev), v.to(dev), norm=norm)
+    assert all(torch.equal(a, b) for a, b in zip(before, (kd, vd, ksd, vsd)))
+
+
+@pytest.mark.parametrize("type_", ["fp16", "fp32"])
+def test_appends_by_tokens_and_by_blocks_agree(dev, type_):
+    """Steps of few tokens a sequence and of many take different launches: the same codes, scales and queries, bit for bit."""
+    g = gen(52)
+    t, kv, D, page = TYPES[type_], 3, 128, 32
+    rot, norm = rotary.Rotary(64, device=dev), rotary.HeadNorm(*((1 + 0.3 * torch.randn(D, generator=g)).to(dev) for _ in range(2)))
+    seqs = [(3, 40), (1, 1), (3, 33), (2, 64), (3, 90)]
+    table, starts, lengths, pages = batch_of(seqs, page, g)
+    T = int(starts[-1])
+    q, k, v = (torch.randn(T, h, D, generator=g).to(t).to(dev) for h in (6, kv, kv))
+    first = on(dev, *codes_of(pages, page, kv, D, 16, g, spread=1.0))
+    results = []
+    for spare in (0, 40):  # tokens of no sequence behind: the mean decides
+        c = [x.clone() for x in first]
+        pad = lambda x: torch.cat((x, x[:1].expand(spare, *x.shape[1:]))) if spare else x  # noqa: E731
+        out = torch.zeros(T + spare, 6, D, dtype=torch.float16, device=dev)
+        paged_kv.append(paged_kv.QuantizedCache(*c), paged_kv.Batch(*on(dev, table, starts, lengths)), pad(k), pad(v), rotary=rot, q=pad(q), q_out=out, norm=norm)
+        results.append((*c, out[:T]))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
 @pytest.mark.parametrize("block", [16, 32, 64])
@@ -298,6 +343,26 @@ def test_first_keys_and_a_window(dev, new, kv, window, prefix):
     seqs = [(new, 3000), (new, 2700), (new, max(new, 350)), (new, 1500), (new, 1024)]
     attend(dev, "fp16", 64, 2 * kv, kv, 64, 32, seqs, seed=21, table_edit=edit, window=window, prefix=prefixes)
     attend(dev, "bf16", 128, kv, kv, 48, 16, seqs[:2], seed=22, window=window, prefix=prefixes[:2], softcap=20.0)
+
+
+@pytest.mark.parametrize("type_,D,options", [("fp16", 128, {}), ("bf16", 64, dict(softcap=30.0)), ("fp16", 64, dict(window=9000)), ("bf16", 128, dict(window=12000, prefix=70))])
+def test_long_runs(dev, type_, D, options):
+    """Runs of more tiles than their lanes hold scales and pages of (64): 64 KV heads, two tiles of 128 rows each, over 17000 keys; eight of the heads against 64 bits."""
+    g = gen(53)
+    t, kv, page, block, new, length = TYPES[type_], 64, 64, 32, 150, 17000
+    table, starts, lengths, pages = batch_of([(new, length)], page, g)
+    k, v, ks, vs = on(dev, *codes_of(pages, page, kv, D, block, g, spread=0.6))
+    q = torch.randn(new, kv, D, generator=g).to(t)
+    q = torch.where(q.abs() < 2.0 ** -10, 0, q)
+    o = dict(options)
+    if "prefix" in o:
+        o["prefix"] = torch.tensor([o["prefix"]], dtype=torch.int32)
+    got = paged_kv.attention(paged_kv.QuantizedCache(k, v, ks, vs), paged_kv.Batch(*on(dev, table, starts, lengths)), q.to(dev),
+                             **{n: x.to(dev) if isinstance(x, torch.Tensor) else x for n, x in o.items()})
+    for h in range(0, kv, 8):
+        one = slice(h, h + 1)
+        ref, off, _ = attended_quantized(q[:, one], *(x[:, :, one].cpu() for x in (k, v, ks, vs)), table, starts, lengths, **o)
+        check(got[:, one], ref, off, t)
 
 
 @pytest.mark.parametrize("type_,kv", [("fp16", 2), ("bf16", 2), ("fp16", 24), ("bf16", 24)])
