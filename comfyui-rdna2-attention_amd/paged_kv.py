@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from .hip_attention import Kernels
-from .rotary import MAX_HEAD, MAX_TOKENS, TYPES, Sizes, distinct, rows_ready, same_device, vector_rows, written
+from .rotary import MAX_HEAD, MAX_TOKENS, TYPES, WEIGHTS_ERROR, Sizes, distinct, rows_ready, same_device, vector_rows, written
 
 HEADS = (64, 128)  # head dims of `attention`
 MAX_SEQUENCES = 8192
@@ -247,7 +247,10 @@ def _append_quantized(cache, batch, k, v, rotary, q, q_out, norm):
         k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
     qw, kw = (None, None) if norm is None else (norm.q, norm.k)
     _no_gradient("append", qw, kw)
-    key = (cache.sizes, batch.sizes, k.dtype, k.shape, k.stride(), v.dtype, v.shape, v.stride(), 0 if rotary is None else rotary.dim, None if kw is None else (qw.dtype, qw.shape, kw.dtype, kw.shape),
+    if kw is not None and (qw.data_ptr() | kw.data_ptr()) % 16:  # (their data may have been replaced)
+        raise ValueError(WEIGHTS_ERROR)
+    key = (cache.sizes, batch.sizes, k.dtype, k.shape, k.stride(), v.dtype, v.shape, v.stride(), 0 if rotary is None else rotary.dim,
+           None if kw is None else (qw.dtype, qw.shape, qw.stride(), kw.dtype, kw.shape, kw.stride()),
            None if q is None else (q.dtype, q.shape, q.stride()), None if q_out is None else (q_out.dtype, q_out.shape, q_out.stride()))
     dims = _append_quantized_sizes.get(key)
     if dims is None:
@@ -283,6 +286,8 @@ def _check_append_quantized(cache, batch, k, v, rotary, q, q_out, norm, key):
         raise ValueError(f"append takes heads of at most {MAX_HEAD} values, and no more rotated ones than these")
     if norm is not None and not (norm.q.shape == norm.k.shape == (D,) and norm.q.dtype == norm.k.dtype and norm.k.dtype in TYPES):
         raise ValueError(f"append takes a norm of {D} weights, of one type: fp16, bf16 or fp32")
+    if norm is not None and not (norm.q.is_contiguous() and norm.k.is_contiguous()):
+        raise ValueError(WEIGHTS_ERROR)
     T, H = k.shape[0], 0
     if q is not None:
         H = q.shape[1] if q.dim() == 3 else 0

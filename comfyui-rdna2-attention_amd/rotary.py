@@ -211,6 +211,9 @@ def _check_rotate(x, positions, rotary, out, key):
     return x, _rotate_sizes.keep(key, values) if ready else _lib.long_array(values)
 
 
+WEIGHTS_ERROR = "HeadNorm takes contiguous weights on 16-byte boundaries"
+
+
 class HeadNorm:
     """RMS norms of a layer's query and key heads: q and k are their weights, (D,) each, contiguous, of one type (fp16, bf16 or fp32), kept as they are -- a
     training step's updates of them are seen --, eps what is added to a head's mean square."""
@@ -219,7 +222,7 @@ class HeadNorm:
         if q.dim() != 1 or q.shape != k.shape or q.dtype not in TYPES or k.dtype != q.dtype or q.device != k.device or q.numel() == 0 or q.numel() % 16:
             raise ValueError("HeadNorm takes weights q and k as (D,) of one type (fp16, bf16 or fp32) on one device, D a multiple of 16")
         if not (rows_ready(q) and rows_ready(k)):
-            raise ValueError("HeadNorm takes contiguous weights on 16-byte boundaries")
+            raise ValueError(WEIGHTS_ERROR)
         if not 0.0 <= eps < 1e30:
             raise ValueError("HeadNorm takes an eps that is not negative")
         self._q, self._k, self.eps = q, k, float(eps)
@@ -260,7 +263,10 @@ def norm_rotate(q, k, positions, rotary, norm):
 
 def _norm_rotate(q, k, positions, rotary, q_weight, k_weight, eps):
     q, k, positions = _aligned(q), _aligned(k), positions.contiguous()
-    key = (q.dtype, q.shape, q.stride(), k.dtype, k.shape, k.stride(), positions.dtype, positions.shape, rotary.dim, q_weight.dtype, q_weight.shape, k_weight.dtype, k_weight.shape)
+    if (q_weight.data_ptr() | k_weight.data_ptr()) % 16:  # (their data may have been replaced)
+        raise ValueError(WEIGHTS_ERROR)
+    key = (q.dtype, q.shape, q.stride(), k.dtype, k.shape, k.stride(), positions.dtype, positions.shape, rotary.dim,
+           q_weight.dtype, q_weight.shape, q_weight.stride(), k_weight.dtype, k_weight.shape, k_weight.stride())
     dims = _norm_sizes.get(key)
     if dims is None:
         q, k, dims = _check_norm_rotate(q, k, positions, rotary, q_weight, k_weight, key)
@@ -317,8 +323,10 @@ def _norm_dims(q, k, rotary):
 
 def _check_norm_rotate(q, k, positions, rotary, weight, k_weight, key):
     """(q and k, copied where the kernel cannot address them; the size arguments) of a norm_rotate call, or ValueError."""
-    if weight.dtype not in TYPES or k_weight.dtype != weight.dtype or k_weight.shape != weight.shape:
+    if weight.dtype not in TYPES or k_weight.dtype != weight.dtype or k_weight.shape != weight.shape or weight.dim() != 1:
         raise ValueError("norm_rotate takes weights of one type (fp16, bf16 or fp32) and size")
+    if not (weight.is_contiguous() and k_weight.is_contiguous()):
+        raise ValueError(WEIGHTS_ERROR)
     D = weight.shape[0]
     if q.dim() not in (3, 4) or q.dtype not in TYPES or q.shape[-1] != D or not 0 < q.shape[-2] <= 65535 or not rotary.dim <= D <= MAX_HEAD:
         raise ValueError(f"norm_rotate takes q as (tokens, heads, D) or (batch, length, heads, D) in fp16, bf16 or fp32, D the weights' {D}, from {rotary.dim} "

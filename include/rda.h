@@ -264,7 +264,7 @@ int rda_paged_append_i8(const void* q, const void* k, const void* v, void* q_out
 int rda_paged_read_i8(const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, const int* table, const int* starts,
                       const int* lengths, void* k_out, void* v_out, int type, const long* dims, void* stream);
 
-/* Attention as rda_paged_attn over a quantized cache, q and out of `type` (0 or 1). dims: T, H, Hkv, D, B, N, table pitch, P, S, block, strides (t, h) of q, of out,
+/* Attention as rda_paged_attn over a quantized cache, q and out of `type` (0 or 1), its rows of codes fewer than 2^28 values apart. dims: T, H, Hkv, D, B, N, table pitch, P, S, block, strides (t, h) of q, of out,
  * and of codes and scales as above. */
 size_t rda_paged_attn_i8_workspace(long T, long B, long H, long Hkv, long D, int type);
 int rda_paged_attn_i8(const void* q, void* out, const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales, const int* table,

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from comfyui_rdna2_attention_amd import _lib, rotary
+from comfyui_rdna2_attention_amd import _lib, paged_kv, rotary
 from helpers import gen
 from paged_reference import rounding
 from quantized_reference import norm_turned, norm_turned_back
@@ -62,6 +62,22 @@ def test_refusals():
     x, w = torch.zeros(1, 1, 16).expand(many, 1, 16), torch.ones(16)
     with pytest.raises(ValueError, match="at most"):
         rotary.norm_rotate(x, x, torch.zeros(1, dtype=torch.int32).expand(many), rotary.Rotary(16, device="cpu"), rotary.HeadNorm(w, w))
+
+
+def test_replaced_weights():
+    """Weights whose data is replaced after the norm was made: by values that the kernels could not address."""
+    rot, n = rotary.Rotary(32, device="cpu"), torch.zeros(4, dtype=torch.int32)
+    q, k = torch.zeros(4, 3, 64), torch.zeros(4, 2, 64)
+    cache, batch = paged_kv.QuantizedCache.empty(2, 32, 2, 64, device="cpu"), paged_kv.Batch(n[:1].view(1, 1), torch.tensor([0, 4], dtype=torch.int32), n[:1] + 4)
+    for which in (0, 1):
+        for data, match in ((torch.ones(65)[1:], "16-byte"), (torch.ones(128)[::2], "contiguous"), (torch.ones(64).half(), "one type"), (torch.ones(48), "takes"), (torch.ones(64), "current GPU")):
+            weights = torch.ones(64), torch.ones(64)
+            norm = rotary.HeadNorm(*weights)
+            weights[which].data = data
+            with pytest.raises(ValueError, match=match):
+                rotary.norm_rotate(q, k, n, rot, norm)
+            with pytest.raises(ValueError, match=match):
+                paged_kv.append(cache, batch, k, k, norm=norm)
 
 
 def test_entry_points_reject_before_any_launch():
