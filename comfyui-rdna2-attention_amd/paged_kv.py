@@ -64,7 +64,7 @@ class QuantizedCache:
     """The pages of a layer's keys and values in 8 bits: k and v int8 codes (pages, page size, KV heads, D), D a multiple of 16, in any order of dimensions in
     memory but the last, which is contiguous, rows on 16-byte boundaries; k_scales and v_scales fp32 (pages, page size / block, KV heads), any strides: a value is
     its code times the scale of its block of 16, 32 or 64 consecutive tokens and KV head. Scales are not negative; one that is not finite stands for
-    a block of NaN. `empty` makes the four tensors.
+    a block of NaN (to attention, of V, one above 2^126 may; append's are below 2^122). `empty` makes the four tensors.
 
     append sets a block's scale to the largest magnitude of its new values / 127. A block that is filled by several appends keeps the largest scale so far:
     where it grows, the older codes are rounded to it once more, so that a value written once is off by half a scale at most (and 2^-16 of it), each
@@ -342,7 +342,8 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     one per sequence) also those j < prefix[b], ahead of it or behind the window. Scores are scale q.k (scale None: D^-0.5); with
     softcap > 0, softcap tanh(scale q.k / softcap), to 7e-7 of softcap, or, in fp32 and from a softcap of 1420 on, to 2e-6 of the score (so a cap
     far above the scores changes nothing); with slopes (fp32, one per head, finite), less slopes[h] |n - j|. heads is a multiple of the
-    cache's KV heads, which they share in order. A token that sees nothing gets 0. Returns out (q's shape, not overlapping q; rows of no
+    cache's KV heads, which they share in order. A token that sees nothing gets 0. Weighted sums are held in fp32 before they are divided: values that pass its range when
+    added up over the keys seen give infinities. Returns out (q's shape, not overlapping q; rows of no
     sequence left as they were), or a new tensor, with those rows 0. Keys between a prefix and the window cost time as if they were seen (over a
     QuantizedCache none). A call takes up to 102 MB of workspace from torch's allocator."""
     kc, vc = cache._k, cache._v

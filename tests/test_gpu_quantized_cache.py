@@ -427,6 +427,35 @@ def test_scales_far_apart(dev, new, kv):
     attend(dev, "bf16", D, kv, kv, page, block, [(new, 300)], seed=19, edit=sized(1e-20, 1e-25))
 
 
+@pytest.mark.parametrize("type_", ["fp16", "bf16"])
+@pytest.mark.parametrize("new,kv,D", [(1, 2, 64), (1, 2, 128), (3, 8, 128), (130, 24, 128), (130, 24, 64)])
+def test_scales_of_zero(dev, type_, new, kv, D):
+    """Blocks whose scales are 0, as `empty` makes them, at the start, between others and at the end: their keys' scores and their values are 0. A cache of nothing
+    but those. Sequences that share their first pages, and a table whose entries past a length are anything."""
+    page, block = 32, 16
+
+    def nothing(which, *at):
+        def edit(k, v, ks, vs, table):
+            for n in at:
+                for s in which(ks, vs):
+                    s[int(table[0, n // page]), n % page // block] = 0.0
+        return edit
+
+    for at in ((0, 16), (100, 116, 200), (299,), tuple(range(0, 300, 16))):
+        attend(dev, type_, D, kv, kv, page, block, [(new, 300), (new, 260)], seed=24, edit=nothing(lambda ks, vs: (vs,), *at))
+        attend(dev, type_, D, kv, kv, page, block, [(new, 300), (new, 260)], seed=25, edit=nothing(lambda ks, vs: (ks,), *at))
+        attend(dev, type_, D, kv, kv, page, block, [(new, 300), (new, 260)], seed=26, edit=nothing(lambda ks, vs: (ks, vs), *at), softcap=20.0)
+    cache = paged_kv.QuantizedCache.empty(12, page, kv, D, block, dev)
+    batch = paged_kv.Batch(*on(dev, torch.arange(10, dtype=torch.int32)[None], torch.tensor([0, new], dtype=torch.int32), torch.tensor([300], dtype=torch.int32)))
+    assert not paged_kv.attention(cache, batch, torch.ones(new, kv, D, dtype=TYPES[type_], device=dev)).any()
+
+    def shared(table):
+        table[1, :8] = table[0, :8]
+        table[1, 9:] = 2 ** 31 - 1  # (its length ends in page 8)
+
+    attend(dev, type_, D, kv, kv, page, block, [(new, 300), (new, 270)], seed=27, table_edit=shared)
+
+
 def test_rows_of_queries_far_from_one(dev):
     """Rows of q of 10^-30 to 10^30 beside one another, with zeros; a row that is not finite is NaN alone."""
     g = gen(20)
