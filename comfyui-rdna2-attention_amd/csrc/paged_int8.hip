@@ -535,39 +535,6 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
         const signed char* vbase = (const signed char*)p.v + run.kvh * p.vph;
         const float *ksbase = p.ks + run.kvh * p.ksh, *vsbase = p.vs + run.kvh * p.vsh;
 
-        // Q as the B operand: lane (g, r) has values 64 x + 16 g .. + 15 of row r, as it has of the K rows.
-        u4v qf[MB][KC][2];
-        int pos[MB], pre[MB];
-        float slope[MB], by[MB];  // by: what a product is times, but the key's scale
-#pragma unroll
-        for (int m = 0; m < MB; m++) {
-            const int row = w.r0 + 16 * m + r, rc = min(row, w.r1), token = div_by(rc, p.G), head = run.kvh * (int)p.G.d + rc - token * (int)p.G.d;
-            const T* src = (const T*)p.q + (long)(w.first + token) * p.sqt + head * p.sqh;
-            f8 x[KC][2];
-            float top = 0.f;
-#pragma unroll
-            for (int c = 0; c < KC; c++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    x[c][h] = load8(src + 64 * c + 16 * g + 8 * h);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[c][h][e]));
-                }
-            top = rows_max(top);
-            const int up = top > 0.f && top <= FLT_TOP ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-            by[m] = ldexpf(p.scale, -up);
-#pragma unroll
-            for (int c = 0; c < KC; c++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[c][h][e] = ldexpf(x[c][h][e], up);
-                    qf[m][c][h] = __builtin_bit_cast(u4v, __builtin_convertvector(x[c][h], h8));
-                }
-            pos[m] = row <= w.r1 ? w.p0 + token : -1;
-            pre[m] = row <= w.r1 ? w.prefix : 0;
-            slope[m] = MOD && p.slopes ? p.slopes[head] * LOG2E : 0.f;
-        }
         const int n0 = uniform(w.p0 + div_by(w.r0, p.G)), n1 = uniform(w.p0 + div_by(w.r1, p.G));
 
         f4 o[MB][VC];
@@ -618,9 +585,52 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
                 vs = vs2;
                 bad = bad2;
             };
+            // A run's start is a chain of accesses to memory, each waited for behind those that it does not need: table entries, Q, then keys and values.
             fetch_ids(0);
+            // Q as the B operand: lane (g, r) has values 64 x + 16 g .. + 15 of row r, as it has of the K rows.
+            u4v qf[MB][KC][2];
+            int pos[MB], pre[MB];
+            float slope[MB], by[MB];  // by: what a product is times, but the key's scale
+#pragma unroll
+            for (int m = 0; m < MB; m++) {
+                const int row = w.r0 + 16 * m + r, rc = min(row, w.r1), token = div_by(rc, p.G), head = run.kvh * (int)p.G.d + rc - token * (int)p.G.d;
+                const T* src = (const T*)p.q + (long)(w.first + token) * p.sqt + head * p.sqh;
+#pragma unroll
+                for (int c = 0; c < KC; c++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) qf[m][c][h] = *(const u4v*)(src + 64 * c + 16 * g + 8 * h);
+                pos[m] = row <= w.r1 ? w.p0 + token : -1;
+                pre[m] = row <= w.r1 ? w.prefix : 0;
+                slope[m] = MOD && p.slopes ? p.slopes[head] * LOG2E : 0.f;
+            }
+            __builtin_amdgcn_sched_barrier(0);
             load_k(0);
             fetch_ids(min(1, n - 1));
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int m = 0; m < MB; m++) {
+                f8 x[KC][2];
+                float top = 0.f;
+#pragma unroll
+                for (int c = 0; c < KC; c++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        x[c][h] = load8((const T*)&qf[m][c][h]);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[c][h][e]));
+                    }
+                top = rows_max(top);
+                const int up = top > 0.f && top <= FLT_TOP ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+                by[m] = ldexpf(p.scale, -up);
+#pragma unroll
+                for (int c = 0; c < KC; c++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[c][h][e] = ldexpf(x[c][h][e], up);
+                        qf[m][c][h] = __builtin_bit_cast(u4v, __builtin_convertvector(x[c][h], h8));
+                    }
+            }
             load_v();
             for (int i = 0;; i++) {
                 const int key0 = key_of(i);
