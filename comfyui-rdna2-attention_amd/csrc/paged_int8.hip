@@ -858,7 +858,6 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
     const int wave = uniform((int)(threadIdx.x >> 6));
     const int block = work_block(p.grid);
     Run run = find_run<MT, UK, AHEAD, 256, true>(p, (int*)smem, (u32*)(smem + L::SHARED), block);
-    int* flags = (int*)(smem + L::SHARED) + 256 + 8;  // a wave's: whether the cache lacks a page that it looked up
     Cut cut = {};
     const u32 smem_u = lds_addr(smem);
 
@@ -881,21 +880,30 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
         // scale of K (NaN if it is not finite), log2 of that of V, and its reciprocal.
         int base = 0, ids = 0;
         float ks0 = 0.f, ks1 = 0.f, lv0 = 0.f, lv1 = 0.f, iv0 = 0.f, iv1 = 0.f;
-        auto refresh = [&](int from) __attribute__((always_inline)) {
+        bool hole = false;  // whether the cache lacks a page of the lane's tile
+        auto look_up = [&](int from) __attribute__((always_inline)) {  // the pages, and the scales' loads (of V into lv0 and lv1)
             base = from;
             const int key = key_of(min(from + lane_again(), n - 1)), k0 = min(key, last16), k1 = min(key + 16, last16), e0 = div_by(k0, p.S), e1 = div_by(k1, p.S);
             const u32 t0 = (u32)table[e0], t1 = (u32)table[e1], p0 = t0 < (u32)p.P ? t0 : 0, p1 = t1 < (u32)p.P ? t1 : 0;
             const u32 r0 = (u32)(k0 - e0 * (int)p.S.d) >> p.shift, r1 = (u32)(k1 - e1 * (int)p.S.d) >> p.shift;
+            hole = p0 != t0 || p1 != t1;
             ids = (int)(wave >> 1 ? p1 : p0);
             ks0 = *(const global_float_t*)(ksbase + row_at(p0, p.ksp, r0, p.ksb));
             ks1 = *(const global_float_t*)(ksbase + row_at(p1, p.ksp, r1, p.ksb));
-            const float v0 = *(const global_float_t*)(vsbase + row_at(p0, p.vsp, r0, p.vsb)), v1 = *(const global_float_t*)(vsbase + row_at(p1, p.vsp, r1, p.vsb));
+            lv0 = *(const global_float_t*)(vsbase + row_at(p0, p.vsp, r0, p.vsb));
+            lv1 = *(const global_float_t*)(vsbase + row_at(p1, p.vsp, r1, p.vsb));
+        };
+        auto make_scales = [&]() __attribute__((always_inline)) {
             ks0 = ks0 <= FLT_TOP ? ks0 : __builtin_nanf("");
             ks1 = ks1 <= FLT_TOP ? ks1 : __builtin_nanf("");
-            lv0 = __builtin_amdgcn_logf(v0);
-            lv1 = __builtin_amdgcn_logf(v1);
-            iv0 = __builtin_amdgcn_rcpf(v0);
-            iv1 = __builtin_amdgcn_rcpf(v1);
+            iv0 = __builtin_amdgcn_rcpf(lv0);
+            iv1 = __builtin_amdgcn_rcpf(lv1);
+            lv0 = __builtin_amdgcn_logf(lv0);
+            lv1 = __builtin_amdgcn_logf(lv1);
+        };
+        auto refresh = [&](int from) __attribute__((always_inline)) {
+            look_up(from);
+            make_scales();
         };
         auto of_tile = [&](float x, int i) __attribute__((always_inline)) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i - base)); };
 
@@ -942,12 +950,56 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
             }
             issue(i + 4);
         };
-        bool holes = false;  // whether the cache lacks any page of the run's part
+        // A run's start is a chain of accesses to memory: Q goes out first, then table entries, then scales and the first copies together (2 x 4096 rows capped in a window of 2048:
+        // 222.5 -> 219.5 us). Q as the B operand of S^T = K Q^T: fp16, its row's largest brought to 2^14 to 2^15, which `by` takes back.
+        u4v qf[KS];
+        float slope = 0.f, by = 0.f;
+        int pos = 0;
+        if (active) {
+            const int row = min(wr0 + lq, w.r1), token = div_by(row, p.G), head = run.kvh * (int)p.G.d + row - token * (int)p.G.d;
+            const T* src = (const T*)p.q + (long)(w.first + token) * p.sqt + head * p.sqh;
+#pragma unroll
+            for (int x = 0; x < KS; x++) qf[x] = *(const u4v*)(src + (2 * x + g) * 8);
+            if constexpr (MOD) {
+                if (p.slopes) slope = p.slopes[head] * LOG2E;
+                pos = w.p0 + token;
+            }
+        }
         if (n > 0) {
-            refresh(0);
-            wait_copies();
+            look_up(0);
             issue(0);
             issue(1);
+        }
+        if (active) {
+            float top = 0.f;
+            auto values = [&](int x) __attribute__((always_inline)) {
+                typedef T t8 __attribute__((ext_vector_type(8)));
+                return __builtin_convertvector(__builtin_bit_cast(t8, qf[x]), f8);
+            };
+#pragma unroll
+            for (int x = 0; x < KS; x++) {
+                const f8 v = values(x);
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(v[e]));
+            }
+            const f2 h = both_halves(top);
+            top = fmaxf(h[0], h[1]);
+            const int up = top > 0.f && top <= FLT_TOP ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+            by = ldexpf(p.scale, -up);
+#pragma unroll
+            for (int x = 0; x < KS; x++) {
+                f8 v = values(x);
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = ldexpf(v[e], up);
+                qf[x] = __builtin_bit_cast(u4v, __builtin_convertvector(v, h8));
+            }
+#pragma unroll
+            for (int x = 0; x < KS; x++) asm volatile("" : "+v"(qf[x]));  // made here, not inside the tile loop
+        }
+        bool holes = false;  // whether the cache lacks any page of the run's part
+        if (n > 0) {
+            make_scales();
+            holes = __any(hole);
             wait_copies();
 #pragma unroll
             for (int t = 0; t < 2; t++) {
@@ -959,11 +1011,12 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
             }
             issue(2);
             issue(3);
-            const int e1 = div_by(min(key_of(n - 1) + UK, w.hi) - 1, p.S);  // (with what is skipped)
-            bool hole = false;
-            for (int e = div_by(key_of(0), p.S) + (int)threadIdx.x; e <= e1; e += 256) hole |= (u32)table[e] >= (u32)p.P;
-            hole = __any(hole);
-            if (lane_again() == 0) flags[wave] = hole;
+            if (n > 64) {  // more tiles than the lanes looked at
+                const int e1 = div_by(min(key_of(n - 1) + UK, w.hi) - 1, p.S);  // (with what is skipped)
+                bool any = false;
+                for (int e = div_by(key_of(0), p.S) + lane_again(); e <= e1; e += 64) any |= (u32)table[e] >= (u32)p.P;
+                holes = __any(any);
+            }
         }
 
         f16v o[DT];
@@ -980,44 +1033,6 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
                 __syncthreads();
             }
         } else {
-            // Q as the B operand of S^T = K Q^T: fp16, its row's largest brought to 2^14 to 2^15, which `by` takes back.
-            u4v qf[KS];
-            float slope = 0.f, by;
-            int pos = 0;
-            {
-                const int row = min(wr0 + lq, w.r1), token = div_by(row, p.G), head = run.kvh * (int)p.G.d + row - token * (int)p.G.d;
-                const T* src = (const T*)p.q + (long)(w.first + token) * p.sqt + head * p.sqh;
-                float top = 0.f;
-#pragma unroll
-                for (int x = 0; x < KS; x++) qf[x] = *(const u4v*)(src + (2 * x + g) * 8);
-                auto values = [&](int x) __attribute__((always_inline)) {
-                    typedef T t8 __attribute__((ext_vector_type(8)));
-                    return __builtin_convertvector(__builtin_bit_cast(t8, qf[x]), f8);
-                };
-#pragma unroll
-                for (int x = 0; x < KS; x++) {
-                    const f8 v = values(x);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(v[e]));
-                }
-                const f2 h = both_halves(top);
-                top = fmaxf(h[0], h[1]);
-                const int up = top > 0.f && top <= FLT_TOP ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-                by = ldexpf(p.scale, -up);
-#pragma unroll
-                for (int x = 0; x < KS; x++) {
-                    f8 v = values(x);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = ldexpf(v[e], up);
-                    qf[x] = __builtin_bit_cast(u4v, __builtin_convertvector(v, h8));
-                }
-#pragma unroll
-                for (int x = 0; x < KS; x++) asm volatile("" : "+v"(qf[x]));  // made here, not inside the tile loop
-                if constexpr (MOD) {
-                    if (p.slopes) slope = p.slopes[head] * LOG2E;
-                    pos = w.p0 + token;
-                }
-            }
             // The lane's K reads: row lq, chunk 2 x + g, at k_base ^ 32 x. Its V^T reads: lane i of 16 reads 8 bytes of row 4 g + i / 4 and gets the
             // transposed values; chunk 4 d on of the row at v_base ^ 64 d.
             u32 k_base = smem_u + (u32)(lq * ROW + ((g ^ (D == 128 ? lq & 15 : lq >> 1 & 7)) << 4));
@@ -1244,7 +1259,6 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
 
             if (n > 0) {
                 __syncthreads();
-                holes = uniform(flags[0] | flags[1] | flags[2] | flags[3]) != 0;
                 if (!holes) {
                     const int upto = min(w.hi, p.window > 0 ? n0 + 1 : max(n0 + 1, w.prefix));
                     const int window_first = key_first + w.skip;
