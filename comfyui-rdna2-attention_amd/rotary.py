@@ -129,12 +129,12 @@ def written(*tensors):
 
 
 class Sizes(dict):
-    """The size arguments of an operator's calls by their tensors' types, shapes and strides: checked and packed once for each."""
+    """The size arguments (and bytes of workspace) of an operator's calls by their tensors' types, shapes and strides: checked and packed once for each."""
 
-    def keep(self, key, values):
+    def keep(self, key, values, workspace=None):
         if len(self) >= 4096:
             self.clear()
-        self[key] = value = _lib.long_array(values)
+        self[key] = value = _lib.long_array(values) if workspace is None else (_lib.long_array(values), workspace)
         return value
 
 
@@ -231,7 +231,7 @@ class HeadNorm:
     k = property(lambda self: self._k, doc="The weights of the key heads.")
 
 
-_norm_sizes, _norm_back_sizes, _norm_workspaces = Sizes(), Sizes(), {}
+_norm_sizes, _norm_back_sizes = Sizes(), Sizes()
 
 
 class _NormTurn(torch.autograd.Function):
@@ -282,25 +282,26 @@ def _norm_rotate(q, k, positions, rotary, q_weight, k_weight, eps):
 
 def _norm_rotate_back(q, k, q_grad, k_grad, positions, rotary, q_weight, k_weight, eps):
     """The gradients of q, k and the weights."""
-    q, k, positions = vector_rows(q), vector_rows(k), positions.contiguous()
-    q_grad, k_grad = vector_rows(q_grad), vector_rows(k_grad)
+    positions = positions.contiguous()
+    key = (q.dtype, q.shape, q.stride(), k.dtype, k.shape, k.stride(), q_grad.shape, q_grad.stride(), k_grad.shape, k_grad.stride(), positions.shape, rotary.dim,
+           q_weight.dtype, q_weight.shape, q_weight.stride(), k_weight.dtype, k_weight.shape, k_weight.stride())
+    sizes = _norm_back_sizes.get(key)
+    if sizes is None or (q.data_ptr() | k.data_ptr() | q_grad.data_ptr() | k_grad.data_ptr()) % 16:
+        if not (q_weight.shape == k_weight.shape == q.shape[-1:] and q_weight.dtype == k_weight.dtype and rows_ready(q_weight) and rows_ready(k_weight)):
+            raise ValueError("norm_rotate's gradient takes the weights that its call took: their data has been replaced")
+        if q_grad.shape != q.shape or k_grad.shape != k.shape or q.dtype != k.dtype or positions.shape != q.shape[:-2] or positions.shape != k.shape[:-2]:
+            raise ValueError("norm_rotate's gradient takes the q, k and positions that its call took: their data has been replaced")
+        ready = all(rows_ready(t) for t in (q, k, q_grad, k_grad))
+        q, k, q_grad, k_grad = vector_rows(q), vector_rows(k), vector_rows(q_grad), vector_rows(k_grad)
+        sizes = _norm_back_dims(q, k, q_grad, k_grad, rotary, key if ready else None)
     q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(k, memory_format=torch.contiguous_format)
     if positions.numel() == 0:
         return q_out, k_out, torch.zeros_like(q_weight), torch.zeros_like(k_weight)
     q_weight_out, k_weight_out = torch.empty_like(q_weight), torch.empty_like(k_weight)
     same_device("norm_rotate's gradient", q, k, q_grad, k_grad, positions, q_weight, k_weight, rotary.turns)
-    key = (q.shape, q.stride(), k.shape, k.stride(), q_grad.stride(), k_grad.stride(), rotary.dim)
-    dims = _norm_back_sizes.get(key)
-    if dims is None:
-        dims = _norm_back_sizes.keep(key, _norm_dims(q, k, rotary) + [s for t in (q_grad, k_grad) for s in _strides(t)])
-    sizes = (positions.numel(), q.shape[-2], k.shape[-2], q.shape[-1])
-    kernels = get_kernels()
-    size = _norm_workspaces.get(sizes)
-    if size is None:
-        if len(_norm_workspaces) >= 4096:
-            _norm_workspaces.clear()
-        size = _norm_workspaces[sizes] = kernels.norm_rotate_back_workspace(*sizes)
+    dims, size = sizes
     workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    kernels = get_kernels()
     _lib.check(kernels.norm_rotate_back(q.data_ptr(), k.data_ptr(), q_grad.data_ptr(), k_grad.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
                                         q_weight_out.data_ptr(), k_weight_out.data_ptr(), positions.data_ptr(), positions.dtype is torch.int64,
                                         q_weight.data_ptr(), k_weight.data_ptr(), TYPES[q_weight.dtype], eps, rotary.turns.data_ptr(), rotary.factor,
@@ -319,6 +320,14 @@ def _strides(t):
 def _norm_dims(q, k, rotary):
     B, L = (1, q.shape[0]) if q.dim() == 3 else q.shape[:2]
     return [B, L, q.shape[-2], k.shape[-2], q.shape[-1], rotary.dim, *_strides(q), *_strides(k)]
+
+
+def _norm_back_dims(q, k, q_grad, k_grad, rotary, key):
+    """(the size arguments, bytes of workspace) of a gradient; kept for the key (None: not)."""
+    values = _norm_dims(q, k, rotary) + [s for t in (q_grad, k_grad) for s in _strides(t)]
+    B, L, H, Hkv, D = values[:5]
+    size = get_kernels().norm_rotate_back_workspace(B * L, H, Hkv, D) if B * L else 0
+    return (_lib.long_array(values), size) if key is None else _norm_back_sizes.keep(key, values, size)
 
 
 def _check_norm_rotate(q, k, positions, rotary, weight, k_weight, key):

@@ -80,6 +80,18 @@ def test_replaced_weights():
                 paged_kv.append(cache, batch, k, k, norm=norm)
 
 
+def test_inputs_replaced_before_the_gradient():
+    rot, n = rotary.Rotary(32, device="cpu"), torch.zeros(4, dtype=torch.int32)
+    q, k, w = torch.zeros(4, 3, 64), torch.zeros(4, 2, 64), torch.ones(64)
+    for data in (torch.ones(48), torch.ones(128)[::2], torch.ones(64).half()):
+        for weights in ((data, w), (w, data)):
+            with pytest.raises(ValueError, match="replaced"):
+                rotary._norm_rotate_back(q, k, q, k, n, rot, *weights, 1e-6)
+    for bad in ((q[:3], k, q, k, n), (q, k[:, :1], q, k, n), (q, k, q, k, n[:3]), (q, k.half(), q, k, n)):
+        with pytest.raises(ValueError, match="replaced"):
+            rotary._norm_rotate_back(*bad, rot, w, w, 1e-6)
+
+
 def test_entry_points_reject_before_any_launch():
     lib = _lib.declare(ctypes.CDLL(_lib.LIB_PATH))
     a = 1 << 20
