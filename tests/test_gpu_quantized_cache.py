@@ -365,6 +365,30 @@ def test_long_runs(dev, type_, D, options):
         check(got[:, one], ref, off, t)
 
 
+@pytest.mark.parametrize("type_,D,missing,options", [("fp16", 128, (0, 100, 265), {}), ("bf16", 64, (3, 131, 200), dict(softcap=30.0)), ("fp16", 64, (130, 190), dict(window=9000, prefix=70))])
+def test_missing_pages_in_long_runs(dev, type_, D, missing, options):
+    """Pages that the cache does not have, where they lie in the first tiles of a run, past its 64th, or at its end: their keys are masked, whatever the codes that are read instead."""
+    g = gen(54)
+    t, kv, page, block, new, length = TYPES[type_], 64, 64, 32, 150, 17000
+    table, starts, lengths, pages = batch_of([(new, length)], page, g)
+    for i, at in enumerate(missing):
+        table[0, at] = (-1, pages, 2 ** 31 - 1)[i]
+    k, v, ks, vs = on(dev, *codes_of(pages, page, kv, D, block, g))
+    vs[0] *= 1000.0  # what page 0 holds would show
+    table[0][table[0] == 0] = 1
+    q = torch.randn(new, kv, D, generator=g).to(t)
+    q = torch.where(q.abs() < 2.0 ** -10, 0, q)
+    o = dict(options)
+    if "prefix" in o:
+        o["prefix"] = torch.tensor([o["prefix"]], dtype=torch.int32)
+    got = paged_kv.attention(paged_kv.QuantizedCache(k, v, ks, vs), paged_kv.Batch(*on(dev, table, starts, lengths)), q.to(dev),
+                             **{n: x.to(dev) if isinstance(x, torch.Tensor) else x for n, x in o.items()})
+    for h in range(3, kv, 12):
+        one = slice(h, h + 1)
+        ref, off, _ = attended_quantized(q[:, one], *(x[:, :, one].cpu() for x in (k, v, ks, vs)), table, starts, lengths, **o)
+        check(got[:, one], ref, off, t)
+
+
 @pytest.mark.parametrize("type_,kv", [("fp16", 2), ("bf16", 2), ("fp16", 24), ("bf16", 24)])
 def test_rows_that_see_nothing(dev, type_, kv):
     """Lengths below the new tokens (negative positions), lengths of zero, pages that the cache does not have, rows behind the last sequence."""
