@@ -72,7 +72,8 @@ __device__ __forceinline__ WorkTile make_tile(const PagedArgs& p, int b, int j) 
         // SKIP leaves them out: the first `head` units are the prefix's, the others begin where the tile's first row's window does.
         if (p.window > 0 && t.prefix > 0 && n0 >= p.window) {
             t.head = (t.prefix + UK - 1) / UK;
-            t.skip = max((n0 - p.window + 1) / UK * UK - t.head * UK, 0);
+            // Where the window begins behind the keys (lengths past the table's capacity), up to their end: the units are then the prefix's.
+            t.skip = max(min((n0 - p.window + 1) / UK, (t.hi + UK - 1) / UK) - t.head, 0) * UK;
         }
     }
     t.units = AHEAD + max((t.hi - t.lo - t.skip + UK - 1) / UK, 1);  // a tile without keys is one unit: its rows are written too
