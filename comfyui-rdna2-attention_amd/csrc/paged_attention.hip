@@ -808,7 +808,7 @@ __global__ __launch_bounds__(256, D == 128 && MOD ? 2 : 3) void tiles_kernel(Pag
                 holes = uniform(flags[0] | flags[1] | flags[2] | flags[3]) != 0;
                 if (!holes) {
                     const int upto = min(w.hi, p.window > 0 ? n0 + 1 : max(n0 + 1, w.prefix));
-                    full0 = p.window > 0 ? max(n1 - p.window + UK - key_first, 0) / UK : 0;  // the first tile with key0 > n1 - window
+                    full0 = first_unit_in_window<UK>(n1, p.window, key_first);
                     full1 = min(max((upto - key_first) / UK, 0), n);
                 }
             }

@@ -1262,7 +1262,7 @@ __global__ __launch_bounds__(256, TILES8_WGS(D, MOD)) void tiles8_kernel(Attn8Ar
                 if (!holes) {
                     const int upto = min(w.hi, p.window > 0 ? n0 + 1 : max(n0 + 1, w.prefix));
                     const int window_first = key_first + w.skip;
-                    full0 = p.window > 0 ? max(n1 - p.window + UK - window_first, 0) / UK : 0;  // the first tile with key0 > n1 - window
+                    full0 = first_unit_in_window<UK>(n1, p.window, window_first);
                     if (w.skip) full0 = max(full0, head);
                     full1 = min(max((upto - window_first) / UK, 0), n);
                 }

@@ -80,6 +80,14 @@ __device__ __forceinline__ WorkTile make_tile(const PagedArgs& p, int b, int j) 
     return t;
 }
 
+// The first unit i whose keys first + i UK and on are all within the window of a row at position n1 (no window: 0). In 64 bits: positions may be up to the
+// last of 32 bits, far behind the keys that a short table holds.
+template <int UK>
+__device__ __forceinline__ int first_unit_in_window(int n1, int window, int first) {
+    const long behind = (long)n1 - window + UK - first;
+    return window > 0 && behind > 0 ? (int)(behind / UK) : 0;
+}
+
 // The same in every lane, which the compiler does not see of values that come from memory: in scalar registers.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 template <class X>

@@ -1,5 +1,6 @@
 """The keys that the tiles of paged attention walk (make_tile in csrc/paged_work.h, its own text compiled with the host g++) against the keys that their rows
-see: each of these once and none twice, whatever the length, the table's capacity, the window and the prefix."""
+see: each of these once and none twice, whatever the length, the table's capacity, the window and the prefix; and the units that are taken without a mask: all
+of whose keys all rows see."""
 import os
 import re
 import shutil
@@ -38,6 +39,7 @@ static long spread(long n) {  // small numbers as often as large ones
 }
 static long bad = 0, capped = 0, skipped = 0;
 
+// Tiles of 128 rows take units full0 .. full1 - 1 without a mask, as the kernels have them for each of their waves of 32 rows.
 template <int MT, int UK, int AHEAD, bool SKIP>
 static void walk(const PagedArgs& p, int group) {
     int first;
@@ -62,6 +64,16 @@ static void walk(const PagedArgs& p, int group) {
             const bool seen = sees(ends[0], k) || sees(ends[1], k) || (p.window > 0 && k > t.p0 + t.r0 / group && k <= t.p0 + t.r1 / group);
             wrong = seen ? k >= t.hi || walked[k] != 1 : k < t.hi && walked[k] > 1;
         }
+        if (MT == 128)
+            for (int w0 = t.r0; w0 <= t.r1 && n > 0 && !wrong; w0 += 32) {
+                const int w1 = min(w0 + 31, t.r1), n0 = t.p0 + w0 / group, n1 = t.p0 + w1 / group, seen_to = min(t.hi, p.window > 0 ? n0 + 1 : max(n0 + 1, t.prefix));
+                const int window_first = t.lo + t.skip;
+                int full0 = first_unit_in_window<UK>(n1, p.window, window_first);
+                if (t.skip) full0 = max(full0, t.head);
+                const int full1 = min(max((seen_to - window_first) / UK, 0), n);
+                for (int i = full0; i < full1; i++)
+                    for (long k = key_of(i); k < key_of(i) + UK; k++) wrong |= !sees(w0, (int)k) || !sees(w1, (int)k) || k >= t.hi;
+            }
         skipped += t.skip > 0;
         if (wrong && !bad++)
             printf("length %d capacity %d window %d prefix %d rows %d tile %d of %d rows, %d keys a unit, skip %d: lo %d hi %d head %d skip %d units %d\n", p.lengths[0], p.capacity,
@@ -75,6 +87,7 @@ int main() {
         if (i % 50 == 0) length = 0x7fffffff - (int)spread(5000);
         PagedArgs p = {starts, &length, upto(3) ? &prefix : nullptr, tokens, capacity, upto(3) ? (int)spread(4000) : 0, {group}};
         if (i % 50 == 0 && upto(1)) p.window = max(length - (int)spread(4000), 1);
+        if (i % 97 == 0) p.window = 0x7fffffff;
         capped += length > capacity;
         walk<16, 256, 1, true>(p, group);
         walk<32, 128, 1, true>(p, group);
@@ -95,8 +108,9 @@ def test_every_visible_key_is_walked_once(tmp_path):
     struct, = re.findall(r"^struct WorkTile \{\n.*?^\};\n", text, re.M | re.S)
     rows, = re.findall(r"^__device__ __forceinline__ int seq_rows\(.*?^\}\n", text, re.M | re.S)
     tile, = re.findall(r"^template <int MT, int UK, int AHEAD, bool SKIP = false>\n__device__ __forceinline__ WorkTile make_tile\(.*?^\}\n", text, re.M | re.S)
+    full, = re.findall(r"^template <int UK>\n__device__ __forceinline__ int first_unit_in_window\(.*?^\}\n", text, re.M | re.S)
     source, exe = tmp_path / "walk.cpp", tmp_path / "walk"
-    source.write_text(SHIM + struct + rows + tile + CHECK)
+    source.write_text(SHIM + struct + rows + tile + full + CHECK)
     subprocess.run(["g++", "-std=c++17", "-O2", "-fwrapv", str(source), "-o", str(exe)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=600)
     assert r.returncode == 0, r.stdout
