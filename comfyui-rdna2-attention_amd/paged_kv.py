@@ -8,13 +8,14 @@ the time where attention waits for it); `append` and `attention` take either, `r
 A step of a serving loop: write the batch's page table, starts and lengths; `append`; `attention` with the rotated queries. All three
 are device tensors that the kernels read: a captured graph of the two calls stays valid while their contents change.
 
-There is no backward pass: where gradients are recorded, tensors that require one are refused.
+There is no backward pass: where gradients are recorded, tensors that require one are refused, as tensors with a forward-mode tangent always are.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .hip_attention import Kernels
-from .rotary import MAX_HEAD, MAX_TOKENS, TYPES, WEIGHTS_ERROR, Sizes, distinct, rows_ready, same_device, vector_rows, written
+from .rotary import MAX_HEAD, MAX_TOKENS, TYPES, WEIGHTS_ERROR, Sizes, distinct, no_tangents, rows_ready, same_device, vector_rows, written
 
 HEADS = (64, 128)  # head dims of `attention`
 MAX_SEQUENCES = 8192
@@ -32,8 +33,11 @@ def get_kernels():
     return kernels
 
 
-def _no_gradient(what, *tensors):
-    """Raises ValueError if any of the tensors (None: none) requires a gradient and gradients are recorded."""
+def _no_gradient(what, *tensors, cache=()):
+    """Raises ValueError if any of the tensors (None: none) requires a gradient and gradients are recorded, or if one of them or of the cache's carries a forward-mode
+    tangent."""
+    if forward_ad._current_level >= 0:
+        no_tangents(what, *tensors, *cache)
     for t in tensors:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{what} has no backward pass and would drop the gradient of its inputs: call it under torch.no_grad(), or with detached tensors")
@@ -53,7 +57,7 @@ class Cache:
             raise ValueError("Cache takes k and v on one device")
         if k.requires_grad or v.requires_grad:
             raise ValueError("Cache takes k and v that require no gradient: append writes them")
-        self._k, self._v = k, v
+        self._k, self._v = self._tensors = k, v
         self.sizes = (k.dtype, k.shape, k.stride(), v.stride())
 
     k = property(lambda self: self._k, doc="The pages of the keys.")
@@ -85,7 +89,7 @@ class QuantizedCache:
             raise ValueError("QuantizedCache takes its tensors on one device")
         if k_scales.requires_grad or v_scales.requires_grad:
             raise ValueError("QuantizedCache takes scales that require no gradient: append writes them")
-        self._k, self._v, self._k_scales, self._v_scales = k, v, k_scales, v_scales
+        self._k, self._v, self._k_scales, self._v_scales = self._tensors = k, v, k_scales, v_scales
         self.block = block
         self.sizes = (k.dtype, k.shape, k.stride(), v.stride(), block, k_scales.stride(), v_scales.stride())
 
@@ -163,7 +167,7 @@ def append(cache, batch, k, v, rotary=None, q=None, q_out=None, norm=None):
     may remain for both. q_out is fp16 or bf16 there (None: in place, q in one of them), and `norm` (a rotary.HeadNorm of D weights) norms k and
     q ahead of their turn as rotary.norm_rotate does. (With a Cache, call rotary.norm_rotate first and append its result.)"""
     kc, vc = cache._k, cache._v
-    _no_gradient("append", k, v, q, q_out)
+    _no_gradient("append", k, v, q, q_out, cache=cache._tensors)
     if isinstance(cache, QuantizedCache):
         return _append_quantized(cache, batch, k, v, rotary, q, q_out, norm)
     if norm is not None:
@@ -321,6 +325,7 @@ def read(cache, batch, tokens, dtype=torch.bfloat16):
         raise ValueError("read takes a QuantizedCache: a Cache's pages hold their values as they are")
     kc, vc, ks, vs = cache._k, cache._v, cache._k_scales, cache._v_scales
     _, _, Hkv, D = kc.shape
+    _no_gradient("read", cache=cache._tensors)
     key = (cache.sizes, batch.sizes, tokens, dtype)
     dims = _read_sizes.get(key)
     if dims is None:
@@ -347,7 +352,7 @@ def attention(cache, batch, q, out=None, scale=None, softcap=0.0, window=0, slop
     sequence left as they were), or a new tensor, with those rows 0. Keys between a prefix and the window cost time as if they were seen (over a
     QuantizedCache none). A call takes up to 102 MB of workspace from torch's allocator."""
     kc, vc = cache._k, cache._v
-    _no_gradient("attention", q, slopes, out)
+    _no_gradient("attention", q, slopes, out, cache=cache._tensors)
     fill = out is None
     if fill:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)

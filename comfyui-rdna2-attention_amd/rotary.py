@@ -6,6 +6,7 @@ way into the cache with the same arithmetic as `rotate`. `norm_rotate` norms que
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .hip_attention import Kernels
@@ -128,6 +129,14 @@ def written(*tensors):
     torch._C._increment_version(tensors)
 
 
+def no_tangents(what, *tensors):
+    """Raises ValueError if any of the tensors (None: none) carries a forward-mode tangent: the kernels would drop it. (torch.no_grad() does not end forward mode.) Called
+    where a level of it is open: that look is all that a call without one pays."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{what} has no forward mode and would drop its tensors' tangents: call it with the primals of torch.autograd.forward_ad.unpack_dual")
+
+
 class Sizes(dict):
     """The size arguments (and bytes of workspace) of an operator's calls by their tensors' types, shapes and strides: checked and packed once for each."""
 
@@ -161,8 +170,10 @@ def rotate(x, positions, rotary, out=None, inverse=False):
     turn in 32, rounded once. Values past rotary.dim are copied. inverse turns back: the gradient of x for a gradient of the result
     (and, where rotary.factor is 1, x itself). Any strides of x with a contiguous last dimension (other heads-first
     layouts are views of these shapes); out, if given, is x itself or does not overlap it. Returns out, or a new contiguous tensor, which
-    carries x's gradient where gradients are recorded (an out carries none, and is refused there if x or out requires one)."""
+    carries x's gradient where gradients are recorded (an out carries none, and is refused there if x or out requires one). Forward-mode tangents are refused."""
     made = out is None
+    if forward_ad._current_level >= 0:
+        no_tangents("rotate", x, out)
     if (x.requires_grad or (not made and out.requires_grad)) and torch.is_grad_enabled():
         if not made:
             raise ValueError("rotate records no gradient through out: leave it, or call under torch.no_grad()")
@@ -255,7 +266,9 @@ def norm_rotate(q, k, positions, rotary, norm):
     `positions`, in one launch: (q, k), new contiguous tensors of their type. A head x becomes the turn of w x / sqrt(mean(x^2) + norm.eps), w norm.q or
     norm.k, in 32 bits, rounded once. Any strides with a contiguous last dimension. Gradients of q, k and the weights are carried where they are
     recorded, those of the weights summed in 32 bits and rounded once; the same inputs give the same bits. (A backward pass is captured as torch's own are: with
-    no graph of the same leaves alive that was recorded outside of the capture.)"""
+    no graph of the same leaves alive that was recorded outside of the capture.) Forward-mode tangents are refused."""
+    if forward_ad._current_level >= 0:
+        no_tangents("norm_rotate", q, k, norm.q, norm.k)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or norm.q.requires_grad or norm.k.requires_grad):
         return _NormTurn.apply(q, k, norm.q, norm.k, positions, rotary, norm.eps)
     return _norm_rotate(q, k, positions, rotary, norm.q, norm.k, norm.eps)
@@ -282,6 +295,8 @@ def _norm_rotate(q, k, positions, rotary, q_weight, k_weight, eps):
 
 def _norm_rotate_back(q, k, q_grad, k_grad, positions, rotary, q_weight, k_weight, eps):
     """The gradients of q, k and the weights."""
+    if forward_ad._current_level >= 0:
+        no_tangents("norm_rotate's gradient", q, k, q_grad, k_grad, q_weight, k_weight)
     positions = positions.contiguous()
     key = (q.dtype, q.shape, q.stride(), k.dtype, k.shape, k.stride(), q_grad.shape, q_grad.stride(), k_grad.shape, k_grad.stride(), positions.shape, rotary.dim,
            q_weight.dtype, q_weight.shape, q_weight.stride(), k_weight.dtype, k_weight.shape, k_weight.stride())
