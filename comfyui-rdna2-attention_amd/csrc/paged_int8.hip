@@ -502,12 +502,12 @@ __device__ __forceinline__ f4 product16(const u4v& a, const u4v& b, const f4& c)
 // before both: P and its sum are then off by roundings of P to fp16 that do not cancel, up to 1.3 times the rms error of a plain form that keeps P in 32 bits (fp16
 // outputs; with bf16 ones the output's rounding hides it).
 //
-// Bound by the keys and values read: 64 single tokens over 8192 keys (8 KV heads of 128), 1.08 GB, 206 us, 5.2 TB/s, in pages of whole heads 188, 5.7, where a large sum
+// Bound by the keys and values read: 64 single tokens over 8192 keys (8 KV heads of 128), 1.08 GB, 206 to 209 us, 5.2 TB/s, in pages of whole heads 188, 5.7, where a large sum
 // reads at 6.0; vector work, half of it widening codes, takes 33% of the cycles. Loads are issued in the order in which they are waited for: each wait is then for
 // its own loads alone, with the next tile's 16 KiB (of K, then of V) behind them.
 //
-// Tiles of 32 rows take 32 keys a wave (64 spill registers: 32 sequences of 5 tokens over 4096 keys 85 us, 75 so); tiles of 16 rows 64 (with 32: 213 us for 64 x 8192, and
-// at three workgroups a CU 219, where 61 ragged sequences gain 5%).
+// Tiles of 32 rows take 32 keys a wave (64 spill registers: 32 sequences of 5 tokens over 4096 keys 67.5 us, 61.6 so); tiles of 16 rows 64 (with 32: 64 x 8192 213 us, 209
+// so, and at three workgroups a CU 219, where 61 ragged sequences gain 5%).
 __host__ __device__ constexpr int rows8_steps(int mb) { return mb == 1 ? 2 : 1; }  // 32 keys each
 template <class T, int D, int MB, bool MOD>
 __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
@@ -830,8 +830,9 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
 // * Where a scale of V is above the row's vm, or below it by more than 2^8, or is not finite, the step is not a full one: the plain steps sum P before it
 //   is scaled, and move vm (to twice the scale: O is then seldom rescaled).
 //
-// A chunk of 2048 tokens over 14336 keys, 32 heads over 8 of 128: 618 to 627 us, 0.82 to 0.83 PFLOP/s, 64% of a library product of 8192^3; the 16-bit cache's kernel takes 568. Products take 37% of the
-// cycles and vector work 56% (ten instructions a product, where the 16-bit kernel has five: widening, scales), which add up on a SIMD. Two workgroups a CU: at three the registers
+// A chunk of 2048 tokens over 14336 keys, 32 heads over 8 of 128: 612 us and 15 of the merge in a kernel trace of 400 calls once the clock has settled (695 in the first 40,
+// up to 830 from an idle GPU), whole calls 618 to 640 by the box, 0.80 to 0.83 PFLOP/s, 62 to 64% of a library product of 8192^3. The 16-bit cache takes 564 over normal values, 604 over those
+// that these codes stand for. Products take 37% of the cycles and vector work 56% (ten instructions a product, where the 16-bit kernel has five: widening, scales), which add up on a SIMD. Two workgroups a CU: at three the registers
 // spill (1920 us). Widening at the start of a step 655, beside the products and two tiles ahead 619; V read ahead of the look at P no faster. With D = 64, half the
 // products beside the same vector work, 414 (16-bit: 312).
 #define TILES8_WGS(D, MOD) ((D) == 64 && !(MOD) ? 3 : 2)
@@ -1417,6 +1418,10 @@ static int make_plan8(long T, long B, long H, long Hkv, long D, int type, Plan8*
     if (T <= 0 || B <= 0 || B > MAX_SEQUENCES || Hkv <= 0 || H <= 0 || H % Hkv || (D != 64 && D != 128) || type < RDA_FP16 || type > RDA_BF16) return RDA_ERR_INVALID;
     if (T * (H / Hkv) >= 1L << 31) return RDA_ERR_INVALID;
     const long rows = T * (H / Hkv) / B;
+    // Rows of a tile, by a sequence's mean (a call cannot look at starts): us at tiles of 16 / 32 / 128, D = 128, 32 heads over 8. 32 sequences over 4096 keys of 4 rows 50 / 55 / 76, 16 rows
+    // 52 / 57 / 78, 20 rows 61 / 58 / 79, 64 rows 114 / 85 / 98, 96 rows 167 / 144 / 108; one prompt over 2000 of 640 rows 38 / 33 / 39, of 1024 47 / 44 / 41, of 2048 81 / 68 / 52. Both bounds stand
+    // where the 16-bit cache's do. What that costs: 8 sequences of 96 rows 55 / 48 / 61 and one of 644 38 / 32 / 42 (128 is taken), and with D = 64 small batches of up to 512 rows, which tiles
+    // of 16 take 5 to 15% faster (one prompt of 512 rows 22.4 / 24.9 / 32.9, 32 sequences of 20 rows 40 / 45 / 56; but of 48 rows 73 / 66 / 66).
     plan->mt = rows <= 16 ? 16 : rows <= 64 || B * ((rows + 127) / 128) * Hkv <= 40 ? 32 : 128;
     // Where a sequence's rows of a KV head are one tile no keys are read twice, and runs go to the XCDs in turn, so that each has parts of all heads: a key's codes of
     // a head are 64 or 128 bytes of a row of all heads (in pages laid out token by token), and XCDs of a head each would use few of their caches'
@@ -1501,7 +1506,9 @@ int rda_paged_append_i8(const void* q, const void* k, const void* v, void* q_out
         using X = decltype(x);
         const auto to = [&](auto y) {
             using Q = decltype(y);
-            // 64 sequences of 1 / 2 / 3 / 5 / 8 tokens: 4.5 / 7.3 / 10.0 / 15.1 / 25.1 us by tokens, 14.4 / 14.2 / 12.5 / 12.7 / 11.7 by blocks; 256 of one 5.3 and 38.6.
+            // 64 sequences of 1 / 2 / 3 / 5 / 8 tokens: 4.5 / 7.3 / 10.0 / 15.0 / 25.2 us by tokens, 14.4 / 14.3 / 12.7 / 12.9 / 11.7 by blocks; 256 of one 5.4 and 39.7. The mean decides,
+            // since a call cannot look at starts, and a chunk among single tokens is written by one wave for each block and slice of heads: 127 tokens beside a chunk of 256 take 71 us (blocks
+            // of 64: 137) where the kernel of blocks would take 23 (40), 63 beside a chunk of 190 70 (137) and 16 (27).
             if (T < 4 * B) {
                 const int held = rows, slices = (int)((H + held - 1) / held + 2 * ((Hkv + held - 1) / held));
                 hipLaunchKernelGGL((append8_few_kernel<X, Q>), dim3((unsigned)T, (unsigned)((slices + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);

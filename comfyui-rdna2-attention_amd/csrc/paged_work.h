@@ -64,12 +64,12 @@ __device__ __forceinline__ WorkTile make_tile(const PagedArgs& p, int b, int j) 
     t.prefix = p.prefix ? min(max(p.prefix[b], 0), t.keys) : 0;
     const int n0 = t.p0 + div_by(t.r0, p.G), n1 = t.p0 + div_by(max(t.r1, 0), p.G);
     t.hi = min(t.keys, max(n1 + 1, t.prefix));
-    // With a prefix a tile's keys begin at 0, and those between the prefix and the window are walked too, though no row sees them: over 65536 keys
-    // with a window of 4096 a single token takes 14 us, with a prefix of 4 keys as well 59, a chunk of 512 tokens 78 and 513.
+    // With a prefix a tile's keys begin at 0, and without SKIP (16- and 32-bit caches) those between the prefix and the window are walked too, though no row sees them: over 65536 keys
+    // with a window of 4096 a single token takes 14 us, with a prefix of 4 keys as well 57, a chunk of 512 tokens 78 and 522.
     t.lo = p.window > 0 && t.prefix == 0 && n0 >= p.window ? (n0 - p.window + 1) / UK * UK : 0;
     t.head = t.skip = 0;
     if constexpr (SKIP) {
-        // SKIP leaves them out: the first `head` units are the prefix's, the others begin where the tile's first row's window does.
+        // SKIP (quantized caches) leaves them out: the first `head` units are the prefix's, the others begin where the tile's first row's window does (12.5 and 69 us).
         if (p.window > 0 && t.prefix > 0 && n0 >= p.window) {
             t.head = (t.prefix + UK - 1) / UK;
             // Where the window begins behind the keys (lengths past the table's capacity), up to their end: the units are then the prefix's.
