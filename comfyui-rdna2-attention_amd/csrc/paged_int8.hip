@@ -831,7 +831,7 @@ __global__ __launch_bounds__(256, 2) void rows8_kernel(Attn8Args p) {
 //   is scaled, and move vm (to twice the scale: O is then seldom rescaled).
 //
 // A chunk of 2048 tokens over 14336 keys, 32 heads over 8 of 128: 612 us and 15 of the merge in a kernel trace of 400 calls once the clock has settled (695 in the first 40,
-// up to 830 from an idle GPU), whole calls 618 to 640 by the box, 0.80 to 0.83 PFLOP/s, 62 to 64% of a library product of 8192^3. The 16-bit cache takes 564 over normal values, 604 over those
+// up to 830 from an idle GPU), whole calls 615 to 640 by the box, 0.80 to 0.83 PFLOP/s, 62 to 64% of a library product of 8192^3. The 16-bit cache takes 564 over normal values, 604 over those
 // that these codes stand for. Products take 37% of the cycles and vector work 56% (ten instructions a product, where the 16-bit kernel has five: widening, scales), which add up on a SIMD. Two workgroups a CU: at three the registers
 // spill (1920 us). Widening at the start of a step 655, beside the products and two tiles ahead 619; V read ahead of the look at P no faster. With D = 64, half the
 // products beside the same vector work, 414 (16-bit: 312).
